@@ -3,6 +3,7 @@ rotary positions, attention over a shared prefix, token log probabilities.
 
 `run` computes a case in its plain form (elementary torch operations in 32 bits, 64 for angles), or, where `own`
 is true, through this repository's operators; `exact` computes it in 64 bits from the definition."""
+import functools
 import math
 import os
 import sys
@@ -16,6 +17,7 @@ DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 PAGE, DIM = 32, 128  # the paged pool's tokens per page and head size
 
 
+@functools.lru_cache(maxsize=None)
 def _ops():
     """This repository's operators, from its package folder as the benchmark finds it."""
     at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "wrinklefree-inference-engine_amd", "python")
