@@ -793,7 +793,7 @@ __device__ __forceinline__ uint4 fp8x8_to_bf16(uint2 r) {
 }
 // int8 K/V caches (the reference's default KVCacheDtype.INT8, kv_cache/kv_cache.py:159-218, with a
 // static per-layer scale): a fragment is 8 signed codes (8 bytes per lane), widened exactly -- each
-// byte biased to unsigned (xor 0x80), v_cvt_f32_ubyteN, -128 (packed), then bf16 (|code| <= 127 is
+// byte biased to unsigned (xor 0x80), v_cvt_f32_ubyteN, -128, then bf16 (|code| <= 127 is
 // exact in bf16). Scales folded like FP8's.
 #ifndef WF_I8_PK  // 0: the round-5 form (hipcc folds the -128 into an integer subtract: SDWA + v_cvt_f32_i32)
 #define WF_I8_PK 1
@@ -802,7 +802,7 @@ __device__ __forceinline__ uint32_t i8x2_to_bf16(uint32_t u, int sh) {
     const float lo = (float)((u >> sh) & 0xffu) - 128.0f, hi = (float)((u >> (sh + 8)) & 0xffu) - 128.0f;
     return pk_bf16(lo, hi);
 }
-// four biased bytes -> floats (v_cvt_f32_ubyte0..3), -128 on pairs (v_pk_add_f32), packed to bf16
+// four biased bytes -> floats (v_cvt_f32_ubyte0..3), -128 on pairs (scalar adds in this build), packed to bf16
 __device__ __forceinline__ uint2 i8x4_to_bf16_pk(uint32_t x) {
     typedef float f2 __attribute__((ext_vector_type(2)));
     f2 a = {(float)(x & 0xffu), (float)((x >> 8) & 0xffu)};
@@ -1462,7 +1462,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_prefill_sdpa(const uint16_t* __
                 // sequential adds per 512-key block instead of 256 (the one long fp32 chain of the kernel;
                 // it moved 2x the decode kernel's share of outputs off the oracle)
                 float ee[16];
-                if (bs - blk0 + 32 <= vmin) {  // packed fp32 pairs (v_pk_mul / v_pk_add / v_pk_fma)
+                if (bs - blk0 + 32 <= vmin) {  // fp32 pairs (scalar ops in this build)
                     const f32x2_t sc2 = {scale, scale}, m2 = {m_run, m_run};
     #pragma unroll
                     for (int j = 0; j < 16; j += 2) {

@@ -550,8 +550,7 @@ struct EpiDec {
     }
     // GU: act = bf16(bf16(relu(g)^2) * u) of the fragment's rows, quad-transposed: lane (quad k <
     // 2, qi) gets row 4q + qi, act columns 4k .. 4k + 3 of the fragment's 8, as 4 packed bf16
-    // (rows in pairs through the packed-fp32 VALU: v_pk_mul_f32 / v_pk_add_f32 round each lane like
-    // the scalar ops, so the float sequence of corrected() and the activation is unchanged)
+    // (rows in pairs; the build compiles pairs to scalar fp32 ops, which round alike, so the float sequence of corrected() and the activation is unchanged)
     __device__ __forceinline__ uint2 gu_pack(const v4i_t& acc, const EpiIn& in, int l16) const {
         typedef float f2 __attribute__((ext_vector_type(2)));
         const GemvArgs& g = *a;

@@ -96,8 +96,8 @@ __device__ __forceinline__ uint2 quad_transpose_pk(uint32_t A, uint32_t B, int q
 }
 
 // Two rows of one 16 x 16 accumulator column through the reference correction
-// (direct_inference_full.py:201-208: fl32(fl32(S ws) - fl32(ws asum)) * s) on the packed-fp32 VALU
-// (v_pk_mul_f32 / v_pk_add_f32 round each lane like the scalar ops), returned as a bf16 pair.
+// (direct_inference_full.py:201-208: fl32(fl32(S ws) - fl32(ws asum)) * s) on fp32 pairs (the build
+// compiles them to scalar ops: packed fp32 instructions are off), returned as a bf16 pair.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t corrected_pk(int s0, int s1, float ws, int a0, int a1, float f0, float f1) {
     const f32x2_t W = {ws, ws};
@@ -261,8 +261,8 @@ __device__ __forceinline__ uint2 quant8(const float (&x)[8], float sf, float inv
     return make_uint2(lo, hi);
 }
 
-// quant8 of eight packed bf16 values on fp32 pairs: v_pk_mul_f32 / v_pk_fma_f32 / v_pk_add_f32
-// round each lane exactly as the scalar ops do, so the codes and the sum are quant8's.
+// quant8 of eight packed bf16 values on fp32 pairs, which the build compiles to
+// scalar ops, so the codes and the sum are quant8's.
 __device__ __forceinline__ uint2 quant8_bf16x8(uint4 v, float sf, float inv, int& asum) {
     const f32x2_t S = {sf, sf}, I = {inv, inv}, G = {12582912.0f, 12582912.0f};
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
