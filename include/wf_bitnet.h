@@ -167,6 +167,44 @@ int wf_decode_attention(const void* q, int q_dtype, int64_t q_sb, int64_t q_sh, 
                         int B, int Hq, int Hkv, int D, int S, const int32_t* seq_lens, float sm_scale, void* out,
                         int out_dtype, int64_t o_sb, int64_t o_sh, void* ws, void* stream);
 
+/* ---- serving operators around the paged decode path ------------------------------------------ */
+/* Block tables and slot maps from request lengths. Sequence b holds cached_lens[b] tokens on pages of
+ * page_size tokens listed in row b of page_table ([B][max_blocks] int32 at table_stride) and gets
+ * new_lens[b] more (negative lengths count as 0). The pages it lacks are taken from free_pages in sequence
+ * order and written behind the ones it has; no other entry of the table is touched. Token i of sequence b
+ * (tokens in sequence order, num_tokens entries in each output):
+ *   rows = b, positions = cached + i, pages = its table row's entry, slots = position mod page_size.
+ * Entries behind the last token are -1. cu_tokens [B + 1]: where each sequence's tokens begin. counts [4]:
+ * tokens, pages needed, pages taken (the first counts[2] of free_pages are in use now), sequences refused. A
+ * sequence is refused whole -- table row untouched, pages = slots = -1 -- when its tokens do not fit the row
+ * or free_pages ends before its last page. ws: wf_kv_page_plan_ws_bytes(B) bytes (0 for ordinary batches). */
+int64_t wf_kv_page_plan_ws_bytes(int B);
+int wf_kv_page_plan(const int32_t* cached_lens, const int32_t* new_lens, int B, const int32_t* free_pages, int num_free,
+                    int32_t* page_table, int64_t table_stride, int max_blocks, int page_size, int num_tokens, int32_t* pages,
+                    int32_t* slots, int32_t* rows, int32_t* positions, int32_t* cu_tokens, int32_t* counts, void* ws,
+                    void* stream);
+/* Rotary positions on rows of q [T][Hq][D] and k [T][Hk][D] (token stride *_st, head stride *_sh in elements, the
+ * head's dims contiguous; dtype F32 / BF16 / F16; Hq or Hk may be 0): pair j < rotary_dim / 2 of a head is turned by
+ * positions[t] * freqs[j] radians and scaled by `scale`; pairs are dims (j, j + rotary_dim / 2), or (2j, 2j + 1) if
+ * interleaved; dims >= rotary_dim are copied. positions: int32, or int64 if positions64. freqs: float64 (the angle
+ * is formed in 64 bits: positions may be far). Outputs may be the inputs themselves (same pointer and strides),
+ * and must not overlap them otherwise. D <= 512. */
+int wf_rotary_embed(const void* q, int64_t q_st, int64_t q_sh, int Hq, const void* k, int64_t k_st, int64_t k_sh, int Hk, int dtype,
+                    const void* positions, int positions64, const double* freqs, int T, int D, int rotary_dim, int interleaved,
+                    float scale, void* q_out, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh, void* stream);
+/* Log probabilities from logits [R][V] (row stride ld; F32 / BF16 / F16), natural log, float32 out:
+ *   tokens [R] (int32, or int64 if tokens64; NULL: none): logprobs[r] = log softmax(row r)[tokens[r]] and ranks[r] = 1 + the
+ *     number of logits that come before it (greater, or equal at a lower index). A negative token asks for nothing
+ *     (logprob 0, rank 0); one >= V gives NaN and rank 0;
+ *   entropy [R] (NULL: not wanted): -sum p log p;
+ *   top_k in [0, 64], <= V: top_ids / top_logprobs [R][top_k], greatest first, equal ones by index.
+ * A row whose logits are all -inf has log probabilities -inf and entropy 0. A row that holds NaN or +inf has NaN
+ * for every log probability and its entropy; NaN logits are no alternatives (id -1 where fewer than top_k others
+ * are left). ws: wf_token_logprobs_ws_bytes(R, V, top_k) bytes, 16-byte aligned. */
+int64_t wf_token_logprobs_ws_bytes(int R, int V, int top_k);
+int wf_token_logprobs(const void* logits, int dtype, int64_t ld, int R, int V, const void* tokens, int tokens64, int top_k,
+                      float* logprobs, int32_t* ranks, float* entropy, int32_t* top_ids, float* top_logprobs, void* ws, void* stream);
+
 /* ---- SGLang BitNet linear method, MSB-interleaved layout ------------------- */
 /* Layout (sglang_backend/bitnet_quantization.py:99-105, :128-133): byte j of row n =
  * code(w[4j])<<6 | code(w[4j+1])<<4 | code(w[4j+2])<<2 | code(w[4j+3]), code = w + 1.        */

@@ -1,0 +1,139 @@
+"""Serving operators, host side: the C entry points' refusals (no kernel is launched: every call here returns before
+one), the Python wrappers' refusals, and rotary_frequencies against its formulas."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+BUF = (C.c_uint8 * 4096)()
+P = (C.addressof(BUF) + 255) // 256 * 256  # a host address: never read, every call below is refused
+
+
+def refused(name, args, text):
+    from wfamd import _lib
+    lib = _lib.load()
+    assert getattr(lib, name)(*args) == _lib.WF_EINVAL
+    assert text in lib.wf_last_error().decode(), lib.wf_last_error()
+
+
+def test_page_plan_refusals():
+    good = dict(c=P, n=P, B=4, free=P, F=8, table=P, ts=16, cols=16, page=32, T=8, pages=P, slots=P, rows=P, pos=P, cu=P, counts=P,
+                ws=None, st=None)
+
+    def call(text, **kw):
+        refused("wf_kv_page_plan", list({**good, **kw}.values()), text)
+    call("negative", B=-1)
+    call("negative", F=-1)
+    call("negative", T=-1)
+    call("page_size", page=0)
+    call("page_size", page=65537)
+    call("stride", ts=15)
+    call("2^31", ts=1 << 30, cols=1 << 27)
+    call("null cu_tokens", cu=None)
+    call("null cu_tokens", counts=None)
+    call("null lengths", n=None)
+    call("null lengths", table=None)
+    call("free list", free=None)
+    call("token arrays", slots=None)
+    call("too many tokens", T=0x7fffffff)
+    call("workspace", B=100000)
+
+
+def test_rotary_refusals():
+    good = dict(q=P, qst=512, qsh=128, hq=4, k=P, kst=128, ksh=128, hk=1, dt=1, pos=P, p64=0, f=P, T=2, D=128, r=128, inter=0, s=1.0,
+                qo=P, qost=512, qosh=128, ko=P, kost=128, kosh=128, st=None)
+
+    def call(text, **kw):
+        refused("wf_rotary_embed", list({**good, **kw}.values()), text)
+    call("dtype", dt=3)
+    call("negative", T=-1)
+    call("negative", hq=-1)
+    call("head_dim", D=0)
+    call("head_dim", D=513, r=64)
+    for r in (0, 7, 130, -2):
+        call("rotary_dim", r=r)
+    call("null", q=None)
+    call("null", ko=None)
+    call("null", f=None)
+    call("null", pos=None)
+    from wfamd import _lib
+    lib = _lib.load()
+    assert lib.wf_rotary_embed(*{**good, "T": 0}.values()) == _lib.WF_OK  # nothing to do, nothing launched
+    assert lib.wf_rotary_embed(*{**good, "hq": 0, "hk": 0}.values()) == _lib.WF_OK
+
+
+def test_token_logprobs_refusals():
+    good = dict(x=P, dt=1, ld=100, R=2, V=100, tok=P, t64=0, k=5, lp=P, rank=P, ent=P, ids=P, top=P, ws=P, st=None)
+
+    def call(text, **kw):
+        refused("wf_token_logprobs", list({**good, **kw}.values()), text)
+    call("dtype", dt=4)
+    call("shape", V=0)
+    call("shape", R=-1)
+    call("shape", V=(1 << 30) + 1)
+    call("top_k", k=65)
+    call("top_k", k=-1)
+    call("top_k", V=4, ld=4)
+    call("stride", ld=99)
+    call("null logits", x=None)
+    call("null logits", ws=None)
+    call("not 16-byte", ws=P + 8)
+    call("logprobs / ranks", rank=None)
+    call("top_ids", ids=None)
+    from wfamd import _lib
+    lib = _lib.load()
+    assert lib.wf_token_logprobs(*{**good, "R": 0}.values()) == _lib.WF_OK
+    assert lib.wf_token_logprobs_ws_bytes(0, 100, 5) == 0 and lib.wf_token_logprobs_ws_bytes(3, 100, 5) >= 3 * (16 + 40)
+
+
+def test_python_wrappers_refuse_host_tensors():
+    from wfamd import ops
+    i = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="device tensors only"):
+        ops.kv_page_plan(i, i, i, torch.zeros(4, 4, dtype=torch.int32), 4)
+    q = torch.zeros(4, 2, 64)
+    with pytest.raises(ValueError, match="device tensors only"):
+        ops.rotary_embed(q, None, i, torch.zeros(32, dtype=torch.float64))
+    with pytest.raises(ValueError, match="device tensors only"):
+        ops.token_logprobs(torch.zeros(4, 10))
+
+
+def test_no_overlap():
+    from wfamd.ops import _no_overlap
+    assert _no_overlap(torch.zeros(4, 3, 8)) and _no_overlap(torch.zeros(4, 6, 8)[:, 1:3]) and _no_overlap(torch.zeros(3, 4, 8).transpose(0, 1))
+    assert not _no_overlap(torch.zeros(1, 3, 8).expand(4, 3, 8)) and not _no_overlap(torch.zeros(100).as_strided((3, 2, 8), (4, 8, 1)))
+    assert _no_overlap(torch.zeros(1, 1, 8).expand(1, 1, 8))
+
+
+@pytest.mark.parametrize("r", [2, 4, 64, 80, 128])
+def test_rotary_frequencies(r):
+    from wfamd.ops import rotary_frequencies
+    f, s = rotary_frequencies(r, 500000.0, device="cpu")
+    assert f.dtype == torch.float64 and s == 1.0
+    for j in range(r // 2):
+        assert f[j].item() == pytest.approx(500000.0 ** (-2 * j / r), rel=1e-14)
+    lin, s = rotary_frequencies(r, 500000.0, scaling="linear", factor=8.0, device="cpu")
+    assert torch.equal(lin, f / 8) and s == 1.0
+    ntk, s = rotary_frequencies(r, 500000.0, scaling="ntk", factor=8.0, device="cpu")
+    assert ntk[0] == 1.0 and s == 1.0
+    if r > 2:
+        assert ntk[-1].item() == pytest.approx(f[-1].item() / 8, rel=1e-12)  # the lowest frequency: as 'linear'
+    yarn, s = rotary_frequencies(r, 500000.0, scaling="yarn", factor=8.0, original_max_position=4096, device="cpu")
+    assert s == pytest.approx(0.1 * math.log(8) + 1)
+    turns = f * 4096 / (2 * math.pi)
+    assert ((yarn <= f * (1 + 1e-15)) & (yarn >= f / 8 * (1 - 1e-15))).all()
+    if r >= 64:
+        # a pair and more away from the ramp's rounded ends
+        assert torch.equal(yarn[:-1][turns[1:] > 32], f[:-1][turns[1:] > 32])
+        assert torch.allclose(yarn[1:][turns[:-1] < 1], f[1:][turns[:-1] < 1] / 8, rtol=1e-14, atol=0)
+
+
+def test_rotary_frequencies_refusals():
+    from wfamd.ops import rotary_frequencies
+    for a, kw in (((7,), {}), ((0,), {}), ((64, 1.0), {}), ((64,), {"factor": 0.5, "scaling": "linear"}), ((64,), {"scaling": "x"}),
+                  ((64,), {"scaling": "yarn", "factor": 2.0}),
+                  ((64,), {"scaling": "yarn", "factor": 2.0, "original_max_position": 64, "beta_fast": 1.0, "beta_slow": 1.0}),
+                  ((64,), {"scaling": "yarn", "factor": 2.0, "original_max_position": 64, "beta_slow": 0.0})):
+        with pytest.raises(ValueError):
+            rotary_frequencies(*a, device="cpu", **kw)

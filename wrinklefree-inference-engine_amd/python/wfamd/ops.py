@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import List, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -402,6 +402,205 @@ def decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_st
          kv_strides[0], kv_strides[1], kv_strides[2], float(k_scale), float(v_scale), B, Hq, Hkv, D, S,
          _ptr(seq_lens), sm, out.data_ptr(), _DT[out_dtype], Hq * D, D, ws.data_ptr(), _stream())
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# Serving operators around the paged decode path: page plans, rotary positions, log probabilities.
+# Device tensors only, all on one device; they run on that device's current stream.
+# ---------------------------------------------------------------------------------------------
+def _serve_args(name: str, dev: torch.device, **tensors) -> None:
+    """ValueError unless every tensor is on `dev`, a HIP device."""
+    for what, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: {what} is on {t.device}, expected one HIP device ({dev})")
+    if dev.type != "cuda":
+        raise ValueError(f"{name}: device tensors only, got {dev}")
+
+
+def _int32_rows(name: str, what: str, t: torch.Tensor, n: Optional[int] = None) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
+        raise ValueError(f"{name}: {what} must be a contiguous int32 [{'n' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """Launch on dev's current stream, with dev current (kernels go to the device that is current)."""
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+        return
+    with torch.cuda.device(dev):
+        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+class KVPagePlan(NamedTuple):
+    """Where the new tokens of a batch go (kv_page_plan); int32 on the device. Entries of the four token arrays
+    behind the last token are -1."""
+    pages: torch.Tensor       # [num_tokens] page of each token (-1: its sequence was refused)
+    slots: torch.Tensor       # [num_tokens] place within the page
+    rows: torch.Tensor        # [num_tokens] sequence of each token
+    positions: torch.Tensor   # [num_tokens] position in the sequence
+    cu_tokens: torch.Tensor   # [B + 1] where each sequence's tokens begin
+    counts: torch.Tensor      # [4] tokens, pages needed, pages taken, sequences refused
+
+
+def kv_page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor, page_table: torch.Tensor,
+                 num_tokens: int, *, page_size: int = 32) -> KVPagePlan:
+    """Block tables and slot maps from request lengths, without the host (include/wf_bitnet.h wf_kv_page_plan):
+    sequence b holds cached_lens[b] tokens and gets new_lens[b] more; the pages it lacks are taken from
+    free_pages (int32 ids, in order) and written into its row of page_table [B, blocks] (in place). num_tokens
+    sizes the token arrays (the sum of new_lens, or a bound). `pages` / `slots` are what KVCacheManager.scatter_kv
+    takes. The first counts[2] of free_pages are in use afterwards; a sequence that does not fit its table row or
+    the free list is refused whole (counts[3]) and its tokens have page -1."""
+    dev = cached_lens.device
+    _serve_args("kv_page_plan", dev, new_lens=new_lens, free_pages=free_pages, page_table=page_table)
+    _int32_rows("kv_page_plan", "cached_lens", cached_lens)
+    b = cached_lens.shape[0]
+    _int32_rows("kv_page_plan", "new_lens", new_lens, b)
+    _int32_rows("kv_page_plan", "free_pages", free_pages)
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != b or (
+            b and page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"kv_page_plan: page_table must be int32 [{b}, blocks] with contiguous rows, got {page_table.dtype} "
+                         f"{tuple(page_table.shape)}")
+    n, cols = int(num_tokens), page_table.shape[1]
+    if n < 0:
+        raise ValueError(f"kv_page_plan: num_tokens {n} is negative")
+    pad = (n + 3) // 4 * 4  # 16-byte steps between the arrays
+    out = torch.empty(4 * pad + b + 5, dtype=torch.int32, device=dev)
+    pages, slots, rows, pos, cu, counts = (out[i:i + m] for i, m in (
+        (0, n), (pad, n), (2 * pad, n), (3 * pad, n), (4 * pad + 4, b + 1), (4 * pad, 4)))
+    nws = int(_lib.load().wf_kv_page_plan_ws_bytes(b))
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    base = out.data_ptr()
+    _call_on(dev, "wf_kv_page_plan", cached_lens.data_ptr(), new_lens.data_ptr(), b, free_pages.data_ptr(), free_pages.shape[0],
+             page_table.data_ptr(), max(page_table.stride(0), cols) if b < 2 else page_table.stride(0), cols, int(page_size), n, base,
+             base + 4 * pad, base + 8 * pad, base + 12 * pad, base + 16 * pad + 16, base + 16 * pad, _ptr(ws))
+    return KVPagePlan(pages, slots, rows, pos, cu, counts)
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
+                       original_max_position: Optional[int] = None, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                       device=None) -> Tuple[torch.Tensor, float]:
+    """(freqs, scale) for rotary_embed: base^(-2j / rotary_dim) radians a position in float64 [rotary_dim / 2], for
+    contexts `factor` times the trained one by
+      'linear': every frequency divided by factor (position interpolation);
+      'ntk':    a larger base, base * factor^(r / (r - 2)): the lowest frequency is divided by factor, the highest kept;
+      'yarn':   pairs that turn more than beta_fast times over original_max_position keep their frequency, those that turn
+                less than beta_slow times have it divided by factor, a linear ramp over the pairs between; scale =
+                0.1 ln(factor) + 1 on the rotated values."""
+    r = int(rotary_dim)
+    if r <= 0 or r % 2:
+        raise ValueError(f"rotary_frequencies: rotary_dim {r} must be even and positive")
+    if not base > 1.0 or not factor >= 1.0:
+        raise ValueError(f"rotary_frequencies: base {base} must be > 1 and factor {factor} >= 1")
+    scale = 1.0
+    if scaling == "ntk" and r > 2:
+        base = base * factor ** (r / (r - 2))
+    f = base ** (-torch.arange(0, r, 2, dtype=torch.float64) / r)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        if not original_max_position or original_max_position < 1 or not beta_fast > beta_slow > 0:
+            raise ValueError("rotary_frequencies: 'yarn' needs original_max_position >= 1 and beta_fast > beta_slow > 0")
+        # the (real) pair that turns n times over the trained context: base^(-2j / r) * length = 2 pi n
+        pair = [r * math.log(original_max_position / (n * 2 * math.pi)) / (2 * math.log(base)) for n in (beta_fast, beta_slow)]
+        lo, hi = max(math.floor(pair[0]), 0), min(math.ceil(pair[1]), r - 1)
+        ramp = ((torch.arange(r // 2, dtype=torch.float64) - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
+        f = f / factor * ramp + f * (1.0 - ramp)
+        scale = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"rotary_frequencies: unknown scaling {scaling!r} (None, 'linear', 'ntk', 'yarn')")
+    return f.to(_device() if device is None else device), scale
+
+
+def _rotary_rows(what: str, t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or t.dtype != like.dtype:
+        raise ValueError(f"rotary_embed: {what} must be [tokens, heads, head_dim] like q in tokens, head_dim and dtype, got "
+                         f"{t.dtype} {tuple(t.shape)}")
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def _no_overlap(t: torch.Tensor) -> bool:
+    """No element of a strided tensor shares its place with another (sizes 1 aside)."""
+    reach = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st < reach:
+            return False
+        reach = st * (n - 1) + reach
+    return True
+
+
+def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, *,
+                 interleaved: bool = False, scale: float = 1.0, inplace: bool = False):
+    """Rotary positions on q [T, Hq, D] and k [T, Hk, D] (or None), bf16 / f16 / f32, any token and head strides
+    (include/wf_bitnet.h wf_rotary_embed). positions [T] int32 or int64; freqs, scale from rotary_frequencies: the first
+    2 len(freqs) dims of a head are turned, the rest copied. Returns (q, k) turned: new tensors, or with
+    inplace=True the given ones. Each result is rounded once, from 32 bits; the angle is formed in 64."""
+    dev = q.device
+    _serve_args("rotary_embed", dev, q=q, k=k, positions=positions, freqs=freqs)
+    code = _dtcode(q)
+    if inplace:
+        for what, t in (("q", q), ("k", k)):
+            if t is not None and t.numel() and ((t.stride(-1) != 1 and t.shape[-1] > 1) or not _no_overlap(t)):
+                raise ValueError(f"rotary_embed: {what} of strides {t.stride()} cannot be turned in place")
+        if k is not None and k.numel() and k.data_ptr() == q.data_ptr():
+            raise ValueError("rotary_embed: q and k are the same memory, turned in place it would be turned twice")
+    q = _rotary_rows("q", q, q)
+    T, Hq, D = q.shape
+    Hk = 0
+    if k is not None:
+        k = _rotary_rows("k", k, q)
+        Hk = k.shape[1]
+    if positions.dim() != 1 or positions.shape[0] != T or positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous():
+        raise ValueError(f"rotary_embed: positions must be a contiguous int32 or int64 [{T}], got {positions.dtype} {tuple(positions.shape)}")
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or not 0 < 2 * freqs.shape[0] <= D:
+        raise ValueError(f"rotary_embed: freqs must be a contiguous float64 [n], 0 < 2 n <= {D}, got {freqs.dtype} {tuple(freqs.shape)}")
+    qo = q if inplace else torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    ko = k if inplace or k is None else torch.empty((T, Hk, D), dtype=q.dtype, device=dev)
+    kk, kko = (q, qo) if k is None else (k, ko)
+    _call_on(dev, "wf_rotary_embed", q.data_ptr(), q.stride(0), q.stride(1), Hq, kk.data_ptr(), kk.stride(0), kk.stride(1), Hk, code,
+             positions.data_ptr(), int(positions.dtype == torch.int64), freqs.data_ptr(), T, D, 2 * freqs.shape[0], int(interleaved),
+             float(scale), qo.data_ptr(), qo.stride(0), qo.stride(1), kko.data_ptr(), kko.stride(0), kko.stride(1))
+    return qo, ko
+
+
+class TokenLogprobs(NamedTuple):
+    """token_logprobs' results on the device (float32 / int32); logprobs and ranks are None without tokens."""
+    logprobs: Optional[torch.Tensor]  # [R] log probability of the row's token
+    ranks: Optional[torch.Tensor]     # [R] 1 = the most likely
+    entropy: torch.Tensor             # [R]
+    top_ids: torch.Tensor             # [R, top_k]
+    top_logprobs: torch.Tensor        # [R, top_k]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top_k: int = 0) -> TokenLogprobs:
+    """Log probability and rank of one given token a row, the row's entropy and its top_k (<= 64) alternatives,
+    from logits [R, V] bf16 / f16 / f32 read once (include/wf_bitnet.h wf_token_logprobs, which also says what rows of
+    -inf, NaN or +inf give). tokens [R] int32 or int64; a negative one asks for nothing. Equal logits rank by index."""
+    dev = logits.device
+    _serve_args("token_logprobs", dev, logits=logits, tokens=tokens)
+    code = _dtcode(logits)
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"token_logprobs: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
+    R, V = logits.shape
+    k = int(top_k)
+    if not 0 <= k <= min(64, V):
+        raise ValueError(f"token_logprobs: top_k {k} not in [0, {min(64, V)}]")
+    if V > 1 and logits.stride(1) != 1 or R > 1 and logits.stride(0) < V:
+        logits = logits.contiguous()
+    if tokens is not None and (tokens.dim() != 1 or tokens.shape[0] != R or tokens.dtype not in (torch.int32, torch.int64)
+                               or not tokens.is_contiguous()):
+        raise ValueError(f"token_logprobs: tokens must be a contiguous int32 or int64 [{R}], got {tokens.dtype} {tuple(tokens.shape)}")
+    lp = rank = None
+    if tokens is not None:
+        lp = torch.empty(R, dtype=torch.float32, device=dev)
+        rank = torch.empty(R, dtype=torch.int32, device=dev)
+    ent = torch.empty(R, dtype=torch.float32, device=dev)
+    ids = torch.empty((R, k), dtype=torch.int32, device=dev)
+    top = torch.empty((R, k), dtype=torch.float32, device=dev)
+    ws = torch.empty(int(_lib.load().wf_token_logprobs_ws_bytes(R, V, k)), dtype=torch.uint8, device=dev)
+    _call_on(dev, "wf_token_logprobs", logits.data_ptr(), code, logits.stride(0), R, V, _ptr(tokens),
+             int(tokens is not None and tokens.dtype == torch.int64), k, _ptr(lp), _ptr(rank), ent.data_ptr(), ids.data_ptr(),
+             top.data_ptr(), ws.data_ptr())
+    return TokenLogprobs(lp, rank, ent, ids, top)
 
 
 # ---------------------------------------------------------------------------------------------
