@@ -192,6 +192,28 @@ int wf_kv_page_plan(const int32_t* cached_lens, const int32_t* new_lens, int B, 
 int wf_rotary_embed(const void* q, int64_t q_st, int64_t q_sh, int Hq, const void* k, int64_t k_st, int64_t k_sh, int Hk, int dtype,
                     const void* positions, int positions64, const double* freqs, int T, int D, int rotary_dim, int interleaved,
                     float scale, void* q_out, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh, void* stream);
+/* Attention of one query token per sequence over the paged pool, for a batch whose sequences share a prefix:
+ *   out[b, h] = softmax(sm_scale q[b, h] . K) V over the keys j < seq_lens[b] of kv head h / (Hq / Hkv),
+ * keys j < prefix_lens[b] on the pages of row prefix_rows[b] of page_table, the others on row b (prefix_rows[b]
+ * outside [0, B): no prefix). Sequences next to each other in the batch with the same prefix_rows and prefix_lens
+ * (both cut at seq_lens) have the prefix read once for all of them; any other arrangement is as exact, without the
+ * saving. The prefix need not end with a page.
+ *   q, out : [B][Hq][128] (strides *_sb, *_sh in elements; dtype F32 / BF16 / F16); lse (NULL: not wanted): [B][Hq]
+ *            float32, the natural log of the sum of exp(score);
+ *   k_pool, v_pool : one layer of the engine's paged pool: page p, kv head h at p * page_stride + h * head_stride
+ *            elements, 32 tokens in the K / V tile layouts of wf_model_desc.k_cache; kv_quant WF_KV_*, one-byte codes
+ *            stand for code * k_scale / code * v_scale; 16-byte aligned, strides multiples of 16 bytes;
+ *   page_table [B][max_blocks] int32 (row stride table_stride). Lengths are cut at 32 * max_blocks. Keys on page ids
+ *            outside [0, num_pages) count as absent.
+ * A sequence without keys, or without a score above -inf, gives zeros and lse -inf. max_blocks also sizes the launch: a
+ * table much wider than the sequences are long costs some idle workgroups.
+ * ws: wf_shared_prefix_attention_ws_bytes(dtype, B, Hq, Hkv, max_blocks) bytes, 16-byte aligned. */
+int64_t wf_shared_prefix_attention_ws_bytes(int dtype, int B, int Hq, int Hkv, int max_blocks);
+int wf_shared_prefix_attention(const void* q, int dtype, int64_t q_sb, int64_t q_sh, const void* k_pool, const void* v_pool, int kv_quant,
+                               int64_t page_stride, int64_t head_stride, int num_pages, const int32_t* page_table,
+                               int64_t table_stride, int max_blocks, const int32_t* seq_lens, const int32_t* prefix_rows,
+                               const int32_t* prefix_lens, float k_scale, float v_scale, float sm_scale, int B, int Hq, int Hkv, int D,
+                               void* out, int64_t o_sb, int64_t o_sh, float* lse, void* ws, void* stream);
 /* Log probabilities from logits [R][V] (row stride ld; F32 / BF16 / F16), natural log, float32 out:
  *   tokens [R] (int32, or int64 if tokens64; NULL: none): logprobs[r] = log softmax(row r)[tokens[r]] and ranks[r] = 1 + the
  *     number of logits that come before it (greater, or equal at a lower index). A negative token asks for nothing

@@ -137,3 +137,37 @@ def test_rotary_frequencies_refusals():
                   ((64,), {"scaling": "yarn", "factor": 2.0, "original_max_position": 64, "beta_slow": 0.0})):
         with pytest.raises(ValueError):
             rotary_frequencies(*a, device="cpu", **kw)
+
+
+def test_shared_prefix_attention_refusals():
+    good = dict(q=P, dt=1, qsb=512, qsh=128, k=P, v=P, kvq=0, pgs=4096, hs=4096, pages=4, pt=P, pts=8, cols=8, lens=P, rows=P, plens=P,
+                ks=1.0, vs=1.0, sm=0.1, B=2, hq=4, hkv=1, D=128, out=P, osb=512, osh=128, lse=None, ws=P, st=None)
+
+    def call(text, **kw):
+        refused("wf_shared_prefix_attention", list({**good, **kw}.values()), text)
+    call("dtype", dt=3)
+    call("kv_quant", kvq=3)
+    call("head_dim 128", D=64)
+    call("bad heads", hq=5, hkv=2)
+    call("bad heads", hkv=0)
+    call("bad heads", B=-1)
+    call("too many", B=65536)
+    call("too many", B=60000, hq=64)
+    call("bad pool or table", pages=0)
+    call("bad pool or table", cols=0)
+    call("bad pool or table", pts=7)
+    call("bad pool or table", cols=1 << 27, pts=1 << 27)
+    call("strides", pgs=4100)
+    call("strides", hs=-4096)
+    call("strides", kvq=1, hs=4104)
+    for kw in ({"sm": 0.0}, {"ks": 0.0}, {"sm": float("inf")}, {"ks": float("nan")}):
+        call("finite, not 0", **kw)
+    for p in ("q", "k", "v", "pt", "lens", "rows", "plens", "out", "ws"):
+        call("null pointer", **{p: None})
+    call("aligned", k=P + 8)
+    call("aligned", ws=P + 4)
+    from wfamd import _lib
+    lib = _lib.load()
+    assert lib.wf_shared_prefix_attention(*{**good, "B": 0}.values()) == _lib.WF_OK
+    assert lib.wf_shared_prefix_attention_ws_bytes(1, 0, 4, 1, 8) == 0 and lib.wf_shared_prefix_attention_ws_bytes(1, 2, 4, 3, 8) == 0
+    assert lib.wf_shared_prefix_attention_ws_bytes(1, 2, 4, 1, 8) >= 2 * 4 * 2 * 520

@@ -1,0 +1,493 @@
+// wf_prefix.hip -- attention of one query token per sequence over the paged K/V pool, for batches whose
+// sequences share a prefix: the prefix's keys are read once for all of them.
+//
+// Sequence b has L keys. Keys j < P stand on the pages of another row of the page table (the prefix's owner), the
+// others on its own:  o = sum_j p_j v_j / l,  p_j = exp(scale q.k_j - m),  l = sum_j p_j,  lse = m + log l.
+// The softmax splits over any partition of the keys into records (m, l, unnormalised o) that a second launch joins.
+//
+//   k_prefix  keys [0, P) of neighbouring sequences with the same owner and P ("shared"): a workgroup takes up to 64
+//             query rows (sequence, head of the kv group) and a range of the keys; every wave takes every fourth
+//             32-key tile for ALL rows, so a K/V byte is loaded once per 64 rows, straight into registers.
+//   k_suffix  the other keys of a sequence (all of them where it shares with no neighbour): one kv head and a range of
+//             the keys a workgroup, the group's heads as the matrix's columns. Bound by memory.
+//   k_prefix_join  one wave a (sequence, head): its records, the division, the output type.
+//
+// Tiles: the pool's 32-key K / V layouts (wf_norm.h k_tile_off / v_tile_off) are the A operands of
+// v_mfma_f32_16x16x32_bf16 as they lie: S^T (16 keys x 16 rows) = K Q^T, two per tile, whose accumulator leaves
+// lane (row l16, quarter q4) with the scores of keys 8 q4 .. 8 q4 + 7 -- the B operand of O^T (16 dims x 16 rows) =
+// V^T P^T. Probabilities never leave their lane; no LDS and no barrier until the waves' records meet.
+// The running max is raised only when a tile passes it by 2^8 (its exchange between the four lanes of a row and
+// the rescaling of o are rare then): p <= 2^8 is as exact in bf16 and 32 bits as p <= 1.
+//
+// Rounding: scores, max, sums and o in 32 bits. A q of f16 / f32 enters as the exact sum of two / three bf16 terms.
+// P is rounded to bf16 for bf16 outputs (2^-9 a term, as much as the output's own rounding); f16 and f32 outputs take
+// two and three terms of it.
+#include "wf_common.h"
+#include "wf_device.h"
+#include "wf_kv.h"
+
+namespace wf {
+
+typedef __bf16 pf_bf8 __attribute__((ext_vector_type(8)));
+typedef float pf_f4 __attribute__((ext_vector_type(4)));
+
+constexpr int kPfDim = 128, kPfPage = 32;
+constexpr int kPfMaxRecords = 64;          // splits of each part
+constexpr int kPfMinTiles = 4;             // prefix: a tile a wave at least
+constexpr int kPfMinSuffix = 8;            // suffix: two
+constexpr float kPfLn2 = 0.69314718055994530942f;
+
+struct PfArgs {
+    const void* q;
+    int64_t q_sb, q_sh;
+    const uint8_t *K, *V;
+    int64_t pgs, hs;  // bytes from page to page and from head to head
+    int np;
+    const int32_t* pt;
+    int64_t pts;
+    int cols;
+    const int32_t *lens, *owners, *plens;
+    int B, Hq, Hkv, G;
+    float sc, neg;  // |scale| log2e, and the sign that went to q
+    float vs;
+    int NP, NS;     // splits of the prefix and of the suffix; records of a row: NP + NS
+    float2* ml;     // [B * Hq][NP + NS]
+    float* o;       // [B * Hq][NP + NS][128]
+    void* out;
+    int64_t o_sb, o_sh;
+    float* lse;
+};
+
+// A sequence's partition: keys [0, P) on owner's pages, [P, L) on its own.
+struct PfSeq {
+    int L, P, owner;
+    __device__ __forceinline__ bool same(const PfSeq& s) const { return P > 0 && P == s.P && owner == s.owner; }
+};
+__device__ __forceinline__ PfSeq pf_seq(const PfArgs& a, int b) {
+    PfSeq s{0, 0, -1};
+    if (b < 0 || b >= a.B) return s;
+    s.L = min(max(a.lens[b], 0), a.cols * kPfPage);
+    s.owner = a.owners[b];
+    if (s.owner >= 0 && s.owner < a.B) s.P = min(max(a.plens[b], 0), s.L);
+    return s;
+}
+// Whether b's prefix is read together with a neighbour's (all three launches ask this).
+__device__ __forceinline__ bool pf_shared(const PfArgs& a, int b, const PfSeq& s) {
+    return s.same(pf_seq(a, b - 1)) || s.same(pf_seq(a, b + 1));
+}
+// tiles of one of `splits` ranges, and how many ranges hold something
+__device__ __forceinline__ int pf_per(int tiles, int splits, int least) { return max((tiles + splits - 1) / splits, least); }
+__device__ __forceinline__ int pf_tiles(int keys) { return (keys + kPfPage - 1) / kPfPage; }
+
+// 8 elements of a tile's fragment as bf16
+template <int KVQ>
+struct PfFrag {
+    static constexpr int kBytes = KVQ == 0 ? 2 : 1;
+    using T = typename std::conditional<KVQ == 0, uint4, uint2>::type;
+    static __device__ __forceinline__ uint4 bf(T t) {
+        if constexpr (KVQ == 0) return t;
+        else if constexpr (KVQ == 1) return fp8x8_to_bf16(t);
+        else return i8x8_to_bf16(t);
+    }
+};
+
+// NT column tiles of 16 query rows: the q fragments, running max, sum and output of one wave.
+template <int NT, int NQ, int NPT>
+struct PfState {
+    pf_bf8 q[NT][NQ][4];
+    pf_f4 acc[NT][8];
+    float m[NT], f[NT], l[NT];  // max (log2 domain), the frame of the exponents (m, or 0 while it is -inf), sum
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            m[t] = -INFINITY, f[t] = 0.f, l[t] = 0.f;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) acc[t][n] = pf_f4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    // fragment c of tile t's row: dims 32 c + 8 q4 ..
+    template <int QDT>
+    __device__ __forceinline__ void load_q(int t, const void* row, float neg) {
+        const int q4 = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = neg * load_as_f32(row, 32 * c + 8 * q4 + e, QDT);
+#pragma unroll
+            for (int k = 0; k < NQ; ++k) {
+                pf_bf8 v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = (__bf16)x[e];
+                    x[e] -= (float)v[e];
+                }
+                q[t][k][c] = v;
+            }
+        }
+    }
+    // One 32-key tile; keys outside [lo, hi) of it are masked. K and V fragments of this lane.
+    template <int KVQ>
+    __device__ __forceinline__ void tile(const typename PfFrag<KVQ>::T (&kf)[8], const typename PfFrag<KVQ>::T (&vf)[8], int lo, int hi,
+                                         float sc, unsigned live) {
+        const int key = (threadIdx.x & 63) >> 4 << 3;  // this lane's keys: key .. key + 7
+        const bool whole = lo <= 0 && hi >= kPfPage;
+        pf_bf8 kb[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) kb[i] = __builtin_bit_cast(pf_bf8, PfFrag<KVQ>::bf(kf[i]));
+        pf_bf8 p[NT][NPT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (!(live >> t & 1)) continue;
+            pf_f4 s[2] = {pf_f4{0.f, 0.f, 0.f, 0.f}, pf_f4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int k = NQ - 1; k >= 0; --k) {
+                    s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[c], q[t][k][c], s[0], 0, 0, 0);
+                    s[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[4 + c], q[t][k][c], s[1], 0, 0, 0);
+                }
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3];
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = key + e >= lo && key + e < hi ? x[e] : -INFINITY;
+            }
+            float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * sc;
+            if (__any(mx > m[t] + 8.f)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m[t]);
+                const float nf = mx == -INFINITY ? 0.f : mx, r = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(f[t] - nf);
+                // (an empty sum stays, also when it is NaN: it holds no finite score to rescale)
+                if (m[t] != -INFINITY) {
+                    l[t] *= r;
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) acc[t][n] *= r;
+                }
+                m[t] = mx;
+                f[t] = nf;
+            }
+            float e8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) e8[e] = __builtin_amdgcn_exp2f(fmaf(x[e], sc, -f[t]));
+            l[t] += ((e8[0] + e8[1]) + (e8[2] + e8[3])) + ((e8[4] + e8[5]) + (e8[6] + e8[7]));
+#pragma unroll
+            for (int k = 0; k < NPT; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[t][k][e] = (__bf16)e8[e];
+                    if (k + 1 < NPT) e8[e] -= (float)p[t][k][e];
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            uint4 v = PfFrag<KVQ>::bf(vf[n]);
+            if (!whole) {  // a masked key's V may hold anything: 0 x NaN is NaN
+                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int k0 = key + 2 * j;
+                    w[j] &= (k0 >= lo && k0 < hi ? 0xffffu : 0u) | (k0 + 1 >= lo && k0 + 1 < hi ? 0xffff0000u : 0u);
+                }
+                v = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            const pf_bf8 vb = __builtin_bit_cast(pf_bf8, v);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (live >> t & 1)
+#pragma unroll
+                    for (int k = NPT - 1; k >= 0; --k) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p[t][k], acc[t][n], 0, 0, 0);
+        }
+    }
+};
+
+// Where a tile of the walk lies: the pool's block of its page and head, the valid keys of it.
+struct PfAt {
+    int64_t off;  // byte offset; < 0: no such page, every key masked
+    int lo, hi;
+};
+template <int KVQ>
+__device__ __forceinline__ void pf_load(const PfArgs& a, const PfAt& at, typename PfFrag<KVQ>::T (&kf)[8], typename PfFrag<KVQ>::T (&vf)[8]) {
+    using F = PfFrag<KVQ>;
+    if (at.off < 0) return;
+    const int lane = threadIdx.x & 63;
+    const typename F::T* k = reinterpret_cast<const typename F::T*>(a.K + at.off) + lane;
+    const typename F::T* v = reinterpret_cast<const typename F::T*>(a.V + at.off) + lane;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kf[i] = k[64 * i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vf[i] = v[64 * i];
+}
+
+// The four waves' states of one column tile -> one record a row. sm: 4 x 16 rows of 132 floats + 4 x 16 (m, l).
+constexpr int kPfRow = kPfDim + 4;
+struct __attribute__((aligned(16))) PfShared {
+    float o[4][16][kPfRow];
+    float m[4][16], l[4][16];
+};
+// row(i): the record's place in ml / o for row i of the column tile, or < 0
+template <class Row>
+__device__ __forceinline__ void pf_merge(const PfArgs& a, PfShared& sm, const pf_f4 (&acc)[8], float m, float l, Row row) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q4 = lane >> 4;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    __syncthreads();  // the last column tile's record has been read
+#pragma unroll
+    for (int n = 0; n < 8; ++n) *reinterpret_cast<pf_f4*>(&sm.o[wave][l16][16 * n + 4 * q4]) = acc[n];
+    if (q4 == 0) sm.m[wave][l16] = m, sm.l[wave][l16] = l;
+    __syncthreads();
+    // 16 threads a row, 8 dims each
+    const int r = threadIdx.x >> 4, d = (threadIdx.x & 15) * 8;
+    const int64_t rec = row(r);
+    if (rec < 0) return;
+    float M = -INFINITY, w[4], L = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) M = fmaxf(M, sm.m[i][r]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // a wave that saw no finite score has l = 0 (or NaN) in the frame 0
+        w[i] = M == -INFINITY ? 1.f : sm.m[i][r] == -INFINITY ? (sm.l[i][r] == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(sm.m[i][r] - M);
+        L += sm.l[i][r] * w[i];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] += sm.o[i][r][d + e] * w[i];
+    }
+    float* o = a.o + rec * kPfDim + d;
+    *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(o + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    if (d == 0) a.ml[rec] = make_float2(M, L);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Shared prefixes. Grid (kv head and key range, rounded up to 8, tile of 16 NT rows): the row tiles of one (head,
+// range) are 8 k workgroups apart, so one XCD's L2 serves them all.
+// ---------------------------------------------------------------------------------------------
+template <int KVQ, int QDT, int NT>
+__global__ __launch_bounds__(256) void k_prefix(PfArgs a) {
+    constexpr int NQ = QDT == DT_BF16 ? 1 : QDT == DT_F16 ? 2 : 3;
+    using F = PfFrag<KVQ>;
+    __shared__ PfShared sm;
+    if ((int)blockIdx.x >= a.Hkv * a.NP) return;
+    const int h = blockIdx.x % a.Hkv, z = blockIdx.x / a.Hkv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
+    const int64_t r0 = (int64_t)blockIdx.y * (16 * NT), rows = (int64_t)a.B * a.G;
+    const int64_t r1 = min(r0 + 16 * NT, rows);
+    const int b0 = (int)(r0 / a.G), b1 = (int)((r1 - 1) / a.G);  // sequences of the tile: at most 64
+    // lane i: sequence b0 + i
+    const PfSeq me = pf_seq(a, b0 + lane <= b1 ? b0 + lane : -1);
+    const PfSeq before = pf_seq(a, b0 + lane <= b1 ? b0 + lane - 1 : -1), after = pf_seq(a, b0 + lane <= b1 ? b0 + lane + 1 : -1);
+    uint64_t todo = __ballot(me.same(before) || me.same(after));
+    const uint64_t joined = __ballot(me.same(before));
+    if (!todo) return;
+    PfState<NT, NQ, NQ> st;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int64_t r = min(r0 + 16 * t + l16, rows - 1);
+        const int b = (int)(r / a.G), g = (int)(r - (int64_t)b * a.G);
+        const int64_t off = (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2);
+        st.template load_q<QDT>(t, (const uint8_t*)a.q + off, a.neg);
+    }
+    while (todo) {
+        // a run of neighbours with one prefix: sequences b0 + i .. b0 + j - 1
+        const int i = __builtin_ctzll(todo);
+        const uint64_t stop = i == 63 ? ~0ull : ~(joined >> (i + 1));
+        const int j = min(i + 1 + (int)__builtin_ctzll(stop | 1ull << 63), b1 - b0 + 1);
+        todo &= j >= 64 ? 0ull : ~0ull << j;
+        const int P = __builtin_amdgcn_readlane(me.P, i), owner = __builtin_amdgcn_readlane(me.owner, i);
+        const int tiles = pf_tiles(P), per = pf_per(tiles, a.NP, kPfMinTiles);
+        const int k0 = z * per, k1 = min(k0 + per, tiles);
+        if (k0 >= k1) continue;  // the whole workgroup
+        const int64_t ra = max(r0, (int64_t)(b0 + i) * a.G), rb = min(r1, (int64_t)(b0 + j) * a.G);  // its rows
+        unsigned live = 0;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            if (r0 + 16 * t < rb && r0 + 16 * t + 16 > ra) live |= 1u << t;
+        st.clear();
+        const int32_t* row = a.pt + owner * a.pts;
+        auto at = [&](int k) {
+            const int page = row[k];
+            PfAt x{page >= 0 && page < a.np ? page * a.pgs + h * a.hs : -1, 0, P - k * kPfPage};
+            if (x.off < 0) x.hi = 0;
+            return x;
+        };
+        typename F::T kf[8] = {}, vf[8] = {};
+        for (int k = k0 + wave; k < k1; k += 4) {
+            const PfAt x = at(__builtin_amdgcn_readfirstlane(k));
+            pf_load<KVQ>(a, x, kf, vf);
+            st.template tile<KVQ>(kf, vf, x.lo, x.hi, a.sc, live);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (!(live >> t & 1)) continue;
+            pf_merge(a, sm, st.acc[t], st.m[t], st.l[t], [&](int i16) -> int64_t {
+                const int64_t r = r0 + 16 * t + i16;
+                if (r < ra || r >= rb) return -1;
+                const int64_t b = r / a.G;
+                return (b * a.Hq + h * a.G + (r - b * a.G)) * (a.NP + a.NS) + z;
+            });
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// The other keys. Grid (key range, kv head and tile of 16 of its heads, sequence).
+// ---------------------------------------------------------------------------------------------
+template <int KVQ, int QDT>
+__global__ __launch_bounds__(256) void k_suffix(PfArgs a) {
+    constexpr int NQ = QDT == DT_BF16 ? 1 : QDT == DT_F16 ? 2 : 3;
+    using F = PfFrag<KVQ>;
+    __shared__ PfShared sm;
+    const int z = blockIdx.x, ct = blockIdx.y / a.Hkv, h = blockIdx.y - ct * a.Hkv, b = blockIdx.z;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
+    const PfSeq s = pf_seq(a, b);
+    // tiles [0, n1) the owner's, below P; then its own from the tile that holds P on
+    const int n1 = pf_shared(a, b, s) ? 0 : pf_tiles(s.P), first = s.P / kPfPage;
+    const int tiles = s.L > s.P ? n1 + pf_tiles(s.L) - first : n1;
+    const int per = pf_per(tiles, a.NS, kPfMinSuffix), k0 = z * per, k1 = min(k0 + per, tiles);
+    if (k0 >= k1) return;
+    PfState<1, NQ, NQ> st;
+    {
+        const int g = min(ct * 16 + l16, a.G - 1);
+        const int64_t off = (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2);
+        st.template load_q<QDT>(0, (const uint8_t*)a.q + off, a.neg);
+    }
+    st.clear();
+    auto at = [&](int k) {
+        const bool pre = k < n1;
+        const int blk = pre ? k : first + k - n1;
+        const int page = a.pt[(pre ? s.owner : b) * a.pts + blk];
+        PfAt x{page >= 0 && page < a.np ? page * a.pgs + h * a.hs : -1, pre ? 0 : s.P - blk * kPfPage, (pre ? s.P : s.L) - blk * kPfPage};
+        if (x.off < 0) x.hi = 0;
+        return x;
+    };
+    typename F::T kf[8] = {}, vf[8] = {};
+    for (int k = k0 + wave; k < k1; k += 4) {
+        const PfAt x = at(__builtin_amdgcn_readfirstlane(k));
+        pf_load<KVQ>(a, x, kf, vf);
+        st.template tile<KVQ>(kf, vf, x.lo, x.hi, a.sc, 1u);
+    }
+    pf_merge(a, sm, st.acc[0], st.m[0], st.l[0], [&](int i16) -> int64_t {
+        const int g = ct * 16 + i16;
+        return g < a.G ? ((int64_t)b * a.Hq + h * a.G + g) * (a.NP + a.NS) + a.NP + z : -1;
+    });
+}
+
+// ---------------------------------------------------------------------------------------------
+// The join: a wave per (sequence, head), lane i the dims 2 i, 2 i + 1.
+// ---------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void k_prefix_join(PfArgs a, int odt) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= (int64_t)a.B * a.Hq) return;
+    const int b = (int)(row / a.Hq), hq = (int)(row - (int64_t)b * a.Hq);
+    const PfSeq s = pf_seq(a, b);
+    const bool sh = pf_shared(a, b, s);
+    const int tp = sh ? pf_tiles(s.P) : 0, pp = pf_per(tp, a.NP, kPfMinTiles), np = (tp + pp - 1) / pp;
+    const int n1 = sh ? 0 : pf_tiles(s.P), ts = s.L > s.P ? n1 + pf_tiles(s.L) - s.P / kPfPage : n1;
+    const int ps = pf_per(ts, a.NS, kPfMinSuffix), ns = (ts + ps - 1) / ps;
+    const float2* ml = a.ml + row * (a.NP + a.NS);
+    const float2* o = reinterpret_cast<const float2*>(a.o + row * (a.NP + a.NS) * kPfDim) + lane;
+    float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
+    for (int i = 0; i < np + ns; ++i) M = fmaxf(M, ml[i < np ? i : a.NP + i - np].x);
+    for (int i = 0; i < np + ns; ++i) {
+        const int r = i < np ? i : a.NP + i - np;
+        const float2 e = ml[r], v = o[r * (kPfDim / 2)];
+        const float w = M == -INFINITY ? 1.f : e.x == -INFINITY ? (e.y == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(e.x - M);
+        L += e.y * w;
+        x += v.x * w;
+        y += v.y * w;
+    }
+    // no key, or none with a score above -inf: zeros
+    const float inv = L == 0.f ? 0.f : a.vs / L;
+    const int64_t at = b * a.o_sb + hq * a.o_sh + 2 * lane;
+    store_from_f32(a.out, at, odt, L == 0.f ? 0.f : x * inv);
+    store_from_f32(a.out, at + 1, odt, L == 0.f ? 0.f : y * inv);
+    if (a.lse && lane == 0) a.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * kPfLn2;
+}
+
+struct PfPlan {
+    int NT, NP, NS, tiles;
+};
+// Launch shape from what the host knows: rows, kv heads and the table's width (an upper bound of every length).
+static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
+    const int64_t rows = (int64_t)B * (Hq / Hkv), groups = (Hq / Hkv + 15) / 16;
+    PfPlan p;
+    // rows a workgroup shares a key among: 64, fewer when there are fewer, or when q's further terms take the registers
+    p.NT = rows <= 16 ? 1 : rows <= 32 || dt != DT_BF16 ? 2 : 4;
+    p.tiles = (int)((rows + 16 * p.NT - 1) / (16 * p.NT));
+    auto clamp = [](int64_t v, int64_t hi) { return (int)max((int64_t)1, min(min(v, hi), (int64_t)kPfMaxRecords)); };
+    // a workgroup a CU for the prefix (its waves fill the register file), eight for the suffix
+    p.NP = clamp(256 / ((int64_t)p.tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
+    p.NS = clamp(2048 / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);
+    return p;
+}
+
+template <int KVQ, int QDT>
+static void pf_launch(const PfArgs& a, const PfPlan& p, int odt, hipStream_t st) {
+    const dim3 grid((a.Hkv * a.NP + 7) / 8 * 8, p.tiles), block(256);
+    if (a.B > 1) {  // one sequence shares nothing
+        if (p.NT == 1) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 1>), grid, block, 0, st, a);
+        else if (p.NT == 2) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 2>), grid, block, 0, st, a);
+        else if constexpr (QDT == DT_BF16) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 4>), grid, block, 0, st, a);
+    }
+    hipLaunchKernelGGL((k_suffix<KVQ, QDT>), dim3(a.NS, a.Hkv * ((a.G + 15) / 16), a.B), block, 0, st, a);
+    hipLaunchKernelGGL(k_prefix_join, dim3((unsigned)(((int64_t)a.B * a.Hq + 3) / 4)), block, 0, st, a, odt);
+}
+
+template <int KVQ>
+static void pf_dispatch(const PfArgs& a, const PfPlan& p, int dt, hipStream_t st) {
+    if (dt == DT_BF16) pf_launch<KVQ, DT_BF16>(a, p, dt, st);
+    else if (dt == DT_F16) pf_launch<KVQ, DT_F16>(a, p, dt, st);
+    else pf_launch<KVQ, DT_F32>(a, p, dt, st);
+}
+
+}  // namespace wf
+
+using namespace wf;
+
+extern "C" {
+
+int64_t wf_shared_prefix_attention_ws_bytes(int dtype, int B, int Hq, int Hkv, int max_blocks) {
+    if (B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || max_blocks <= 0) return 0;
+    const PfPlan p = pf_plan(dtype, B, Hq, Hkv, max_blocks);
+    return (int64_t)B * Hq * (p.NP + p.NS) * (int64_t)(sizeof(float2) + 4 * kPfDim);
+}
+
+int wf_shared_prefix_attention(const void* q, int dtype, int64_t q_sb, int64_t q_sh, const void* k_pool, const void* v_pool, int kv_quant,
+                               int64_t page_stride, int64_t head_stride, int num_pages, const int32_t* page_table,
+                               int64_t table_stride, int max_blocks, const int32_t* seq_lens, const int32_t* prefix_rows,
+                               const int32_t* prefix_lens, float k_scale, float v_scale, float sm_scale, int B, int Hq, int Hkv, int D,
+                               void* out, int64_t o_sb, int64_t o_sh, float* lse, void* ws, void* stream) {
+    WF_REQUIRE(dtype == WF_F32 || dtype == WF_BF16 || dtype == WF_F16, "shared_prefix_attention: bad dtype %d", dtype);
+    WF_REQUIRE(kv_quant == WF_KV_BF16 || kv_quant == WF_KV_FP8 || kv_quant == WF_KV_INT8, "shared_prefix_attention: bad kv_quant %d", kv_quant);
+    WF_REQUIRE(D == kPfDim, "shared_prefix_attention: the pool's tile layouts need head_dim 128 (got %d)", D);
+    WF_REQUIRE(B >= 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0, "shared_prefix_attention: bad heads or batch (B %d, Hq %d, Hkv %d)", B, Hq, Hkv);
+    WF_REQUIRE(B <= 65535 && (int64_t)Hkv * ((Hq / Hkv + 15) / 16) <= 65535 && (int64_t)B * (Hq / Hkv) <= 16 * 65535,
+               "shared_prefix_attention: batch %d or heads %d / %d too many", B, Hq, Hkv);
+    WF_REQUIRE(num_pages > 0 && max_blocks > 0 && max_blocks <= 0x7fffffff / kPfPage && table_stride >= max_blocks,
+               "shared_prefix_attention: bad pool or table (%d pages, rows of %d at stride %lld)", num_pages, max_blocks, (long long)table_stride);
+    const int eb = kv_quant == WF_KV_BF16 ? 2 : 1;
+    WF_REQUIRE(page_stride >= 0 && head_stride >= 0 && page_stride * eb % 16 == 0 && head_stride * eb % 16 == 0,
+               "shared_prefix_attention: page and head strides must be multiples of 16 bytes");
+    const float sc = sm_scale * k_scale * 1.44269504088896340736f;
+    WF_REQUIRE(fabsf(sc) > 0.f && fabsf(sc) < INFINITY, "shared_prefix_attention: sm_scale %g times k_scale %g must be finite, not 0", sm_scale,
+               k_scale);
+    if (B == 0) return WF_OK;
+    WF_REQUIRE(q && k_pool && v_pool && page_table && seq_lens && prefix_rows && prefix_lens && out && ws,
+               "shared_prefix_attention: null pointer");
+    WF_REQUIRE(aligned16(k_pool) && aligned16(v_pool) && aligned16(ws), "shared_prefix_attention: pools and workspace must be 16-byte aligned");
+    const PfPlan p = pf_plan(dtype, B, Hq, Hkv, max_blocks);
+    const int64_t recs = (int64_t)B * Hq * (p.NP + p.NS);
+    float* o = reinterpret_cast<float*>(ws);
+    PfArgs a{q, q_sb, q_sh, (const uint8_t*)k_pool, (const uint8_t*)v_pool, page_stride * eb, head_stride * eb, num_pages, page_table,
+             table_stride, max_blocks, seq_lens, prefix_rows, prefix_lens, B, Hq, Hkv, Hq / Hkv, fabsf(sc), sc < 0.f ? -1.f : 1.f, v_scale,
+             p.NP, p.NS, reinterpret_cast<float2*>(o + recs * kPfDim), o, out, o_sb, o_sh, lse};
+    hipStream_t st = as_stream(stream);
+    if (kv_quant == WF_KV_BF16) pf_dispatch<0>(a, p, dtype, st);
+    else if (kv_quant == WF_KV_FP8) pf_dispatch<1>(a, p, dtype, st);
+    else pf_dispatch<2>(a, p, dtype, st);
+    return check_launch("shared_prefix_attention");
+}
+
+}  // extern "C"

@@ -62,6 +62,9 @@ SIGNATURES = {
     "wf_kv_page_plan": (i32, [vp, vp, i32, vp, i32, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     "wf_rotary_embed": (i32, [vp, i64, i64, i32, vp, i64, i64, i32, i32, vp, i32, vp, i32, i32, i32, i32, f32, vp, i64, i64,
                               vp, i64, i64, vp]),
+    "wf_shared_prefix_attention_ws_bytes": (i64, [i32, i32, i32, i32, i32]),
+    "wf_shared_prefix_attention": (i32, [vp, i32, i64, i64, vp, vp, i32, i64, i64, i32, vp, i64, i32, vp, vp, vp, f32, f32, f32, i32,
+                                         i32, i32, i32, vp, i64, i64, vp, vp, vp]),
     "wf_token_logprobs_ws_bytes": (i64, [i32, i32, i32]),
     "wf_token_logprobs": (i32, [vp, i32, i64, i32, i32, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp]),
     "wf_absmax": (i32, [vp, i32, i64, vp, vp]),

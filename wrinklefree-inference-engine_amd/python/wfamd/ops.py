@@ -562,6 +562,57 @@ def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     return qo, ko
 
 
+_KV_QUANT = {"bf16": (_lib.WF_KV_BF16, torch.bfloat16), "fp8": (_lib.WF_KV_FP8, torch.uint8), "int8": (_lib.WF_KV_INT8, torch.uint8)}
+
+
+def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
+                            seq_lens: torch.Tensor, prefix_rows: torch.Tensor, prefix_lens: torch.Tensor, *, kv_dtype: str = "bf16",
+                            k_scale: float = 1.0, v_scale: float = 1.0, sm_scale: Optional[float] = None, return_lse: bool = False):
+    """Attention of one query token per sequence over the paged pool, the keys of a shared prefix read once
+    (include/wf_bitnet.h wf_shared_prefix_attention). q [B, Hq, 128] bf16 / f16 / f32; k_pool, v_pool one layer of a paged
+    BitNetDecoder's k_cache / v_cache, [pages, Hkv, 32 * 128] in the tile layouts (bf16, or uint8 codes of kv_dtype
+    'fp8' / 'int8' with their scales); page_table [B, blocks] int32. Sequence b attends to its first seq_lens[b] keys:
+    those below prefix_lens[b] stand on the pages of row prefix_rows[b] (a negative row: no prefix), the rest on its
+    own. Neighbours in the batch with the same prefix_rows and prefix_lens share its reading. Returns out [B, Hq, 128] in
+    q's dtype, with return_lse=True also the log of the sum of exponentials [B, Hq] float32. A sequence of no keys
+    gives zeros and -inf."""
+    name = "shared_prefix_attention"
+    dev = q.device
+    _serve_args(name, dev, q=q, k_pool=k_pool, v_pool=v_pool, page_table=page_table, seq_lens=seq_lens, prefix_rows=prefix_rows,
+                prefix_lens=prefix_lens)
+    code = _dtcode(q)
+    if kv_dtype not in _KV_QUANT:
+        raise ValueError(f"{name}: kv_dtype must be 'bf16', 'fp8' or 'int8', got {kv_dtype!r}")
+    quant, kvt = _KV_QUANT[kv_dtype]
+    if q.dim() != 3 or q.shape[2] != 128:
+        raise ValueError(f"{name}: q must be [batch, heads, 128], got {tuple(q.shape)}")
+    B, Hq, D = q.shape
+    if k_pool.dim() != 3 or k_pool.shape != v_pool.shape or k_pool.shape[2] != 32 * D or k_pool.dtype != kvt or v_pool.dtype != kvt or (
+            k_pool.stride() != v_pool.stride() or k_pool.stride(2) != 1):
+        raise ValueError(f"{name}: k_pool / v_pool must be {kvt} [pages, kv_heads, {32 * D}] alike, got {k_pool.dtype} {tuple(k_pool.shape)} "
+                         f"and {v_pool.dtype} {tuple(v_pool.shape)}")
+    pages, Hkv = k_pool.shape[:2]
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
+        raise ValueError(f"{name}: {Hq} query heads for {Hkv} kv heads")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B or (
+            B and page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"{name}: page_table must be int32 [{B}, blocks] with contiguous rows, got {page_table.dtype} {tuple(page_table.shape)}")
+    for what, t in (("seq_lens", seq_lens), ("prefix_rows", prefix_rows), ("prefix_lens", prefix_lens)):
+        _int32_rows(name, what, t, B)
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    cols = page_table.shape[1]
+    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    ws = torch.empty(int(_lib.load().wf_shared_prefix_attention_ws_bytes(code, B, Hq, Hkv, cols)), dtype=torch.uint8, device=dev)
+    _call_on(dev, "wf_shared_prefix_attention", q.data_ptr(), code, q.stride(0), q.stride(1), k_pool.data_ptr(), v_pool.data_ptr(), quant,
+             k_pool.stride(0), k_pool.stride(1), pages, page_table.data_ptr(), max(page_table.stride(0), cols) if B < 2 else page_table.stride(0),
+             cols, seq_lens.data_ptr(), prefix_rows.data_ptr(), prefix_lens.data_ptr(), float(k_scale), float(v_scale),
+             float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(D), B, Hq, Hkv, D, out.data_ptr(), out.stride(0),
+             out.stride(1), _ptr(lse), ws.data_ptr())
+    return (out, lse) if return_lse else out
+
+
 class TokenLogprobs(NamedTuple):
     """token_logprobs' results on the device (float32 / int32); logprobs and ranks are None without tokens."""
     logprobs: Optional[torch.Tensor]  # [R] log probability of the row's token
