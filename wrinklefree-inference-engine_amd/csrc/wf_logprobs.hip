@@ -30,30 +30,80 @@ struct LpPart {  // one chunk's sums (z = 0: it holds nothing but -inf)
     int rank;       // elements of the chunk that come before the row's token
 };
 
-// The wave's k best (value, index) so far, sorted across lanes: value descending, lower index first.
+// lane ^ X of a wave: DPP within 16 lanes, an LDS permute beyond
+template <int X>
+__device__ __forceinline__ int lp_xor(int v) {
+    if constexpr (X == 1) return dpp_i<DPP_QP_1032>(v);
+    else if constexpr (X == 2) return dpp_i<DPP_QP_2301>(v);
+    else if constexpr (X == 3) return dpp_i<0x1B>(v);  // quad_perm 3, 2, 1, 0
+    else if constexpr (X == 4) return dpp_i<DPP_HALF_MIRROR>(dpp_i<0x1B>(v));
+    else if constexpr (X == 7) return dpp_i<DPP_HALF_MIRROR>(v);
+    else if constexpr (X == 8) return dpp_i<DPP_ROW_ROR8>(v);
+    else if constexpr (X == 15) return dpp_i<DPP_MIRROR>(v);
+    else return __shfl_xor(v, X, 64);
+}
+constexpr int kDppWaveShr1 = 0x138;  // lane l reads lane l - 1
+
+// The wave's best (value, index) so far, sorted across lanes: value descending, lower index first.
 // Empty places hold (-inf, INT_MAX), behind every real entry; a NaN never enters.
 struct LpList {
     float v;
     int i;
     __device__ __forceinline__ LpList() : v(-INFINITY), i(0x7fffffff) {}
     static __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
-    // the candidates (one a lane) that come before entry k - 1, one after the other
+    // one step of a bitonic network: of lanes l and l ^ X, the one without bit BIT keeps the entry that comes first
+    template <int X, int BIT>
+    static __device__ __forceinline__ void step(float& v, int& i) {
+        const float w = __int_as_float(lp_xor<X>(__float_as_int(v)));
+        const int j = lp_xor<X>(i);
+        const bool keep = before(v, i, w, j) != ((threadIdx.x & BIT) != 0);
+        v = keep ? v : w;
+        i = keep ? i : j;
+    }
+    template <int X>
+    static __device__ __forceinline__ void clean(float& v, int& i) {
+        step<X, X>(v, i);
+        if constexpr (X > 1) clean<X / 2>(v, i);
+    }
+    static __device__ __forceinline__ void sort(float& v, int& i) {
+        step<1, 1>(v, i);
+        step<3, 2>(v, i), clean<1>(v, i);
+        step<7, 4>(v, i), clean<2>(v, i);
+        step<15, 8>(v, i), clean<4>(v, i);
+        step<31, 16>(v, i), clean<8>(v, i);
+        step<63, 32>(v, i), clean<16>(v, i);
+    }
+    // entry k - 1
+    __device__ __forceinline__ float last_v(int k) const { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k - 1)); }
+    __device__ __forceinline__ int last_i(int k) const { return __builtin_amdgcn_readlane(i, k - 1); }
+    // Takes in the candidates (one a lane) that come before entry k - 1: many by a sort and a merge (27 steps of the
+    // network), few one after the other.
     __device__ __forceinline__ void add(float cv, int ci, int k) {
-        float kv = __shfl(v, k - 1, 64);
-        int ki = __shfl(i, k - 1, 64);
-        for (uint64_t todo = __ballot(before(cv, ci, kv, ki)); todo;) {
+        uint64_t todo = __ballot(before(cv, ci, last_v(k), last_i(k)));
+        if (__builtin_popcountll(todo) > 16) {
+            const bool in = todo >> (threadIdx.x & 63) & 1;
+            cv = in ? cv : -INFINITY;
+            ci = in ? ci : 0x7fffffff;
+            sort(cv, ci);
+            const float w = __int_as_float(lp_xor<63>(__float_as_int(cv)));
+            const int j = lp_xor<63>(ci);
+            const bool keep = before(v, i, w, j);  // the first 64 of both lists, a bitonic sequence
+            v = keep ? v : w;
+            i = keep ? i : j;
+            clean<32>(v, i);
+            return;
+        }
+        while (todo) {
             const int l = __builtin_ctzll(todo);
             const float nv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(cv), l));
             const int ni = __builtin_amdgcn_readlane(ci, l);
             const int at = __builtin_popcountll(__ballot(before(v, i, nv, ni))), lane = threadIdx.x & 63;
-            const float pv = __shfl_up(v, 1, 64);
-            const int pi = __shfl_up(i, 1, 64);
+            const float pv = dpp_f<kDppWaveShr1>(v, v);
+            const int pi = dpp_i<kDppWaveShr1>(i, i);
             v = lane < at ? v : lane == at ? nv : pv;
             i = lane < at ? i : lane == at ? ni : pi;
-            kv = __shfl(v, k - 1, 64);
-            ki = __shfl(i, k - 1, 64);
             todo &= todo - 1;
-            todo &= __ballot(before(cv, ci, kv, ki));
+            todo &= __ballot(before(cv, ci, last_v(k), last_i(k)));
         }
     }
 };
@@ -119,35 +169,53 @@ __device__ __forceinline__ float lp_above(float x) {
     return __int_as_float(x >= 0.f ? b + 1 : b - 1);
 }
 
-// Running sums of one lane over the logits it has seen: z = sum 2^y, t = sum y 2^y, y = (x - m) log2e. The
-// difference is taken before the product: m log2e overflows for logits at the type's lowest or highest value.
+// Running sums of one lane over the logits it has seen: z = sum 2^y, t = sum y 2^y, y = (x - m) log2e + c. In the
+// loop y is one fma, x log2e - g with g = m log2e rounded; c = m log2e - g is what the rounding took and goes back in when
+// the frame moves. Where m log2e might overflow (logits near the type's lowest or highest value) c is 0 and the
+// difference is taken first.
 struct LpSums {
-    float m, z, t;
-    __device__ __forceinline__ LpSums() : m(-INFINITY), z(0.f), t(0.f) {}
-    // x's frame: 0 while nothing but -inf (or NaN) was seen, so that -inf - m is no NaN
+    float m, c, z, t;
+    __device__ __forceinline__ LpSums() : m(-INFINITY), c(0.f), z(0.f), t(0.f) {}
+    // 0 while nothing but -inf (or NaN) was seen, so that -inf - m is no NaN
     __device__ __forceinline__ float frame() const { return m == -INFINITY ? 0.f : m; }
-    // the sums in the frame of a max nm >= m; z = NaN stays
-    __device__ __forceinline__ void move(float nm) {
-        if (z == 0.f) return;
-        const float d = (frame() - nm) * kLog2e, s = exp2f(d);
-        t = s == 0.f ? 0.f : (t + d * z) * s;
-        z *= s;
+    static __device__ __forceinline__ bool huge(float f) { return !(fabsf(f) < 1e30f); }
+    // the sums in the frame (nm, nc), nm >= m; z = NaN stays
+    __device__ __forceinline__ void move(float nm, float nc) {
+        if (z != 0.f) {
+            const float d = (frame() - nm) * kLog2e - c + nc, s = exp2f(d);
+            t = s == 0.f ? 0.f : (t + d * z) * s;
+            z *= s;
+        }
+        c = nc;
     }
     __device__ __forceinline__ void raise(float tm) {
         if (tm > m) {
-            move(tm);
+            move(tm, huge(tm) ? 0.f : fmaf(tm, kLog2e, -(tm * kLog2e)));
             m = tm;
         }
     }
-    __device__ __forceinline__ void one(float x, float f) {
-        const float y = (x - f) * kLog2e, e = __builtin_amdgcn_exp2f(y);
+    __device__ __forceinline__ void sum(float y) {
+        const float e = __builtin_amdgcn_exp2f(y);
         z += e;
-        t = fmaf(fmaxf(y, -200.f), e, t);  // y = -inf: 0, not NaN
+        t = fmaf(fmaxf(y, -200.f), e, t);  // y = -inf: 0, not NaN (a NaN stays in z)
+    }
+    // N logits whose max is not above m (the caller raised it)
+    template <int N>
+    __device__ __forceinline__ void add(const float (&x)[N]) {
+        const float f = frame();
+        if (__ballot(huge(f))) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum(fmaf(x[e] - f, kLog2e, c));
+        } else {
+            const float g = f * kLog2e;
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum(fmaf(x[e], kLog2e, -g));
+        }
     }
     // all lanes' sums in one frame (the max of those that hold something)
     __device__ __forceinline__ void join() {
         const float nm = wave_max(z == 0.f ? -INFINITY : m);
-        move(nm == -INFINITY ? 0.f : nm);
+        move(nm == -INFINITY ? 0.f : nm, 0.f);
         m = nm;
         z = wave_sum(z);
         t = wave_sum(t);
@@ -184,7 +252,8 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
         const int j = lane < head ? lo + lane : lane < head + hi - tail ? tail + lane - head : -1;
         const float x = j >= 0 ? E::up(row[j]) : -INFINITY;
         sum.raise(x);
-        if (j >= 0) sum.one(x, sum.frame());
+        const float one[1] = {x};
+        sum.add(one);
         if constexpr (TOK) rank += __builtin_popcountll(__ballot(tok >= 0 && j >= 0 && (x > xt || (x == xt && j < tok))));
         if constexpr (TOP) elems.add(x, j >= 0 ? j : 0x7fffffff, a.k);
     }
@@ -203,36 +272,37 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
             if (i < nv) nx[u] = vec[i];
         }
         float x[U][N], vm[U], tm = -INFINITY;
+        const bool whole = base + 64 * U <= nv;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             E::unpack(cur[u], x[u]);
-            const bool in = base + u * 64 + lane < nv;
+            if (!whole) {
+                const bool in = base + u * 64 + lane < nv;
 #pragma unroll
-            for (int e = 0; e < N; ++e) x[u][e] = in ? x[u][e] : -INFINITY;
+                for (int e = 0; e < N; ++e) x[u][e] = in ? x[u][e] : -INFINITY;
+            }
             vm[u] = x[u][0];
 #pragma unroll
             for (int e = 1; e < N; ++e) vm[u] = fmaxf(vm[u], x[u][e]);
             tm = fmaxf(tm, vm[u]);
         }
         sum.raise(tm);
-        const float f = sum.frame();
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < N; ++e) sum.one(x[u][e], f);
+        for (int u = 0; u < U; ++u) sum.add(x[u]);
         if constexpr (TOK) {
             // before the token >= counts, from it on >; the vector that holds it one by one
+            if (tok >= 0 && __any(tm >= xt)) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = base + u * 64 + lane, j = v0 + i * N;
-                const bool hold = j <= tok && tok < j + N;
-                const float lim = i >= nv || tok < 0 ? NAN : j + N <= tok ? xt : gt;
+                for (int u = 0; u < U; ++u) {
+                    const int i = base + u * 64 + lane, j = v0 + i * N;
+                    const bool hold = j <= tok && tok < j + N && i < nv;
+                    const float lim = i >= nv ? NAN : j + N <= tok ? xt : gt;
 #pragma unroll
-                for (int e = 0; e < N; ++e) rank += __builtin_popcountll(__ballot(x[u][e] >= lim));
-                if (__ballot(hold && i < nv)) {
+                    for (int e = 0; e < N; ++e) rank += __builtin_popcountll(__ballot(x[u][e] >= lim));
+                    if (__any(hold)) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        rank += __builtin_popcountll(__ballot(hold && i < nv && x[u][e] == xt && j + e < tok));
+                        for (int e = 0; e < N; ++e) rank += __builtin_popcountll(__ballot(hold && x[u][e] == xt && j + e < tok));
+                    }
                 }
             }
         }
@@ -253,14 +323,27 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     const int64_t at = (int64_t)r * a.S + s;
     if (lane == 0) a.part[at] = LpPart{sum.m, sum.z, sum.t, rank};
     if constexpr (TOP) {
-        // the elements of the k best groups, 64 / (4 N) groups a round
-        constexpr int G = 64 / (4 * N);
-        for (int i = 0; i < a.k; i += G) {
-            const int g = __shfl(groups.i, i + lane / (4 * N), 64);
-            const int j = g == 0x7fffffff || i + lane / (4 * N) >= a.k ? hi : v0 + g * 4 * N + lane % (4 * N);
-            const bool in = j < tail;
-            if (!__ballot(in)) break;  // groups are sorted: none behind an empty place
-            elems.add(in ? E::up(row[j]) : -INFINITY, in ? j : 0x7fffffff, a.k);
+        // the k best groups again, a vector a lane: 16 groups a load, all of them under way before the first is looked at
+        constexpr int M = kLpMaxTop / 16;
+        uint4 w[M];
+        int at_vec[M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const int e = 16 * i + (lane >> 2), g = __shfl(groups.i, e, 64);
+            at_vec[i] = e < a.k && g != 0x7fffffff && 4 * g + (lane & 3) < nv ? 4 * g + (lane & 3) : -1;
+            if (at_vec[i] >= 0) w[i] = vec[at_vec[i]];
+        }
+        const float least = groups.last_v(a.k);  // k maxima reach it: nothing below it is among the k first
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            if (16 * i >= a.k) break;
+            float x[N];
+            E::unpack(w[i], x);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const bool in = at_vec[i] >= 0 && x[e] >= least;
+                elems.add(in ? x[e] : -INFINITY, in ? v0 + at_vec[i] * N + e : 0x7fffffff, a.k);
+            }
         }
         if (lane < a.k) {
             a.list_v[at * a.k + lane] = elems.v;
@@ -296,12 +379,17 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     if (a.k == 0) return;
     // the chunks' sorted lists, a lane each, from the front until no front can enter
     LpList top;
-    for (int i = 0; i < a.k; ++i) {
-        float v = -INFINITY;
-        int j = 0x7fffffff;
-        if (lane < a.S) v = a.list_v[(at + lane) * a.k + i], j = a.list_i[(at + lane) * a.k + i];
-        if (!__ballot(LpList::before(v, j, __shfl(top.v, a.k - 1, 64), __shfl(top.i, a.k - 1, 64)))) break;
-        top.add(v, j, a.k);
+    for (int i = 0; i < a.k; i += 4) {
+        float v[4];
+        int j[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = -INFINITY, j[e] = 0x7fffffff;
+            if (lane < a.S && i + e < a.k) v[e] = a.list_v[(at + lane) * a.k + i + e], j[e] = a.list_i[(at + lane) * a.k + i + e];
+        }
+        if (!__ballot(LpList::before(v[0], j[0], top.last_v(a.k), top.last_i(a.k)))) break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top.add(v[e], j[e], a.k);
     }
     if (lane < a.k) {
         const bool in = top.i != 0x7fffffff;  // no: fewer than k logits of the row are numbers

@@ -15,8 +15,8 @@
 namespace wf {
 
 constexpr int kPlanThreads = 256;
-constexpr int kPlanTokens = 4 * kPlanThreads;  // tokens a workgroup fills, four neighbours a thread
-constexpr int kPlanLdsSeqs = 2048;             // two int32 arrays of this many + 1 in LDS (16 KiB)
+constexpr int kPlanLdsSeqs = 2048;   // four int32 arrays of this many in LDS (32 KiB)
+constexpr int kPlanWide = 1 << 15;   // tokens from which a thread takes four neighbours (16-byte stores) instead of one
 
 struct PlanArgs {
     const int32_t *cached, *fresh;
@@ -25,83 +25,100 @@ struct PlanArgs {
     int F;
     int32_t* table;
     int64_t ts;
-    int cols, page, T;
+    int cols, page, shift, T;  // shift: log2 of page, or -1
     int32_t *pages, *slots, *rows, *pos, *cu, *counts;
     int32_t *ws_off, *ws_cu;  // [B + 1] each, B > kPlanLdsSeqs only
-    int vec;                  // the four token arrays are 16-byte aligned
 };
 
 // Lengths are clamped to >= 0; sums are 64 bits and saturate where they are stored as 32.
 __device__ __forceinline__ int32_t sat32(int64_t v) { return (int32_t)(v < 0x7fffffff ? v : 0x7fffffff); }
+__device__ __forceinline__ uint32_t plan_div(const PlanArgs& a, uint32_t v) { return a.shift >= 0 ? v >> a.shift : v / (uint32_t)a.page; }
 
 struct PlanSeq {
-    int64_t c, n;         // held and new tokens
-    int64_t have, total;  // pages held, pages after
+    uint32_t c, n;        // held and new tokens
+    uint32_t have;        // pages held
+    uint32_t need;        // pages missing, 0 if lng
     bool lng;             // does not fit the table row
-    __device__ __forceinline__ int64_t need() const { return lng ? 0 : total - have; }
     // pages [off, off + need) of the free list are there
-    __device__ __forceinline__ bool fit(int64_t off, int F) const { return !lng && (need() == 0 || off + need() <= F); }
+    __device__ __forceinline__ bool fit(int64_t off, int F) const { return !lng && (need == 0 || off + need <= F); }
 };
-__device__ __forceinline__ PlanSeq plan_seq(const PlanArgs& a, int b) {
+__device__ __forceinline__ PlanSeq plan_seq(const PlanArgs& a, int c, int n) {
     PlanSeq s;
-    s.c = max(a.cached[b], 0);
-    s.n = max(a.fresh[b], 0);
-    const uint32_t p = (uint32_t)a.page;
-    s.have = ((uint32_t)s.c + (p - 1)) / p;  // c + p - 1 < 2^32
-    // c + n may pass 2^32: quotients and remainders apart
-    const uint32_t c = (uint32_t)s.c, n = (uint32_t)s.n;
-    const uint32_t rem = c % p + n % p;
-    s.total = (int64_t)(c / p) + n / p + (rem + p - 1) / p;
-    s.lng = s.total > a.cols;
+    s.c = (uint32_t)max(c, 0);
+    s.n = (uint32_t)max(n, 0);
+    const uint32_t up = (uint32_t)a.page - 1;
+    s.have = plan_div(a, s.c + up);                     // c + up < 2^32
+    const uint32_t total = s.c + s.n;                   // < 2^32
+    const uint32_t q = plan_div(a, total), blocks = q + (q * (uint32_t)a.page < total);
+    s.lng = blocks > (uint32_t)a.cols;
+    s.need = s.lng ? 0 : blocks - s.have;
     return s;
 }
 
-// Exclusive sums of need and n over all sequences into off[0..B], cu[0..B]; thread t takes four
-// neighbours of every 1024. Workgroup 0's call also leaves the counts.
-__device__ void plan_scan(const PlanArgs& a, int32_t* off, int32_t* cu, bool report) {
+// inclusive sum over the wave's lanes (DPP: rows of 16, then across rows)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t plan_add(int64_t v) {
+    const uint32_t lo = (uint32_t)dpp_i<CTRL, ROWS>((int)(uint32_t)v, 0), hi = (uint32_t)dpp_i<CTRL, ROWS>((int)(v >> 32), 0);
+    return v + (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int64_t plan_wave_sum(int64_t v) {
+    v = plan_add<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+    v = plan_add<0x112, 0xF>(v);
+    v = plan_add<0x114, 0xF>(v);
+    v = plan_add<0x118, 0xF>(v);
+    v = plan_add<DPP_BCAST15, 0xA>(v);
+    return plan_add<DPP_BCAST31, 0xC>(v);
+}
+
+// Exclusive sums of need and n over all sequences into off[0..B], cu[0..B], a thread taking E neighbours of every
+// 256 E; lengths into cl, nl where a workgroup keeps them. `report`: this workgroup leaves the counts.
+template <int E>
+__device__ void plan_scan(const PlanArgs& a, int32_t* off, int32_t* cu, int32_t* cl, int32_t* nl, bool report) {
     __shared__ int64_t sm_n[4], sm_t[4];
     __shared__ int sh_taken, sh_refused;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (threadIdx.x == 0) sh_taken = sh_refused = 0;
-    int64_t cn = 0, ct = 0;  // sums before this 1024
-    for (int b0 = 0; b0 < a.B; b0 += kPlanTokens) {
-        int64_t n4[4], t4[4], n = 0, t = 0;
+    int64_t cn = 0, ct = 0;  // sums before this round
+    for (int b0 = 0; b0 < a.B; b0 += kPlanThreads * E) {
+        PlanSeq s[E];
+        int64_t n = 0, t = 0;
+        int c[E], f[E];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int b = b0 + 4 * threadIdx.x + i;
-            n4[i] = t4[i] = 0;
-            if (b < a.B) {
-                const PlanSeq s = plan_seq(a, b);
-                n4[i] = s.need();
-                t4[i] = s.n;
-            }
-            n += n4[i];
-            t += t4[i];
+        for (int i = 0; i < E; ++i) {
+            const int b = b0 + E * threadIdx.x + i;
+            c[i] = b < a.B ? a.cached[b] : 0;
+            f[i] = b < a.B ? a.fresh[b] : 0;
         }
-        int64_t in = n, it = t;  // inclusive over the wave
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t un = __shfl_up(in, d, 64), ut = __shfl_up(it, d, 64);
-            if (lane >= d) in += un, it += ut;
+        for (int i = 0; i < E; ++i) {
+            s[i] = plan_seq(a, c[i], f[i]);
+            n += s[i].need;
+            t += s[i].n;
         }
+        const int64_t in = plan_wave_sum(n), it = plan_wave_sum(t);
         __syncthreads();  // the last round's sums have been read
         if (lane == 63) sm_n[wave] = in, sm_t[wave] = it;
         __syncthreads();
         int64_t on = cn + in - n, ot = ct + it - t;
-        for (int w = 0; w < wave; ++w) on += sm_n[w], ot += sm_t[w];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int b = b0 + 4 * threadIdx.x + i;
-            if (b < a.B) off[b] = sat32(on), cu[b] = sat32(ot);
-            if (report && b < a.B) {
-                const PlanSeq s = plan_seq(a, b);
-                if (!s.fit(on, a.F)) atomicAdd(&sh_refused, 1);
-                else if (n4[i]) atomicMax(&sh_taken, (int)(on + n4[i]));
-            }
-            on += n4[i];
-            ot += t4[i];
+        for (int w = 0; w < 4; ++w) {
+            if (w < wave) on += sm_n[w], ot += sm_t[w];
+            cn += sm_n[w], ct += sm_t[w];
         }
-        for (int w = 0; w < 4; ++w) cn += sm_n[w], ct += sm_t[w];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int b = b0 + E * threadIdx.x + i;
+            if (b < a.B) {
+                off[b] = sat32(on), cu[b] = sat32(ot);
+                if (cl) cl[b] = c[i], nl[b] = f[i];
+                if (report) {
+                    if (!s[i].fit(on, a.F)) atomicAdd(&sh_refused, 1);
+                    else if (s[i].need) atomicMax(&sh_taken, (int)(on + s[i].need));
+                }
+            }
+            on += s[i].need;
+            ot += s[i].n;
+        }
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -117,73 +134,93 @@ __device__ void plan_scan(const PlanArgs& a, int32_t* off, int32_t* cu, bool rep
     __syncthreads();
 }
 
-__global__ __launch_bounds__(kPlanThreads) void k_page_plan_scan(PlanArgs a) { plan_scan(a, a.ws_off, a.ws_cu, true); }
+__global__ __launch_bounds__(kPlanThreads) void k_page_plan_scan(PlanArgs a) { plan_scan<4>(a, a.ws_off, a.ws_cu, nullptr, nullptr, true); }
 
-template <bool LDS>
-__global__ __launch_bounds__(kPlanThreads) void k_page_plan(PlanArgs a) {
-    __shared__ int32_t sm[LDS ? 2 * (kPlanLdsSeqs + 1) : 1];
-    const int32_t *off = a.ws_off, *cu = a.ws_cu;
-    if constexpr (LDS) {
-        plan_scan(a, sm, sm + kPlanLdsSeqs + 1, blockIdx.x == 0);
-        off = sm, cu = sm + kPlanLdsSeqs + 1;
-    }
-    // the table rows, a wave per sequence: entries [have, total) only
-    for (int b = blockIdx.x * 4 + (threadIdx.x >> 6); b < a.B; b += gridDim.x * 4) {
-        const PlanSeq s = plan_seq(a, b);
-        const int64_t o = off[b];
-        if (!s.fit(o, a.F)) continue;
-        for (int64_t i = threadIdx.x & 63; i < s.need(); i += 64) a.table[b * a.ts + s.have + i] = a.free_pages[o + i];
-    }
-    for (int b = blockIdx.x * kPlanThreads + threadIdx.x; b <= a.B; b += gridDim.x * kPlanThreads) a.cu[b] = cu[b];
-    // the tokens: four neighbours a thread
-    const int64_t t0 = (int64_t)blockIdx.x * kPlanTokens + 4 * threadIdx.x;
-    if (t0 >= a.T) return;
-    int lo = 0, hi = a.B;  // the last b with cu[b] <= t0 (cu[0] = 0)
+// the last b with at[b] <= v (at ascends, at[0] = 0, v < at[B])
+__device__ __forceinline__ int plan_find(const int32_t* at, int B, int v) {
+    int lo = 0, hi = B;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (cu[mid] <= t0) lo = mid;
+        if (at[mid] <= v) lo = mid;
         else hi = mid;
     }
-    int b = lo, pg[4], sl[4], rw[4], ps[4];
+    return lo;
+}
+
+// LDS: the sums in LDS, scanned here. N: tokens a thread takes.
+template <bool LDS, int N>
+__global__ __launch_bounds__(kPlanThreads) void k_page_plan(PlanArgs a) {
+    __shared__ int32_t sm[LDS ? 4 * (kPlanLdsSeqs + 1) : 1];
+    const int32_t *off = a.ws_off, *cu = a.ws_cu, *cl = a.cached, *nl = a.fresh;
+    if constexpr (LDS) {
+        constexpr int S = kPlanLdsSeqs + 1;
+        if (a.B <= kPlanThreads) plan_scan<1>(a, sm, sm + S, sm + 2 * S, sm + 3 * S, blockIdx.x == 0);
+        else plan_scan<4>(a, sm, sm + S, sm + 2 * S, sm + 3 * S, blockIdx.x == 0);
+        off = sm, cu = sm + S, cl = sm + 2 * S, nl = sm + 3 * S;
+    }
+    const int me = blockIdx.x * kPlanThreads + threadIdx.x, all = gridDim.x * kPlanThreads;
+    // the pages that are taken, one a thread: into their sequence's row
+    for (int i = me, n = min(off[a.B], a.F); i < n; i += all) {
+        const int b = plan_find(off, a.B, i);
+        const PlanSeq s = plan_seq(a, cl[b], nl[b]);
+        if (s.fit(off[b], a.F)) a.table[b * a.ts + s.have + (i - off[b])] = a.free_pages[i];
+    }
+    for (int b = me; b <= a.B; b += all) a.cu[b] = cu[b];
+    // the tokens
+    const int64_t t0 = (int64_t)me * N;
+    if (t0 >= a.T) return;
+    int pg[N], sl[N], rw[N], ps[N];
+    int b = t0 < cu[a.B] ? plan_find(cu, a.B, (int)t0) : -1, known = -1;
     int64_t o = 0;
-    PlanSeq s;
+    PlanSeq s{};
     bool fit = false;
-    int known = -1;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
         const int64_t t = t0 + i;
         pg[i] = sl[i] = rw[i] = ps[i] = -1;
-        if (t >= cu[a.B]) continue;  // behind the last sequence (also B == 0)
+        if (t >= cu[a.B]) continue;  // behind the last sequence
         while (cu[b + 1] <= t) ++b;
         if (b != known) {
-            s = plan_seq(a, b);
+            s = plan_seq(a, cl[b], nl[b]);
             o = off[b];
             fit = s.fit(o, a.F);
             known = b;
         }
-        const int64_t pos = s.c + (t - cu[b]);
+        const uint32_t pos = s.c + (uint32_t)(t - cu[b]);  // < c + n < 2^32
         rw[i] = b;
         ps[i] = sat32(pos);
         if (!fit) continue;
-        const uint32_t blk = (uint32_t)pos / (uint32_t)a.page;  // fits the row: pos < cols * page
-        sl[i] = (int)((uint32_t)pos - blk * (uint32_t)a.page);
+        const uint32_t blk = plan_div(a, pos);
+        sl[i] = (int)(pos - blk * (uint32_t)a.page);
         pg[i] = blk < s.have ? a.table[b * a.ts + blk] : a.free_pages[o + blk - s.have];
     }
-    if (a.vec && t0 + 4 <= a.T) {
-        *reinterpret_cast<int4*>(a.pages + t0) = make_int4(pg[0], pg[1], pg[2], pg[3]);
-        *reinterpret_cast<int4*>(a.slots + t0) = make_int4(sl[0], sl[1], sl[2], sl[3]);
-        *reinterpret_cast<int4*>(a.rows + t0) = make_int4(rw[0], rw[1], rw[2], rw[3]);
-        *reinterpret_cast<int4*>(a.pos + t0) = make_int4(ps[0], ps[1], ps[2], ps[3]);
-        return;
+    if constexpr (N == 4) {
+        if (t0 + 4 <= a.T) {  // the launch saw to the arrays' alignment
+            *reinterpret_cast<int4*>(a.pages + t0) = make_int4(pg[0], pg[1], pg[2], pg[3]);
+            *reinterpret_cast<int4*>(a.slots + t0) = make_int4(sl[0], sl[1], sl[2], sl[3]);
+            *reinterpret_cast<int4*>(a.rows + t0) = make_int4(rw[0], rw[1], rw[2], rw[3]);
+            *reinterpret_cast<int4*>(a.pos + t0) = make_int4(ps[0], ps[1], ps[2], ps[3]);
+            return;
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
         if (t0 + i >= a.T) break;
         a.pages[t0 + i] = pg[i];
         a.slots[t0 + i] = sl[i];
         a.rows[t0 + i] = rw[i];
         a.pos[t0 + i] = ps[i];
     }
+}
+
+template <bool LDS>
+static void plan_launch(const PlanArgs& a, hipStream_t st) {
+    const bool wide = a.T >= kPlanWide && aligned16(a.pages) && aligned16(a.slots) && aligned16(a.rows) && aligned16(a.pos);
+    const int each = kPlanThreads * (wide ? 4 : 1);
+    // a thread for every token; at least one for every second sequence up to 64 workgroups (the table's entries)
+    const int grid = max(max((a.T + each - 1) / each, min((a.B + 511) / 512, 64)), 1);
+    if (wide) hipLaunchKernelGGL((k_page_plan<LDS, 4>), dim3(grid), dim3(kPlanThreads), 0, st, a);
+    else hipLaunchKernelGGL((k_page_plan<LDS, 1>), dim3(grid), dim3(kPlanThreads), 0, st, a);
 }
 
 }  // namespace wf
@@ -208,21 +245,19 @@ int wf_kv_page_plan(const int32_t* cached_lens, const int32_t* new_lens, int B, 
     WF_REQUIRE(B == 0 || (cached_lens && new_lens && (page_table || max_blocks == 0)), "kv_page_plan: null lengths / table");
     WF_REQUIRE(num_free == 0 || free_pages, "kv_page_plan: null free list");
     WF_REQUIRE(num_tokens == 0 || (pages && slots && rows && positions), "kv_page_plan: null token arrays");
-    WF_REQUIRE(num_tokens <= 0x7fffffff - kPlanTokens, "kv_page_plan: too many tokens");
-    PlanArgs a{cached_lens, new_lens, B, free_pages, num_free, page_table, table_stride, max_blocks, page_size, num_tokens, pages,
-               slots, rows, positions, cu_tokens, counts, nullptr, nullptr,
-               aligned16(pages) && aligned16(slots) && aligned16(rows) && aligned16(positions)};
-    // at least a workgroup for every 1024 tokens; the table rows spread over up to 256
-    const int grid = max(max((num_tokens + kPlanTokens - 1) / kPlanTokens, min((B + 63) / 64, 256)), 1);
+    WF_REQUIRE(num_tokens <= 0x7fffffff - 4096, "kv_page_plan: too many tokens");
+    PlanArgs a{cached_lens, new_lens, B, free_pages, num_free, page_table, table_stride, max_blocks, page_size,
+               page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size), num_tokens, pages, slots, rows, positions, cu_tokens, counts,
+               nullptr, nullptr};
     hipStream_t st = as_stream(stream);
     if (B <= kPlanLdsSeqs) {
-        hipLaunchKernelGGL((k_page_plan<true>), dim3(grid), dim3(kPlanThreads), 0, st, a);
+        plan_launch<true>(a, st);
     } else {
         WF_REQUIRE(ws, "kv_page_plan: null workspace");
         a.ws_off = reinterpret_cast<int32_t*>(ws);
         a.ws_cu = a.ws_off + B + 1;
         hipLaunchKernelGGL(k_page_plan_scan, dim3(1), dim3(kPlanThreads), 0, st, a);
-        hipLaunchKernelGGL((k_page_plan<false>), dim3(grid), dim3(kPlanThreads), 0, st, a);
+        plan_launch<false>(a, st);
     }
     return check_launch("kv_page_plan");
 }

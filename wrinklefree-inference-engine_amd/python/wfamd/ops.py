@@ -422,13 +422,16 @@ def _int32_rows(name: str, what: str, t: torch.Tensor, n: Optional[int] = None) 
         raise ValueError(f"{name}: {what} must be a contiguous int32 [{'n' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a torch.cuda.Stream around it (2 us)
+
+
 def _call_on(dev: torch.device, name: str, *args) -> None:
     """Launch on dev's current stream, with dev current (kernels go to the device that is current)."""
     if dev.index == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+        call(name, *args, _raw_stream(dev.index))
         return
     with torch.cuda.device(dev):
-        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+        call(name, *args, _raw_stream(dev.index))
 
 
 class KVPagePlan(NamedTuple):
@@ -463,16 +466,15 @@ def kv_page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
     n, cols = int(num_tokens), page_table.shape[1]
     if n < 0:
         raise ValueError(f"kv_page_plan: num_tokens {n} is negative")
-    pad = (n + 3) // 4 * 4  # 16-byte steps between the arrays
-    out = torch.empty(4 * pad + b + 5, dtype=torch.int32, device=dev)
-    pages, slots, rows, pos, cu, counts = (out[i:i + m] for i, m in (
-        (0, n), (pad, n), (2 * pad, n), (3 * pad, n), (4 * pad + 4, b + 1), (4 * pad, 4)))
+    pad = -n % 4  # every array begins on a 16-byte line
+    out = torch.empty(4 * (n + pad) + b + 5, dtype=torch.int32, device=dev)
+    pages, _, slots, _, rows, _, pos, _, counts, cu = out.split([n, pad, n, pad, n, pad, n, pad, 4, b + 1])
     nws = int(_lib.load().wf_kv_page_plan_ws_bytes(b))
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    base = out.data_ptr()
+    base, step = out.data_ptr(), 4 * (n + pad)
     _call_on(dev, "wf_kv_page_plan", cached_lens.data_ptr(), new_lens.data_ptr(), b, free_pages.data_ptr(), free_pages.shape[0],
              page_table.data_ptr(), max(page_table.stride(0), cols) if b < 2 else page_table.stride(0), cols, int(page_size), n, base,
-             base + 4 * pad, base + 8 * pad, base + 12 * pad, base + 16 * pad + 16, base + 16 * pad, _ptr(ws))
+             base + step, base + 2 * step, base + 3 * step, base + 4 * step + 16, base + 4 * step, _ptr(ws))
     return KVPagePlan(pages, slots, rows, pos, cu, counts)
 
 
