@@ -108,6 +108,43 @@ struct LpList {
     }
 };
 
+// Candidates on their way to a list: packed into the wave's 64 places in LDS by a ballot and a lane count each, taken in
+// by one sort and merge when the places are full or at the end -- an insertion at a time costs 500 cycles of dependent
+// scalar and vector steps, a sort and merge of 64 about 4000.
+struct LpPlaces {
+    float v[64];
+    int i[64];
+};
+struct LpQueue {
+    LpPlaces& q;
+    int n;  // of the wave, in a scalar
+    __device__ __forceinline__ explicit LpQueue(LpPlaces& p) : q(p), n(0) {}
+    static __device__ __forceinline__ void meet() {  // LDS of one wave: its accesses are in order, the compiler's too
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    __device__ __forceinline__ void flush(LpList& l, int k) {
+        meet();
+        const int lane = threadIdx.x & 63;
+        const bool in = lane < n;
+        const float v = in ? q.v[lane] : -INFINITY;
+        const int i = in ? q.i[lane] : 0x7fffffff;
+        meet();
+        n = 0;
+        l.add(v, i, k);
+    }
+    // the lanes' (v, i) where `in`; the caller flushes
+    __device__ __forceinline__ bool full(uint64_t in) const { return n + __builtin_popcountll(in) > 64; }
+    __device__ __forceinline__ void push(uint64_t in, float v, int i) {
+        if (in >> (threadIdx.x & 63) & 1) {
+            const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+            q.v[at] = v;
+            q.i[at] = i;
+        }
+        n += __builtin_popcountll(in);
+    }
+};
+
 template <int DT>
 struct LpElem;  // logit type, logits of a 16-byte vector
 template <>
@@ -115,6 +152,13 @@ struct LpElem<DT_F32> {
     using T = float;
     static constexpr int N = 4;
     static __device__ __forceinline__ float up(T v) { return v; }
+    static __device__ __forceinline__ uint32_t bits(T v) { return __float_as_uint(v); }
+    // the vector's first logit; the vector without it
+    static __device__ __forceinline__ float pop(uint4& w) {
+        const float x = __uint_as_float(w.x);
+        w = make_uint4(w.y, w.z, w.w, 0);
+        return x;
+    }
     static __device__ __forceinline__ void unpack(uint4 w, float (&x)[N]) {
         x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
     }
@@ -124,6 +168,13 @@ struct LpElem<DT_BF16> {
     using T = uint16_t;
     static constexpr int N = 8;
     static __device__ __forceinline__ float up(T v) { return bf2f(v); }
+    static __device__ __forceinline__ uint32_t bits(T v) { return v; }
+    static __device__ __forceinline__ float pop(uint4& w) {
+        const float x = bf2f(w.x & 0xffffu);
+        w = make_uint4(__builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16), __builtin_amdgcn_alignbit(w.w, w.z, 16),
+                       w.w >> 16);
+        return x;
+    }
     static __device__ __forceinline__ void unpack(uint4 w, float (&x)[N]) {
         const uint32_t d[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -135,6 +186,13 @@ struct LpElem<DT_F16> {
     using T = uint16_t;
     static constexpr int N = 8;
     static __device__ __forceinline__ float up(T v) { return h2f(v); }
+    static __device__ __forceinline__ uint32_t bits(T v) { return v; }
+    static __device__ __forceinline__ float pop(uint4& w) {
+        const float x = h2f(w.x & 0xffffu);
+        w = make_uint4(__builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16), __builtin_amdgcn_alignbit(w.w, w.z, 16),
+                       w.w >> 16);
+        return x;
+    }
     static __device__ __forceinline__ void unpack(uint4 w, float (&x)[N]) {
         const uint32_t d[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -226,6 +284,7 @@ template <int DT, bool TOP, bool TOK>
 __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     using E = LpElem<DT>;
     constexpr int N = E::N, U = kLpUnroll;
+    __shared__ LpPlaces places[4];
     const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
     if (w >= a.R * a.S) return;
     const int r = w / a.S, s = w - r * a.S;
@@ -245,17 +304,19 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
         }
     }
     LpSums sum;
-    LpList groups, elems;
+    LpList groups;
     int rank = 0;  // of the wave, in a scalar
     // head and tail logits
+    const int edge = lane < head ? lo + lane : lane < head + hi - tail ? tail + lane - head : -1;
+    typename E::T edge_x = 0;
     {
-        const int j = lane < head ? lo + lane : lane < head + hi - tail ? tail + lane - head : -1;
-        const float x = j >= 0 ? E::up(row[j]) : -INFINITY;
+        const int j = edge;
+        if (j >= 0) edge_x = row[j];
+        const float x = j >= 0 ? E::up(edge_x) : -INFINITY;
         sum.raise(x);
         const float one[1] = {x};
         sum.add(one);
         if constexpr (TOK) rank += __builtin_popcountll(__ballot(tok >= 0 && j >= 0 && (x > xt || (x == xt && j < tok))));
-        if constexpr (TOP) elems.add(x, j >= 0 ? j : 0x7fffffff, a.k);
     }
     const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
     uint4 nx[U];
@@ -323,28 +384,33 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     const int64_t at = (int64_t)r * a.S + s;
     if (lane == 0) a.part[at] = LpPart{sum.m, sum.z, sum.t, rank};
     if constexpr (TOP) {
-        // the k best groups again, a vector a lane: 16 groups a load, all of them under way before the first is looked at
-        constexpr int M = kLpMaxTop / 16;
-        uint4 w[M];
-        int at_vec[M];
-#pragma unroll
-        for (int i = 0; i < M; ++i) {
-            const int e = 16 * i + (lane >> 2), g = __shfl(groups.i, e, 64);
-            at_vec[i] = e < a.k && g != 0x7fffffff && 4 * g + (lane & 3) < nv ? 4 * g + (lane & 3) : -1;
-            if (at_vec[i] >= 0) w[i] = vec[at_vec[i]];
-        }
+        // the k best groups again, a vector a lane, 16 groups a load, and before them the head and tail logits; one copy of
+        // the list's code in a rolled loop: unrolled, fetching instructions took longer than running them
         const float least = groups.last_v(a.k);  // k maxima reach it: nothing below it is among the k first
-#pragma unroll
-        for (int i = 0; i < M; ++i) {
-            if (16 * i >= a.k) break;
-            float x[N];
-            E::unpack(w[i], x);
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const bool in = at_vec[i] >= 0 && x[e] >= least;
-                elems.add(in ? x[e] : -INFINITY, in ? v0 + at_vec[i] * N + e : 0x7fffffff, a.k);
+        LpList elems;
+        auto fetch = [&](int i, uint4& w, int& j) {
+            const int e = 16 * i + (lane >> 2), g = __shfl(groups.i, e, 64), vi = 4 * g + (lane & 3);
+            j = e < a.k && g != 0x7fffffff && vi < nv ? v0 + vi * N : -1;
+            if (j >= 0) w = vec[vi];
+        };
+        uint4 w = make_uint4(E::bits(edge_x), 0, 0, 0), w1 = w;
+        int j = edge, n = 1, j1;
+        fetch(0, w1, j1);
+        LpQueue queue(places[threadIdx.x >> 6]);
+#pragma unroll 1
+        for (int i = 1;; ++i) {
+#pragma unroll 1
+            for (int e = 0; e < n; ++e) {
+                const float x = E::pop(w);
+                const uint64_t in = __ballot(j >= 0 && x >= least);
+                if (queue.full(in)) queue.flush(elems, a.k);
+                queue.push(in, x, j + e);
             }
+            if (16 * (i - 1) >= a.k) break;
+            w = w1, j = j1, n = N;
+            if (16 * i < a.k) fetch(i, w1, j1);
         }
+        queue.flush(elems, a.k);
         if (lane < a.k) {
             a.list_v[at * a.k + lane] = elems.v;
             a.list_i[at * a.k + lane] = elems.i;
@@ -355,6 +421,7 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
 template <int DT>
 __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     using E = LpElem<DT>;
+    __shared__ LpPlaces places[4];
     const int r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
     if (r >= a.R) return;
     const int64_t at = (int64_t)r * a.S;
@@ -379,18 +446,31 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     if (a.k == 0) return;
     // the chunks' sorted lists, a lane each, from the front until no front can enter
     LpList top;
-    for (int i = 0; i < a.k; i += 4) {
-        float v[4];
-        int j[4];
+    const float* lv = a.list_v + (at + lane) * a.k;
+    const int* li = a.list_i + (at + lane) * a.k;
+    auto fetch = [&](int i, float& v, int& j) {
+        v = -INFINITY, j = 0x7fffffff;
+        if (lane < a.S && i < a.k) v = lv[i], j = li[i];
+    };
+    float v[3];
+    int j[3];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] = -INFINITY, j[e] = 0x7fffffff;
-            if (lane < a.S && i + e < a.k) v[e] = a.list_v[(at + lane) * a.k + i + e], j[e] = a.list_i[(at + lane) * a.k + i + e];
-        }
-        if (!__ballot(LpList::before(v[0], j[0], top.last_v(a.k), top.last_i(a.k)))) break;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top.add(v[e], j[e], a.k);
+    for (int e = 0; e < 3; ++e) fetch(e, v[e], j[e]);
+    // the heads first; what comes before the k-th of them is all that can still enter, and it stands at the lists' fronts
+    top.add(v[0], j[0], a.k);
+    const float least = top.last_v(a.k);
+    const int least_i = top.last_i(a.k);
+    LpQueue queue(places[threadIdx.x >> 6]);
+#pragma unroll 1
+    for (int i = 1; i < a.k; ++i) {
+        const uint64_t in = __ballot(LpList::before(v[1], j[1], least, least_i));
+        if (!in) break;
+        if (queue.full(in)) queue.flush(top, a.k);
+        queue.push(in, v[1], j[1]);
+        v[1] = v[2], j[1] = j[2];
+        fetch(i + 2, v[2], j[2]);
     }
+    queue.flush(top, a.k);
     if (lane < a.k) {
         const bool in = top.i != 0x7fffffff;  // no: fewer than k logits of the row are numbers
         a.top_i[(int64_t)r * a.k + lane] = in ? top.i : -1;
