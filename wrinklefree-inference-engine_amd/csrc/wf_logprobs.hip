@@ -42,83 +42,80 @@ __device__ __forceinline__ int lp_xor(int v) {
     else if constexpr (X == 15) return dpp_i<DPP_MIRROR>(v);
     else return __shfl_xor(v, X, 64);
 }
+template <int X>
+__device__ __forceinline__ double lp_xor(double v) {
+    return __hiloint2double(lp_xor<X>(__double2hiint(v)), lp_xor<X>(__double2loint(v)));
+}
 constexpr int kDppWaveShr1 = 0x138;  // lane l reads lane l - 1
 
-// The wave's best (value, index) so far, sorted across lanes: value descending, lower index first.
-// Empty places hold (-inf, INT_MAX), behind every real entry; a NaN never enters.
+// A logit and its index as one key that orders them (value descending, lower index first, +0 = -0), so that a step of a sort
+// is one max and one min: 32 bits in the values' order above 2^31 - 1 - index, read as a double. From -inf to
+// +inf these are positive normal doubles (exponents 3 to 0x7fc); 0 stands for no entry, and for NaN.
+__device__ __forceinline__ double lp_key(float v, int i) {
+    const uint32_t b = __float_as_uint(v + 0.f), o = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+    return v == v ? __longlong_as_double((long long)((uint64_t)o << 31 | (uint32_t)(0x7fffffff - i))) : 0.;
+}
+__device__ __forceinline__ float lp_value(double k) {
+    const uint32_t o = (uint32_t)((uint64_t)__double_as_longlong(k) >> 31);
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+__device__ __forceinline__ int lp_index(double k) { return 0x7fffffff - (int)(__double2loint(k) & 0x7fffffff); }
+
+// The wave's greatest keys so far, descending across its lanes.
 struct LpList {
-    float v;
-    int i;
-    __device__ __forceinline__ LpList() : v(-INFINITY), i(0x7fffffff) {}
-    static __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
-    // one step of a bitonic network: of lanes l and l ^ X, the one without bit BIT keeps the entry that comes first
+    double v;
+    __device__ __forceinline__ LpList() : v(0.) {}
+    // one step of a bitonic network: of lanes l and l ^ X, the one without bit BIT keeps the greater key
     template <int X, int BIT>
-    static __device__ __forceinline__ void step(float& v, int& i) {
-        const float w = __int_as_float(lp_xor<X>(__float_as_int(v)));
-        const int j = lp_xor<X>(i);
-        const bool keep = before(v, i, w, j) != ((threadIdx.x & BIT) != 0);
-        v = keep ? v : w;
-        i = keep ? i : j;
+    static __device__ __forceinline__ void step(double& v) {
+        const double w = lp_xor<X>(v), hi = __builtin_fmax(v, w), lo = __builtin_fmin(v, w);
+        v = threadIdx.x & BIT ? lo : hi;
     }
     template <int X>
-    static __device__ __forceinline__ void clean(float& v, int& i) {
-        step<X, X>(v, i);
-        if constexpr (X > 1) clean<X / 2>(v, i);
+    static __device__ __forceinline__ void clean(double& v) {
+        step<X, X>(v);
+        if constexpr (X > 1) clean<X / 2>(v);
     }
-    static __device__ __forceinline__ void sort(float& v, int& i) {
-        step<1, 1>(v, i);
-        step<3, 2>(v, i), clean<1>(v, i);
-        step<7, 4>(v, i), clean<2>(v, i);
-        step<15, 8>(v, i), clean<4>(v, i);
-        step<31, 16>(v, i), clean<8>(v, i);
-        step<63, 32>(v, i), clean<16>(v, i);
+    static __device__ __forceinline__ void sort(double& v) {
+        step<1, 1>(v);
+        step<3, 2>(v), clean<1>(v);
+        step<7, 4>(v), clean<2>(v);
+        step<15, 8>(v), clean<4>(v);
+        step<31, 16>(v), clean<8>(v);
+        step<63, 32>(v), clean<16>(v);
     }
-    // entry k - 1
-    __device__ __forceinline__ float last_v(int k) const { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), k - 1)); }
-    __device__ __forceinline__ int last_i(int k) const { return __builtin_amdgcn_readlane(i, k - 1); }
-    // Takes in the candidates (one a lane) that come before entry k - 1: many by a sort and a merge (27 steps of the
-    // network), few one after the other.
-    __device__ __forceinline__ void add(float cv, int ci, int k) {
-        uint64_t todo = __ballot(before(cv, ci, last_v(k), last_i(k)));
-        if (__builtin_popcountll(todo) > 16) {
-            const bool in = todo >> (threadIdx.x & 63) & 1;
-            cv = in ? cv : -INFINITY;
-            ci = in ? ci : 0x7fffffff;
-            sort(cv, ci);
-            const float w = __int_as_float(lp_xor<63>(__float_as_int(cv)));
-            const int j = lp_xor<63>(ci);
-            const bool keep = before(v, i, w, j);  // the first 64 of both lists, a bitonic sequence
-            v = keep ? v : w;
-            i = keep ? i : j;
-            clean<32>(v, i);
+    static __device__ __forceinline__ double lane(double v, int l) {
+        return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l));
+    }
+    __device__ __forceinline__ double last(int k) const { return lane(v, k - 1); }  // entry k - 1
+    // Takes in the candidates (one a lane) above entry k - 1: many by a sort and a merge (27 steps of the network), few one
+    // after the other.
+    __device__ __forceinline__ void add(double c, int k) {
+        uint64_t todo = __ballot(c > last(k));
+        if (__builtin_popcountll(todo) > 8) {
+            c = todo >> (threadIdx.x & 63) & 1 ? c : 0.;
+            sort(c);
+            v = __builtin_fmax(v, lp_xor<63>(c));  // the first 64 of both lists, a bitonic sequence
+            clean<32>(v);
             return;
         }
         while (todo) {
-            const int l = __builtin_ctzll(todo);
-            const float nv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(cv), l));
-            const int ni = __builtin_amdgcn_readlane(ci, l);
-            const int at = __builtin_popcountll(__ballot(before(v, i, nv, ni))), lane = threadIdx.x & 63;
-            const float pv = dpp_f<kDppWaveShr1>(v, v);
-            const int pi = dpp_i<kDppWaveShr1>(i, i);
-            v = lane < at ? v : lane == at ? nv : pv;
-            i = lane < at ? i : lane == at ? ni : pi;
+            const double n = lane(c, __builtin_ctzll(todo));
+            const int at = __builtin_popcountll(__ballot(v > n)), l = threadIdx.x & 63;
+            const double p = __hiloint2double(dpp_i<kDppWaveShr1>(__double2hiint(v)), dpp_i<kDppWaveShr1>(__double2loint(v)));
+            v = l < at ? v : l == at ? n : p;
             todo &= todo - 1;
-            todo &= __ballot(before(cv, ci, last_v(k), last_i(k)));
+            todo &= __ballot(c > last(k));
         }
     }
 };
 
 // Candidates on their way to a list: packed into the wave's 64 places in LDS by a ballot and a lane count each, taken in
-// by one sort and merge when the places are full or at the end -- an insertion at a time costs 500 cycles of dependent
-// scalar and vector steps, a sort and merge of 64 about 4000.
-struct LpPlaces {
-    float v[64];
-    int i[64];
-};
+// together when the places are full or at the end.
 struct LpQueue {
-    LpPlaces& q;
+    double* q;
     int n;  // of the wave, in a scalar
-    __device__ __forceinline__ explicit LpQueue(LpPlaces& p) : q(p), n(0) {}
+    __device__ __forceinline__ explicit LpQueue(double* places) : q(places), n(0) {}
     static __device__ __forceinline__ void meet() {  // LDS of one wave: its accesses are in order, the compiler's too
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -126,21 +123,15 @@ struct LpQueue {
     __device__ __forceinline__ void flush(LpList& l, int k) {
         meet();
         const int lane = threadIdx.x & 63;
-        const bool in = lane < n;
-        const float v = in ? q.v[lane] : -INFINITY;
-        const int i = in ? q.i[lane] : 0x7fffffff;
+        const double c = lane < n ? q[lane] : 0.;
         meet();
         n = 0;
-        l.add(v, i, k);
+        l.add(c, k);
     }
-    // the lanes' (v, i) where `in`; the caller flushes
-    __device__ __forceinline__ bool full(uint64_t in) const { return n + __builtin_popcountll(in) > 64; }
-    __device__ __forceinline__ void push(uint64_t in, float v, int i) {
-        if (in >> (threadIdx.x & 63) & 1) {
-            const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
-            q.v[at] = v;
-            q.i[at] = i;
-        }
+    // the lanes' keys where `in`
+    __device__ __forceinline__ void push(uint64_t in, double c, LpList& l, int k) {
+        if (n + __builtin_popcountll(in) > 64) flush(l, k);
+        if (in >> (threadIdx.x & 63) & 1) q[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0))] = c;
         n += __builtin_popcountll(in);
     }
 };
@@ -207,8 +198,7 @@ struct LpArgs {
     const void* tok;
     int tok64, k;
     LpPart* part;   // [R][S]
-    float* list_v;  // [R][S][k]
-    int* list_i;
+    double* list;   // [R][S][k] keys
     float *lp, *ent, *top_v;
     int *rank, *top_i;
 };
@@ -284,7 +274,7 @@ template <int DT, bool TOP, bool TOK>
 __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     using E = LpElem<DT>;
     constexpr int N = E::N, U = kLpUnroll;
-    __shared__ LpPlaces places[4];
+    __shared__ double places[4][64];
     const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
     if (w >= a.R * a.S) return;
     const int r = w / a.S, s = w - r * a.S;
@@ -305,6 +295,7 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     }
     LpSums sum;
     LpList groups;
+    LpQueue queue(places[threadIdx.x >> 6]);
     int rank = 0;  // of the wave, in a scalar
     // head and tail logits
     const int edge = lane < head ? lo + lane : lane < head + hi - tail ? tail + lane - head : -1;
@@ -322,7 +313,7 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     uint4 nx[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-        if (u * 64 + lane < nv) nx[u] = vec[u * 64 + lane];
+        if (u * 64 + lane < nv) nx[u] = ldg_nt(reinterpret_cast<const uint8_t*>(vec + u * 64 + lane));
     for (int base = 0; base < nv; base += 64 * U) {
         uint4 cur[U];
 #pragma unroll
@@ -330,7 +321,7 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {  // the next tile's vectors are under way while this one is summed
             const int i = base + (U + u) * 64 + lane;
-            if (i < nv) nx[u] = vec[i];
+            if (i < nv) nx[u] = ldg_nt(reinterpret_cast<const uint8_t*>(vec + i));  // read once
         }
         float x[U][N], vm[U], tm = -INFINITY;
         const bool whole = base + 64 * U <= nv;
@@ -377,7 +368,9 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
                 if ((lane & 3) == u) gm = m;
             }
             const int g = (base >> 2) + (lane & 3) * 16 + (lane >> 2);
-            groups.add(gm, 4 * g < nv ? g : 0x7fffffff, a.k);
+            const double c = 4 * g < nv ? lp_key(gm, g) : 0.;
+            const uint64_t in = __ballot(c > groups.last(a.k));
+            if (in) queue.push(in, c, groups, a.k);
         }
     }
     sum.join();
@@ -386,42 +379,42 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     if constexpr (TOP) {
         // the k best groups again, a vector a lane, 16 groups a load, and before them the head and tail logits; one copy of
         // the list's code in a rolled loop: unrolled, fetching instructions took longer than running them
-        const float least = groups.last_v(a.k);  // k maxima reach it: nothing below it is among the k first
+        queue.flush(groups, a.k);
+        // k maxima reach the k-th: nothing below it is among the k first
+        const double kth = groups.last(a.k);
+        const float least = kth > 0. ? lp_value(kth) : -INFINITY;
         LpList elems;
         auto fetch = [&](int i, uint4& w, int& j) {
-            const int e = 16 * i + (lane >> 2), g = __shfl(groups.i, e, 64), vi = 4 * g + (lane & 3);
-            j = e < a.k && g != 0x7fffffff && vi < nv ? v0 + vi * N : -1;
+            const int e = 16 * i + (lane >> 2);
+            const double c = __shfl(groups.v, e, 64);
+            const int vi = 4 * lp_index(c) + (lane & 3);
+            j = e < a.k && c > 0. && vi < nv ? v0 + vi * N : -1;
             if (j >= 0) w = vec[vi];
         };
         uint4 w = make_uint4(E::bits(edge_x), 0, 0, 0), w1 = w;
         int j = edge, n = 1, j1;
         fetch(0, w1, j1);
-        LpQueue queue(places[threadIdx.x >> 6]);
 #pragma unroll 1
         for (int i = 1;; ++i) {
 #pragma unroll 1
             for (int e = 0; e < n; ++e) {
                 const float x = E::pop(w);
                 const uint64_t in = __ballot(j >= 0 && x >= least);
-                if (queue.full(in)) queue.flush(elems, a.k);
-                queue.push(in, x, j + e);
+                if (in) queue.push(in, lp_key(x, j + e), elems, a.k);
             }
             if (16 * (i - 1) >= a.k) break;
             w = w1, j = j1, n = N;
             if (16 * i < a.k) fetch(i, w1, j1);
         }
         queue.flush(elems, a.k);
-        if (lane < a.k) {
-            a.list_v[at * a.k + lane] = elems.v;
-            a.list_i[at * a.k + lane] = elems.i;
-        }
+        if (lane < a.k) a.list[at * a.k + lane] = elems.v;
     }
 }
 
 template <int DT>
 __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     using E = LpElem<DT>;
-    __shared__ LpPlaces places[4];
+    __shared__ double places[4][64];
     const int r = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
     if (r >= a.R) return;
     const int64_t at = (int64_t)r * a.S;
@@ -446,35 +439,26 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     if (a.k == 0) return;
     // the chunks' sorted lists, a lane each, from the front until no front can enter
     LpList top;
-    const float* lv = a.list_v + (at + lane) * a.k;
-    const int* li = a.list_i + (at + lane) * a.k;
-    auto fetch = [&](int i, float& v, int& j) {
-        v = -INFINITY, j = 0x7fffffff;
-        if (lane < a.S && i < a.k) v = lv[i], j = li[i];
-    };
-    float v[3];
-    int j[3];
-#pragma unroll
-    for (int e = 0; e < 3; ++e) fetch(e, v[e], j[e]);
+    const double* list = a.list + (at + lane) * a.k;
+    auto fetch = [&](int i) { return lane < a.S && i < a.k ? list[i] : 0.; };
+    double c0 = fetch(0), c1 = fetch(1), c2 = fetch(2);
     // the heads first; what comes before the k-th of them is all that can still enter, and it stands at the lists' fronts
-    top.add(v[0], j[0], a.k);
-    const float least = top.last_v(a.k);
-    const int least_i = top.last_i(a.k);
+    top.add(c0, a.k);
+    const double least = top.last(a.k);
     LpQueue queue(places[threadIdx.x >> 6]);
 #pragma unroll 1
     for (int i = 1; i < a.k; ++i) {
-        const uint64_t in = __ballot(LpList::before(v[1], j[1], least, least_i));
+        const uint64_t in = __ballot(c1 > least);
         if (!in) break;
-        if (queue.full(in)) queue.flush(top, a.k);
-        queue.push(in, v[1], j[1]);
-        v[1] = v[2], j[1] = j[2];
-        fetch(i + 2, v[2], j[2]);
+        queue.push(in, c1, top, a.k);
+        c1 = c2;
+        c2 = fetch(i + 2);
     }
     queue.flush(top, a.k);
     if (lane < a.k) {
-        const bool in = top.i != 0x7fffffff;  // no: fewer than k logits of the row are numbers
-        a.top_i[(int64_t)r * a.k + lane] = in ? top.i : -1;
-        a.top_v[(int64_t)r * a.k + lane] = !in ? NAN : empty ? -INFINITY : top.v - sum.m - ln_z;
+        const bool in = top.v > 0.;  // no: fewer than k logits of the row are numbers
+        a.top_i[(int64_t)r * a.k + lane] = in ? lp_index(top.v) : -1;
+        a.top_v[(int64_t)r * a.k + lane] = !in ? NAN : empty ? -INFINITY : lp_value(top.v) - sum.m - ln_z;
     }
 }
 
@@ -520,9 +504,7 @@ int wf_token_logprobs(const void* logits, int dtype, int64_t ld, int R, int V, c
     WF_REQUIRE((int64_t)R * S <= 0x7fffffff - 4, "token_logprobs: too many rows");
     const int chunk = (int)((((int64_t)V + S - 1) / S + 31) / 32 * 32);
     LpPart* part = reinterpret_cast<LpPart*>(ws);
-    float* list_v = reinterpret_cast<float*>(part + (int64_t)R * S);
-    int* list_i = reinterpret_cast<int*>(list_v + (int64_t)R * S * top_k);
-    LpArgs a{logits, ld, R, V, S, chunk, tokens, tokens64, top_k, part, list_v, list_i, logprobs, entropy, top_logprobs, ranks, top_ids};
+    LpArgs a{logits, ld, R, V, S, chunk, tokens, tokens64, top_k, part, reinterpret_cast<double*>(part + (int64_t)R * S), logprobs, entropy, top_logprobs, ranks, top_ids};
     hipStream_t st = as_stream(stream);
     if (dtype == WF_F32) lp_launch<DT_F32>(a, st);
     else if (dtype == WF_BF16) lp_launch<DT_BF16>(a, st);
