@@ -40,6 +40,7 @@ constexpr float kPfLn2 = 0.69314718055994530942f;
 struct PfArgs {
     const void* q;
     int64_t q_sb, q_sh;
+    int qvec;  // q's rows are 16-byte aligned
     const uint8_t *K, *V;
     int64_t pgs, hs;  // bytes from page to page and from head to head
     int np;
@@ -64,11 +65,13 @@ struct PfSeq {
     __device__ __forceinline__ bool same(const PfSeq& s) const { return P > 0 && P == s.P && owner == s.owner; }
 };
 __device__ __forceinline__ PfSeq pf_seq(const PfArgs& a, int b) {
-    PfSeq s{0, 0, -1};
-    if (b < 0 || b >= a.B) return s;
-    s.L = min(max(a.lens[b], 0), a.cols * kPfPage);
-    s.owner = a.owners[b];
-    if (s.owner >= 0 && s.owner < a.B) s.P = min(max(a.plens[b], 0), s.L);
+    const bool in = b >= 0 && b < a.B;
+    const int i = in ? b : 0;  // no branch around the loads: three sequences' lengths are fetched at once
+    const int len = a.lens[i], owner = a.owners[i], plen = a.plens[i];
+    PfSeq s;
+    s.L = in ? min(max(len, 0), a.cols * kPfPage) : 0;
+    s.owner = in ? owner : -1;
+    s.P = owner >= 0 && owner < a.B ? min(max(plen, 0), s.L) : 0;
     return s;
 }
 // Whether b's prefix is read together with a neighbour's (all three launches ask this).
@@ -106,52 +109,81 @@ struct PfState {
             for (int n = 0; n < 8; ++n) acc[t][n] = pf_f4{0.f, 0.f, 0.f, 0.f};
         }
     }
-    // fragment c of tile t's row: dims 32 c + 8 q4 ..
+    // tile t's row; fragment c: dims 32 c + 8 q4 ..; vec: the row is 16-byte aligned
     template <int QDT>
-    __device__ __forceinline__ void load_q(int t, const void* row, float neg) {
+    __device__ __forceinline__ void load_q(int t, const uint8_t* row, float neg, bool vec) {
         const int q4 = (threadIdx.x & 63) >> 4;
+        float x[4][8];
+        if (vec) {
+            constexpr int W = QDT == DT_F32 ? 2 : 1;
+            uint4 w[4][W];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < W; ++i) w[c][i] = reinterpret_cast<const uint4*>(row)[(4 * c + q4) * W + i];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const uint32_t d[4] = {w[c][i].x, w[c][i].y, w[c][i].z, w[c][i].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (QDT == DT_F32) x[c][4 * i + e] = __uint_as_float(d[e]);
+                        else if constexpr (QDT == DT_BF16) x[c][2 * e] = bf_lo(d[e]), x[c][2 * e + 1] = bf_hi(d[e]);
+                        else x[c][2 * e] = h2f(d[e] & 0xffffu), x[c][2 * e + 1] = h2f(d[e] >> 16);
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[c][e] = load_as_f32(row, 32 * c + 8 * q4 + e, QDT);
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = neg * load_as_f32(row, 32 * c + 8 * q4 + e, QDT);
+            for (int e = 0; e < 8; ++e) x[c][e] *= neg;
 #pragma unroll
             for (int k = 0; k < NQ; ++k) {
                 pf_bf8 v;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[e] = (__bf16)x[e];
-                    x[e] -= (float)v[e];
+                    v[e] = (__bf16)x[c][e];
+                    x[c][e] -= (float)v[e];
                 }
                 q[t][k][c] = v;
             }
         }
     }
-    // One 32-key tile; keys outside [lo, hi) of it are masked. K and V fragments of this lane.
+    using Scores = pf_f4[NT][2];
+    // scores of a 32-key tile: lane (row l16, quarter q4) gets keys 8 q4 + 4 h + r in s[t][h][r]
     template <int KVQ>
-    __device__ __forceinline__ void tile(const typename PfFrag<KVQ>::T (&kf)[8], const typename PfFrag<KVQ>::T (&vf)[8], int lo, int hi,
-                                         float sc, unsigned live) {
+    __device__ __forceinline__ void scores(const typename PfFrag<KVQ>::T (&kf)[8], Scores& s) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = pf_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const pf_bf8 k0 = __builtin_bit_cast(pf_bf8, PfFrag<KVQ>::bf(kf[c])), k1 = __builtin_bit_cast(pf_bf8, PfFrag<KVQ>::bf(kf[4 + c]));
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int k = NQ - 1; k >= 0; --k) {
+                        s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[t][k][c], s[t][0], 0, 0, 0);
+                        s[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[t][k][c], s[t][1], 0, 0, 0);
+                    }
+        }
+    }
+    // scores -> probabilities in the rows' frames; keys outside [lo, hi) of the tile are masked
+    __device__ __forceinline__ void softmax(const Scores& s, pf_bf8 (&p)[NT][NPT], int lo, int hi, float sc) {
         const int key = (threadIdx.x & 63) >> 4 << 3;  // this lane's keys: key .. key + 7
         const bool whole = lo <= 0 && hi >= kPfPage;
-        pf_bf8 kb[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) kb[i] = __builtin_bit_cast(pf_bf8, PfFrag<KVQ>::bf(kf[i]));
-        pf_bf8 p[NT][NPT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            if (!(live >> t & 1)) continue;
-            pf_f4 s[2] = {pf_f4{0.f, 0.f, 0.f, 0.f}, pf_f4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int k = NQ - 1; k >= 0; --k) {
-                    s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[c], q[t][k][c], s[0], 0, 0, 0);
-                    s[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[4 + c], q[t][k][c], s[1], 0, 0, 0);
-                }
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3];
+            for (int e = 0; e < 8; ++e) x[e] = s[t][e >> 2][e & 3];
             if (!whole) {
+                asm volatile("");  // a branch, not selects on every tile
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = key + e >= lo && key + e < hi ? x[e] : -INFINITY;
             }
@@ -159,66 +191,99 @@ struct PfState {
             if (__any(mx > m[t] + 8.f)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m[t]);
-                const float nf = mx == -INFINITY ? 0.f : mx, r = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(f[t] - nf);
+                const float nf = mx == -INFINITY ? 0.f : mx;
                 // (an empty sum stays, also when it is NaN: it holds no finite score to rescale)
-                if (m[t] != -INFINITY) {
-                    l[t] *= r;
+                const float r = m[t] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(f[t] - nf);
+                l[t] *= r;
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) acc[t][n] *= r;
-                }
+                for (int n = 0; n < 8; ++n) acc[t][n] *= r;
                 m[t] = mx;
                 f[t] = nf;
             }
-            float e8[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) e8[e] = __builtin_amdgcn_exp2f(fmaf(x[e], sc, -f[t]));
-            l[t] += ((e8[0] + e8[1]) + (e8[2] + e8[3])) + ((e8[4] + e8[5]) + (e8[6] + e8[7]));
+            for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], sc, -f[t]));
+            l[t] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
             for (int k = 0; k < NPT; ++k)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    p[t][k][e] = (__bf16)e8[e];
-                    if (k + 1 < NPT) e8[e] -= (float)p[t][k][e];
+                    p[t][k][e] = (__bf16)x[e];
+                    if (k + 1 < NPT) x[e] -= (float)p[t][k][e];
                 }
+        }
+    }
+    // o += P V
+    template <int KVQ>
+    __device__ __forceinline__ void values(const typename PfFrag<KVQ>::T (&vf)[8], const pf_bf8 (&p)[NT][NPT], int lo, int hi) {
+        const int key = (threadIdx.x & 63) >> 4 << 3;
+        const bool whole = lo <= 0 && hi >= kPfPage;
+        uint4 v[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) v[n] = PfFrag<KVQ>::bf(vf[n]);
+        if (!whole) {  // a masked key's V may hold anything: 0 x NaN is NaN
+            asm volatile("");
+            uint32_t mask[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k0 = key + 2 * j;
+                mask[j] = (k0 >= lo && k0 < hi ? 0xffffu : 0u) | (k0 + 1 >= lo && k0 + 1 < hi ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) v[n] = make_uint4(v[n].x & mask[0], v[n].y & mask[1], v[n].z & mask[2], v[n].w & mask[3]);
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
-            uint4 v = PfFrag<KVQ>::bf(vf[n]);
-            if (!whole) {  // a masked key's V may hold anything: 0 x NaN is NaN
-                uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int k0 = key + 2 * j;
-                    w[j] &= (k0 >= lo && k0 < hi ? 0xffffu : 0u) | (k0 + 1 >= lo && k0 + 1 < hi ? 0xffff0000u : 0u);
-                }
-                v = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-            const pf_bf8 vb = __builtin_bit_cast(pf_bf8, v);
+            const pf_bf8 vb = __builtin_bit_cast(pf_bf8, v[n]);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
-                if (live >> t & 1)
 #pragma unroll
                     for (int k = NPT - 1; k >= 0; --k) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p[t][k], acc[t][n], 0, 0, 0);
         }
     }
 };
 
-// Where a tile of the walk lies: the pool's block of its page and head, the valid keys of it.
-struct PfAt {
-    int64_t off;  // byte offset; < 0: no such page, every key masked
-    int lo, hi;
-};
-template <int KVQ>
-__device__ __forceinline__ void pf_load(const PfArgs& a, const PfAt& at, typename PfFrag<KVQ>::T (&kf)[8], typename PfFrag<KVQ>::T (&vf)[8]) {
-    using F = PfFrag<KVQ>;
-    if (at.off < 0) return;
-    const int lane = threadIdx.x & 63;
-    const typename F::T* k = reinterpret_cast<const typename F::T*>(a.K + at.off) + lane;
-    const typename F::T* v = reinterpret_cast<const typename F::T*>(a.V + at.off) + lane;
+// One wave's walk over tiles k0, k0 + 4, .. below k1: page(k) is the page of tile k (per lane, k may differ by lane),
+// range(k, lo, hi) its valid keys. 64 page ids are fetched at a time, a lane each. The next tile's K is under way from
+// the moment this one's scores are done, its V from the moment this one's products are: one set of registers,
+// and half a tile's work over each load's latency.
+template <int KVQ, int NT, int NQ, class Page, class Range>
+__device__ __forceinline__ void pf_walk(const PfArgs& a, PfState<NT, NQ, NQ>& st, int64_t head, int k0, int k1, Page page, Range range) {
+    using T = typename PfFrag<KVQ>::T;
+    const int lane = threadIdx.x & 63, n = (k1 - k0 + 3) / 4;
+    if (n <= 0) return;
+    T kf[8], vf[8];
+    int ids = -1;
+    // the id of tile number i (0, 1, ..) of the walk; < 0 where the pool has no such page
+    auto find = [&](int i) {
+        if ((i & 63) == 0) {
+            const int k = k0 + 4 * (i + lane);
+            ids = k < k1 ? page(k) : -1;
+            ids = ids < a.np ? ids : -1;
+        }
+        return __builtin_amdgcn_readlane(ids, i & 63);
+    };
+    auto load = [&](int id, const uint8_t* pool, T (&f)[8]) {
+        const T* p = reinterpret_cast<const T*>(pool + max(id, 0) * a.pgs + head) + lane;  // no such page: page 0, masked
 #pragma unroll
-    for (int i = 0; i < 8; ++i) kf[i] = k[64 * i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) vf[i] = v[64 * i];
+        for (int e = 0; e < 8; ++e) f[e] = p[64 * e];
+    };
+    int id = find(0);
+    load(id, a.K, kf);
+    load(id, a.V, vf);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        int lo, hi;
+        range(k0 + 4 * i, lo, hi);
+        if (id < 0) hi = 0;
+        id = i + 1 < n ? find(i + 1) : -1;
+        pf_f4 s[NT][2];
+        pf_bf8 p[NT][NQ];
+        st.template scores<KVQ>(kf, s);
+        load(id, a.K, kf);
+        st.softmax(s, p, lo, hi, a.sc);
+        st.template values<KVQ>(vf, p, lo, hi);
+        load(id, a.V, vf);
+    }
 }
 
 // The four waves' states of one column tile -> one record a row. sm: 4 x 16 rows of 132 floats + 4 x 16 (m, l).
@@ -260,34 +325,48 @@ __device__ __forceinline__ void pf_merge(const PfArgs& a, PfShared& sm, const pf
 }
 
 // ---------------------------------------------------------------------------------------------
-// Shared prefixes. Grid (kv head and key range, rounded up to 8, tile of 16 NT rows): the row tiles of one (head,
-// range) are 8 k workgroups apart, so one XCD's L2 serves them all.
+// Shared prefixes. Grid (kv head and key range, rounded up to 8, tile of 16 MT rows): the row tiles of one (head,
+// range) are 8 k workgroups apart, so one XCD's L2 serves them all. A tile's rows are taken in runs of sequences with
+// one prefix, in the smallest of 16, 32 or 64 rows that holds the run.
 // ---------------------------------------------------------------------------------------------
 template <int KVQ, int QDT, int NT>
-__global__ __launch_bounds__(256) void k_prefix(PfArgs a) {
+__device__ __forceinline__ void pf_run(const PfArgs& a, PfShared& sm, int h, int z, int64_t ra, int64_t rb, int P, int owner, int k0, int k1) {
     constexpr int NQ = QDT == DT_BF16 ? 1 : QDT == DT_F16 ? 2 : 3;
-    using F = PfFrag<KVQ>;
-    __shared__ PfShared sm;
-    if ((int)blockIdx.x >= a.Hkv * a.NP) return;
-    const int h = blockIdx.x % a.Hkv, z = blockIdx.x / a.Hkv;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
-    const int64_t r0 = (int64_t)blockIdx.y * (16 * NT), rows = (int64_t)a.B * a.G;
-    const int64_t r1 = min(r0 + 16 * NT, rows);
-    const int b0 = (int)(r0 / a.G), b1 = (int)((r1 - 1) / a.G);  // sequences of the tile: at most 64
-    // lane i: sequence b0 + i
-    const PfSeq me = pf_seq(a, b0 + lane <= b1 ? b0 + lane : -1);
-    const PfSeq before = pf_seq(a, b0 + lane <= b1 ? b0 + lane - 1 : -1), after = pf_seq(a, b0 + lane <= b1 ? b0 + lane + 1 : -1);
-    uint64_t todo = __ballot(me.same(before) || me.same(after));
-    const uint64_t joined = __ballot(me.same(before));
-    if (!todo) return;
+    const int wave = threadIdx.x >> 6, l16 = threadIdx.x & 15;
     PfState<NT, NQ, NQ> st;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int64_t r = min(r0 + 16 * t + l16, rows - 1);
+        const int64_t r = min(ra + 16 * t + l16, rb - 1);
         const int b = (int)(r / a.G), g = (int)(r - (int64_t)b * a.G);
         const int64_t off = (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2);
-        st.template load_q<QDT>(t, (const uint8_t*)a.q + off, a.neg);
+        st.template load_q<QDT>(t, (const uint8_t*)a.q + off, a.neg, a.qvec);
     }
+    st.clear();
+    const int32_t* row = a.pt + owner * a.pts;
+    pf_walk<KVQ>(a, st, h * a.hs, k0 + wave, k1, [&](int k) { return row[k]; },
+                 [&](int k, int& lo, int& hi) { lo = 0, hi = P - k * kPfPage; });
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+        pf_merge(a, sm, st.acc[t], st.m[t], st.l[t], [&](int i16) -> int64_t {
+            const int64_t r = ra + 16 * t + i16;
+            if (r >= rb) return -1;
+            const int64_t b = r / a.G;
+            return (b * a.Hq + h * a.G + (r - b * a.G)) * (a.NP + a.NS) + z;
+        });
+}
+
+template <int KVQ, int QDT, int MT>
+__global__ __launch_bounds__(256) void k_prefix(PfArgs a) {
+    __shared__ PfShared sm;
+    if ((int)blockIdx.x >= a.Hkv * a.NP) return;
+    const int h = blockIdx.x % a.Hkv, z = blockIdx.x / a.Hkv, lane = threadIdx.x & 63;
+    const int64_t r0 = (int64_t)blockIdx.y * (16 * MT), r1 = min(r0 + 16 * MT, (int64_t)a.B * a.G);
+    const int b0 = (int)(r0 / a.G), b1 = (int)((r1 - 1) / a.G);  // sequences of the tile: at most 64
+    // lane i: sequence b0 + i
+    const int bl = b0 + lane <= b1 ? b0 + lane : -2;
+    const PfSeq me = pf_seq(a, bl), before = pf_seq(a, bl - 1), after = pf_seq(a, bl + 1);
+    uint64_t todo = __ballot(me.same(before) || me.same(after));
+    const uint64_t joined = __ballot(me.same(before));
     while (todo) {
         // a run of neighbours with one prefix: sequences b0 + i .. b0 + j - 1
         const int i = __builtin_ctzll(todo);
@@ -299,34 +378,9 @@ __global__ __launch_bounds__(256) void k_prefix(PfArgs a) {
         const int k0 = z * per, k1 = min(k0 + per, tiles);
         if (k0 >= k1) continue;  // the whole workgroup
         const int64_t ra = max(r0, (int64_t)(b0 + i) * a.G), rb = min(r1, (int64_t)(b0 + j) * a.G);  // its rows
-        unsigned live = 0;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-            if (r0 + 16 * t < rb && r0 + 16 * t + 16 > ra) live |= 1u << t;
-        st.clear();
-        const int32_t* row = a.pt + owner * a.pts;
-        auto at = [&](int k) {
-            const int page = row[k];
-            PfAt x{page >= 0 && page < a.np ? page * a.pgs + h * a.hs : -1, 0, P - k * kPfPage};
-            if (x.off < 0) x.hi = 0;
-            return x;
-        };
-        typename F::T kf[8] = {}, vf[8] = {};
-        for (int k = k0 + wave; k < k1; k += 4) {
-            const PfAt x = at(__builtin_amdgcn_readfirstlane(k));
-            pf_load<KVQ>(a, x, kf, vf);
-            st.template tile<KVQ>(kf, vf, x.lo, x.hi, a.sc, live);
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (!(live >> t & 1)) continue;
-            pf_merge(a, sm, st.acc[t], st.m[t], st.l[t], [&](int i16) -> int64_t {
-                const int64_t r = r0 + 16 * t + i16;
-                if (r < ra || r >= rb) return -1;
-                const int64_t b = r / a.G;
-                return (b * a.Hq + h * a.G + (r - b * a.G)) * (a.NP + a.NS) + z;
-            });
-        }
+        if (MT > 2 && rb - ra > 32) pf_run<KVQ, QDT, MT>(a, sm, h, z, ra, rb, P, owner, k0, k1);
+        else if (MT > 1 && rb - ra > 16) pf_run<KVQ, QDT, (MT > 1 ? 2 : 1)>(a, sm, h, z, ra, rb, P, owner, k0, k1);
+        else pf_run<KVQ, QDT, 1>(a, sm, h, z, ra, rb, P, owner, k0, k1);
     }
 }
 
@@ -336,7 +390,6 @@ __global__ __launch_bounds__(256) void k_prefix(PfArgs a) {
 template <int KVQ, int QDT>
 __global__ __launch_bounds__(256) void k_suffix(PfArgs a) {
     constexpr int NQ = QDT == DT_BF16 ? 1 : QDT == DT_F16 ? 2 : 3;
-    using F = PfFrag<KVQ>;
     __shared__ PfShared sm;
     const int z = blockIdx.x, ct = blockIdx.y / a.Hkv, h = blockIdx.y - ct * a.Hkv, b = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
@@ -350,23 +403,16 @@ __global__ __launch_bounds__(256) void k_suffix(PfArgs a) {
     {
         const int g = min(ct * 16 + l16, a.G - 1);
         const int64_t off = (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2);
-        st.template load_q<QDT>(0, (const uint8_t*)a.q + off, a.neg);
+        st.template load_q<QDT>(0, (const uint8_t*)a.q + off, a.neg, a.qvec);
     }
     st.clear();
-    auto at = [&](int k) {
-        const bool pre = k < n1;
-        const int blk = pre ? k : first + k - n1;
-        const int page = a.pt[(pre ? s.owner : b) * a.pts + blk];
-        PfAt x{page >= 0 && page < a.np ? page * a.pgs + h * a.hs : -1, pre ? 0 : s.P - blk * kPfPage, (pre ? s.P : s.L) - blk * kPfPage};
-        if (x.off < 0) x.hi = 0;
-        return x;
-    };
-    typename F::T kf[8] = {}, vf[8] = {};
-    for (int k = k0 + wave; k < k1; k += 4) {
-        const PfAt x = at(__builtin_amdgcn_readfirstlane(k));
-        pf_load<KVQ>(a, x, kf, vf);
-        st.template tile<KVQ>(kf, vf, x.lo, x.hi, a.sc, 1u);
-    }
+    pf_walk<KVQ>(a, st, h * a.hs, k0 + wave, k1,
+                 [&](int k) { return a.pt[(k < n1 ? s.owner : b) * a.pts + (k < n1 ? k : first + k - n1)]; },
+                 [&](int k, int& lo, int& hi) {
+                     const int at = (k < n1 ? k : first + k - n1) * kPfPage;
+                     lo = k < n1 ? 0 : s.P - at;
+                     hi = (k < n1 ? s.P : s.L) - at;
+                 });
     pf_merge(a, sm, st.acc[0], st.m[0], st.l[0], [&](int i16) -> int64_t {
         const int g = ct * 16 + i16;
         return g < a.G ? ((int64_t)b * a.Hq + h * a.G + g) * (a.NP + a.NS) + a.NP + z : -1;
@@ -388,15 +434,28 @@ __global__ __launch_bounds__(256) void k_prefix_join(PfArgs a, int odt) {
     const int ps = pf_per(ts, a.NS, kPfMinSuffix), ns = (ts + ps - 1) / ps;
     const float2* ml = a.ml + row * (a.NP + a.NS);
     const float2* o = reinterpret_cast<const float2*>(a.o + row * (a.NP + a.NS) * kPfDim) + lane;
-    float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
-    for (int i = 0; i < np + ns; ++i) M = fmaxf(M, ml[i < np ? i : a.NP + i - np].x);
-    for (int i = 0; i < np + ns; ++i) {
-        const int r = i < np ? i : a.NP + i - np;
-        const float2 e = ml[r], v = o[r * (kPfDim / 2)];
-        const float w = M == -INFINITY ? 1.f : e.x == -INFINITY ? (e.y == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(e.x - M);
-        L += e.y * w;
-        x += v.x * w;
-        y += v.y * w;
+    // lane i: the max and sum of records i and i + 64 (2 kPfMaxRecords at most)
+    const int n = np + ns;
+    auto place = [&](int i) { return i < np ? i : a.NP + i - np; };
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2 e0 = lane < n ? ml[place(lane)] : none, e1 = lane + 64 < n ? ml[place(lane + 64)] : none;
+    const float M = wave_max(fmaxf(e0.x, e1.x));
+    auto weight = [&](float2 e) {
+        return M == -INFINITY ? 1.f : e.x == -INFINITY ? (e.y == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(e.x - M);
+    };
+    const float w0 = weight(e0), w1 = weight(e1), L = wave_sum(e0.y * w0 + e1.y * w1);
+    float x = 0.f, y = 0.f;
+    for (int i = 0; i < n; i += 4) {
+        float2 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = i + k < n ? o[place(i + k) * (kPfDim / 2)] : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float wk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(i + k < 64 ? w0 : w1), (i + k) & 63));
+            const float w = i + k < n ? wk : 0.f;
+            x += v[k].x * w;
+            y += v[k].y * w;
+        }
     }
     // no key, or none with a score above -inf: zeros
     const float inv = L == 0.f ? 0.f : a.vs / L;
@@ -407,15 +466,15 @@ __global__ __launch_bounds__(256) void k_prefix_join(PfArgs a, int odt) {
 }
 
 struct PfPlan {
-    int NT, NP, NS, tiles;
+    int MT, NP, NS, tiles;
 };
 // Launch shape from what the host knows: rows, kv heads and the table's width (an upper bound of every length).
 static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
     const int64_t rows = (int64_t)B * (Hq / Hkv), groups = (Hq / Hkv + 15) / 16;
     PfPlan p;
     // rows a workgroup shares a key among: 64, fewer when there are fewer, or when q's further terms take the registers
-    p.NT = rows <= 16 ? 1 : rows <= 32 || dt != DT_BF16 ? 2 : 4;
-    p.tiles = (int)((rows + 16 * p.NT - 1) / (16 * p.NT));
+    p.MT = rows <= 16 ? 1 : rows <= 32 || dt != DT_BF16 ? 2 : 4;
+    p.tiles = (int)((rows + 16 * p.MT - 1) / (16 * p.MT));
     auto clamp = [](int64_t v, int64_t hi) { return (int)max((int64_t)1, min(min(v, hi), (int64_t)kPfMaxRecords)); };
     // a workgroup a CU for the prefix (its waves fill the register file), eight for the suffix
     p.NP = clamp(256 / ((int64_t)p.tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
@@ -427,8 +486,8 @@ template <int KVQ, int QDT>
 static void pf_launch(const PfArgs& a, const PfPlan& p, int odt, hipStream_t st) {
     const dim3 grid((a.Hkv * a.NP + 7) / 8 * 8, p.tiles), block(256);
     if (a.B > 1) {  // one sequence shares nothing
-        if (p.NT == 1) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 1>), grid, block, 0, st, a);
-        else if (p.NT == 2) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 2>), grid, block, 0, st, a);
+        if (p.MT == 1) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 1>), grid, block, 0, st, a);
+        else if (p.MT == 2) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 2>), grid, block, 0, st, a);
         else if constexpr (QDT == DT_BF16) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 4>), grid, block, 0, st, a);
     }
     hipLaunchKernelGGL((k_suffix<KVQ, QDT>), dim3(a.NS, a.Hkv * ((a.G + 15) / 16), a.B), block, 0, st, a);
@@ -480,7 +539,8 @@ int wf_shared_prefix_attention(const void* q, int dtype, int64_t q_sb, int64_t q
     const PfPlan p = pf_plan(dtype, B, Hq, Hkv, max_blocks);
     const int64_t recs = (int64_t)B * Hq * (p.NP + p.NS);
     float* o = reinterpret_cast<float*>(ws);
-    PfArgs a{q, q_sb, q_sh, (const uint8_t*)k_pool, (const uint8_t*)v_pool, page_stride * eb, head_stride * eb, num_pages, page_table,
+    const int per16 = dtype == WF_F32 ? 4 : 8;
+    PfArgs a{q, q_sb, q_sh, aligned16(q) && q_sb % per16 == 0 && q_sh % per16 == 0, (const uint8_t*)k_pool, (const uint8_t*)v_pool, page_stride * eb, head_stride * eb, num_pages, page_table,
              table_stride, max_blocks, seq_lens, prefix_rows, prefix_lens, B, Hq, Hkv, Hq / Hkv, fabsf(sc), sc < 0.f ? -1.f : 1.f, v_scale,
              p.NP, p.NS, reinterpret_cast<float2*>(o + recs * kPfDim), o, out, o_sb, o_sh, lse};
     hipStream_t st = as_stream(stream);
