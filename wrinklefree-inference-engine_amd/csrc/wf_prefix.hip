@@ -33,6 +33,15 @@ typedef float pf_f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPfDim = 128, kPfPage = 32;
 constexpr int kPfMaxRecords = 64;          // splits of each part
+#ifndef PF_APART
+#define PF_APART 128
+#endif
+#ifndef PF_NP
+#define PF_NP 256
+#endif
+#ifndef PF_NS
+#define PF_NS 2048
+#endif
 constexpr int kPfMinTiles = 4;             // prefix: a tile a wave at least
 constexpr int kPfMinSuffix = 8;            // suffix: two
 constexpr float kPfLn2 = 0.69314718055994530942f;
@@ -94,142 +103,170 @@ struct PfFrag {
     }
 };
 
-// NT column tiles of 16 query rows: the q fragments, running max, sum and output of one wave.
-template <int NT, int NQ, int NPT>
+// NT column tiles of W query rows: the q fragments, running max, sum and output of one wave. A K or V tile is 8 fragments
+// of 8 elements a lane, and either way the accumulator of S^T leaves a lane with the keys that it needs in P^T:
+//   W = 16 (v_mfma_f32_16x16x32_bf16): lane (l = row, g = quarter); scores of keys 8 g + e, e = 0..7;
+//   W = 32 (v_mfma_f32_32x32x16_bf16, 1.7 times the rate: 32 cycles to 2 x 27 measured): lane (l = row, g = half); scores of
+//          keys 16 j + 8 g + e, j = 0, 1 -- K's 32 rows are the two 16-row halves of the tile one after the other.
+template <int W, int NT, int NQ, int NPT>
 struct PfState {
-    pf_bf8 q[NT][NQ][4];
-    pf_f4 acc[NT][8];
+    static constexpr int J = W / 16;            // groups of 8 keys a lane
+    static constexpr int M = kPfDim / W;        // accumulators of a column tile
+    static constexpr int S = W == 16 ? 4 : 8;   // dim steps of a score
+    typedef float Acc __attribute__((ext_vector_type(W == 16 ? 4 : 16)));
+    pf_bf8 q[NT][NQ][S];
+    Acc acc[NT][M];
     float m[NT], f[NT], l[NT];  // max (log2 domain), the frame of the exponents (m, or 0 while it is -inf), sum
+
+    static __device__ __forceinline__ int row() { return threadIdx.x & (W - 1); }
+    static __device__ __forceinline__ int group() { return (threadIdx.x & 63) / W; }
+    // where fragment i of this lane lies in a tile: K's (score step or half), V's (accumulator and key group)
+    static __device__ __forceinline__ int k_at(int i) {
+        if constexpr (W == 16) return i * 512 + (threadIdx.x & 63) * 8;  // i = 4 half + step
+        else return (row() >> 4) * 2048 + i * 256 + group() * 128 + (row() & 15) * 8;
+    }
+    static __device__ __forceinline__ int v_at(int i) {
+        if constexpr (W == 16) return i * 512 + (threadIdx.x & 63) * 8;
+        else return (i >> 1) * 1024 + (row() >> 4) * 512 + (i & 1) * 256 + group() * 128 + (row() & 15) * 8;  // i = 2 m + j
+    }
+    static __device__ __forceinline__ Acc mfma(pf_bf8 x, pf_bf8 y, Acc c) {
+        if constexpr (W == 16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+    }
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             m[t] = -INFINITY, f[t] = 0.f, l[t] = 0.f;
 #pragma unroll
-            for (int n = 0; n < 8; ++n) acc[t][n] = pf_f4{0.f, 0.f, 0.f, 0.f};
+            for (int n = 0; n < M; ++n) acc[t][n] = Acc{};
         }
     }
-    // tile t's row; fragment c: dims 32 c + 8 q4 ..; vec: the row is 16-byte aligned
+    // tile t's row; fragment c: its dims 8 (64 / W c + g) ..; vec: the row is 16-byte aligned
     template <int QDT>
     __device__ __forceinline__ void load_q(int t, const uint8_t* row, float neg, bool vec) {
-        const int q4 = (threadIdx.x & 63) >> 4;
-        float x[4][8];
-        if (vec) {
-            constexpr int W = QDT == DT_F32 ? 2 : 1;
-            uint4 w[4][W];
+        constexpr int G = 64 / W, V = QDT == DT_F32 ? 2 : 1;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < S; ++c) {
+            float x[8];
+            if (vec) {
 #pragma unroll
-                for (int i = 0; i < W; ++i) w[c][i] = reinterpret_cast<const uint4*>(row)[(4 * c + q4) * W + i];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    const uint32_t d[4] = {w[c][i].x, w[c][i].y, w[c][i].z, w[c][i].w};
+                for (int i = 0; i < V; ++i) {
+                    const uint4 w = reinterpret_cast<const uint4*>(row)[(G * c + group()) * V + i];
+                    const uint32_t d[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if constexpr (QDT == DT_F32) x[c][4 * i + e] = __uint_as_float(d[e]);
-                        else if constexpr (QDT == DT_BF16) x[c][2 * e] = bf_lo(d[e]), x[c][2 * e + 1] = bf_hi(d[e]);
-                        else x[c][2 * e] = h2f(d[e] & 0xffffu), x[c][2 * e + 1] = h2f(d[e] >> 16);
+                        if constexpr (QDT == DT_F32) x[4 * i + e] = __uint_as_float(d[e]);
+                        else if constexpr (QDT == DT_BF16) x[2 * e] = bf_lo(d[e]), x[2 * e + 1] = bf_hi(d[e]);
+                        else x[2 * e] = h2f(d[e] & 0xffffu), x[2 * e + 1] = h2f(d[e] >> 16);
                     }
                 }
-        } else {
+            } else {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+                for (int e = 0; e < 8; ++e) x[e] = load_as_f32(row, 8 * (G * c + group()) + e, QDT);
+            }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[c][e] = load_as_f32(row, 32 * c + 8 * q4 + e, QDT);
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[c][e] *= neg;
+            for (int e = 0; e < 8; ++e) x[e] *= neg;
 #pragma unroll
             for (int k = 0; k < NQ; ++k) {
                 pf_bf8 v;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[e] = (__bf16)x[c][e];
-                    x[c][e] -= (float)v[e];
+                    v[e] = (__bf16)x[e];
+                    x[e] -= (float)v[e];
                 }
                 q[t][k][c] = v;
             }
         }
     }
-    using Scores = pf_f4[NT][2];
-    // scores of a 32-key tile: lane (row l16, quarter q4) gets keys 8 q4 + 4 h + r in s[t][h][r]
+    using Scores = float[NT][8 * J];
+    using Probs = pf_bf8[NT][NPT][J];
+    // scores of a 32-key tile: s[t][8 j + e] for key 8 (64 / W j + g) + e
     template <int KVQ>
     __device__ __forceinline__ void scores(const typename PfFrag<KVQ>::T (&kf)[8], Scores& s) {
+        Acc c[NT][W == 16 ? 2 : 1];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = pf_f4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const pf_bf8 k0 = __builtin_bit_cast(pf_bf8, PfFrag<KVQ>::bf(kf[c])), k1 = __builtin_bit_cast(pf_bf8, PfFrag<KVQ>::bf(kf[4 + c]));
+            for (int h = 0; h < (W == 16 ? 2 : 1); ++h) c[t][h] = Acc{};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int step = W == 16 ? i >> 1 : i, h = W == 16 ? i & 1 : 0;
+            const pf_bf8 kb = __builtin_bit_cast(pf_bf8, PfFrag<KVQ>::bf(kf[W == 16 ? 4 * h + step : i]));
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int k = NQ - 1; k >= 0; --k) {
-                        s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[t][k][c], s[t][0], 0, 0, 0);
-                        s[t][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[t][k][c], s[t][1], 0, 0, 0);
-                    }
+                for (int k = NQ - 1; k >= 0; --k) c[t][h] = mfma(kb, q[t][k][step], c[t][h]);
         }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 8 * J; ++e)
+                s[t][e] = W == 16 ? c[t][(e >> 2) & (W == 16)][e & 3] : c[t][0][(8 * ((e >> 2) & 1) + 4 * (e >> 3) + (e & 3)) & (W / 2 - 1)];
     }
+    static __device__ __forceinline__ int key(int j) { return 8 * (64 / W * j + group()); }
     // scores -> probabilities in the rows' frames; keys outside [lo, hi) of the tile are masked
-    __device__ __forceinline__ void softmax(const Scores& s, pf_bf8 (&p)[NT][NPT], int lo, int hi, float sc) {
-        const int key = (threadIdx.x & 63) >> 4 << 3;  // this lane's keys: key .. key + 7
+    __device__ __forceinline__ void softmax(Scores& s, pf_bf8 (&p)[NT][NPT][J], int lo, int hi, float sc) {
         const bool whole = lo <= 0 && hi >= kPfPage;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[t][e >> 2][e & 3];
+            float (&x)[8 * J] = s[t];
             if (!whole) {
                 asm volatile("");  // a branch, not selects on every tile
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = key + e >= lo && key + e < hi ? x[e] : -INFINITY;
+                for (int e = 0; e < 8 * J; ++e) x[e] = key(e >> 3) + (e & 7) >= lo && key(e >> 3) + (e & 7) < hi ? x[e] : -INFINITY;
             }
-            float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * sc;
+            float mx = x[0];
+#pragma unroll
+            for (int e = 1; e < 8 * J; ++e) mx = fmaxf(mx, x[e]);
+            mx *= sc;
             if (__any(mx > m[t] + 8.f)) {
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                if constexpr (W == 16) mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m[t]);
                 const float nf = mx == -INFINITY ? 0.f : mx;
                 // (an empty sum stays, also when it is NaN: it holds no finite score to rescale)
                 const float r = m[t] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(f[t] - nf);
                 l[t] *= r;
 #pragma unroll
-                for (int n = 0; n < 8; ++n) acc[t][n] *= r;
+                for (int n = 0; n < M; ++n) acc[t][n] *= r;
                 m[t] = mx;
                 f[t] = nf;
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], sc, -f[t]));
-            l[t] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            for (int e = 0; e < 8 * J; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], sc, -f[t]));
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const float* y = x + 8 * j;
+                l[t] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+            }
 #pragma unroll
             for (int k = 0; k < NPT; ++k)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    p[t][k][e] = (__bf16)x[e];
-                    if (k + 1 < NPT) x[e] -= (float)p[t][k][e];
+                for (int e = 0; e < 8 * J; ++e) {
+                    p[t][k][e >> 3][e & 7] = (__bf16)x[e];
+                    if (k + 1 < NPT) x[e] -= (float)p[t][k][e >> 3][e & 7];
                 }
         }
     }
     // o += P V
     template <int KVQ>
-    __device__ __forceinline__ void values(const typename PfFrag<KVQ>::T (&vf)[8], const pf_bf8 (&p)[NT][NPT], int lo, int hi) {
-        const int key = (threadIdx.x & 63) >> 4 << 3;
-        const bool whole = lo <= 0 && hi >= kPfPage;
+    __device__ __forceinline__ void values(const typename PfFrag<KVQ>::T (&vf)[8], const pf_bf8 (&p)[NT][NPT][J], int lo, int hi) {
         uint4 v[8];
 #pragma unroll
         for (int n = 0; n < 8; ++n) v[n] = PfFrag<KVQ>::bf(vf[n]);
-        if (!whole) {  // a masked key's V may hold anything: 0 x NaN is NaN
+        if (!(lo <= 0 && hi >= kPfPage)) {  // a masked key's V may hold anything: 0 x NaN is NaN
             asm volatile("");
-            uint32_t mask[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int k0 = key + 2 * j;
-                mask[j] = (k0 >= lo && k0 < hi ? 0xffffu : 0u) | (k0 + 1 >= lo && k0 + 1 < hi ? 0xffff0000u : 0u);
+            for (int j = 0; j < J; ++j) {
+                uint32_t mask[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k0 = key(j) + 2 * i;
+                    mask[i] = (k0 >= lo && k0 < hi ? 0xffffu : 0u) | (k0 + 1 >= lo && k0 + 1 < hi ? 0xffff0000u : 0u);
+                }
+#pragma unroll
+                for (int n = j; n < 8; n += J) v[n] = make_uint4(v[n].x & mask[0], v[n].y & mask[1], v[n].z & mask[2], v[n].w & mask[3]);
             }
-#pragma unroll
-            for (int n = 0; n < 8; ++n) v[n] = make_uint4(v[n].x & mask[0], v[n].y & mask[1], v[n].z & mask[2], v[n].w & mask[3]);
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
@@ -237,7 +274,7 @@ struct PfState {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int k = NPT - 1; k >= 0; --k) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p[t][k], acc[t][n], 0, 0, 0);
+                for (int k = NPT - 1; k >= 0; --k) acc[t][n / J] = mfma(vb, p[t][k][n % J], acc[t][n / J]);
         }
     }
 };
@@ -246,8 +283,8 @@ struct PfState {
 // range(k, lo, hi) its valid keys. 64 page ids are fetched at a time, a lane each. The next tile's K is under way from
 // the moment this one's scores are done, its V from the moment this one's products are: one set of registers,
 // and half a tile's work over each load's latency.
-template <int KVQ, int NT, int NQ, class Page, class Range>
-__device__ __forceinline__ void pf_walk(const PfArgs& a, PfState<NT, NQ, NQ>& st, int64_t head, int k0, int k1, Page page, Range range) {
+template <int KVQ, class State, class Page, class Range>
+__device__ __forceinline__ void pf_walk(const PfArgs& a, State& st, int64_t head, int k0, int k1, Page page, Range range) {
     using T = typename PfFrag<KVQ>::T;
     const int lane = threadIdx.x & 63, n = (k1 - k0 + 3) / 4;
     if (n <= 0) return;
@@ -262,93 +299,106 @@ __device__ __forceinline__ void pf_walk(const PfArgs& a, PfState<NT, NQ, NQ>& st
         }
         return __builtin_amdgcn_readlane(ids, i & 63);
     };
-    auto load = [&](int id, const uint8_t* pool, T (&f)[8]) {
-        const T* p = reinterpret_cast<const T*>(pool + max(id, 0) * a.pgs + head) + lane;  // no such page: page 0, masked
+    auto load = [&](int id, const uint8_t* pool, T (&f)[8], bool v) {
+        const uint8_t* p = pool + max(id, 0) * a.pgs + head;  // no such page: page 0, masked
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = p[64 * e];
+        for (int e = 0; e < 8; ++e) f[e] = *reinterpret_cast<const T*>(p + (v ? State::v_at(e) : State::k_at(e)) * PfFrag<KVQ>::kBytes);
     };
     int id = find(0);
-    load(id, a.K, kf);
-    load(id, a.V, vf);
+    load(id, a.K, kf, false);
+    load(id, a.V, vf, true);
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
         int lo, hi;
         range(k0 + 4 * i, lo, hi);
         if (id < 0) hi = 0;
         id = i + 1 < n ? find(i + 1) : -1;
-        pf_f4 s[NT][2];
-        pf_bf8 p[NT][NQ];
+        typename State::Scores s;
+        typename State::Probs p;
         st.template scores<KVQ>(kf, s);
-        load(id, a.K, kf);
+        load(id, a.K, kf, false);
         st.softmax(s, p, lo, hi, a.sc);
         st.template values<KVQ>(vf, p, lo, hi);
-        load(id, a.V, vf);
+        load(id, a.V, vf, true);
     }
 }
 
-// The four waves' states of one column tile -> one record a row. sm: 4 x 16 rows of 132 floats + 4 x 16 (m, l).
+// The four waves' states of one column tile -> one record a row.
 constexpr int kPfRow = kPfDim + 4;
+template <int W>
 struct __attribute__((aligned(16))) PfShared {
-    float o[4][16][kPfRow];
-    float m[4][16], l[4][16];
+    float o[4][W][kPfRow];
+    float m[4][W], l[4][W];
 };
 // row(i): the record's place in ml / o for row i of the column tile, or < 0
-template <class Row>
-__device__ __forceinline__ void pf_merge(const PfArgs& a, PfShared& sm, const pf_f4 (&acc)[8], float m, float l, Row row) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q4 = lane >> 4;
-    l += __shfl_xor(l, 16, 64);
+template <int W, class Acc, int M, class Row>
+__device__ __forceinline__ void pf_merge(const PfArgs& a, PfShared<W>& sm, const Acc (&acc)[M], float m, float l, Row row) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & (W - 1), g = lane / W;
+    if constexpr (W == 16) l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     __syncthreads();  // the last column tile's record has been read
+    // accumulator n, registers 4 i ..: dims W n + 8 i + 4 g .. (W = 16: i = 0)
 #pragma unroll
-    for (int n = 0; n < 8; ++n) *reinterpret_cast<pf_f4*>(&sm.o[wave][l16][16 * n + 4 * q4]) = acc[n];
-    if (q4 == 0) sm.m[wave][l16] = m, sm.l[wave][l16] = l;
+    for (int n = 0; n < M; ++n)
+#pragma unroll
+        for (int i = 0; i < (W == 16 ? 1 : 4); ++i)
+            *reinterpret_cast<pf_f4*>(&sm.o[wave][r][W * n + 8 * i + 4 * g]) = pf_f4{acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
+    if (g == 0) sm.m[wave][r] = m, sm.l[wave][r] = l;
     __syncthreads();
-    // 16 threads a row, 8 dims each
-    const int r = threadIdx.x >> 4, d = (threadIdx.x & 15) * 8;
-    const int64_t rec = row(r);
+    // 256 / W threads a row, 8 dims each at a time
+    constexpr int T = 256 / W;
+    const int y = threadIdx.x / T;
+    const int64_t rec = row(y);
     if (rec < 0) return;
-    float M = -INFINITY, w[4], L = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float mm = -INFINITY, w[4], sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) M = fmaxf(M, sm.m[i][r]);
+    for (int i = 0; i < 4; ++i) mm = fmaxf(mm, sm.m[i][y]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         // a wave that saw no finite score has l = 0 (or NaN) in the frame 0
-        w[i] = M == -INFINITY ? 1.f : sm.m[i][r] == -INFINITY ? (sm.l[i][r] == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(sm.m[i][r] - M);
-        L += sm.l[i][r] * w[i];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] += sm.o[i][r][d + e] * w[i];
+        w[i] = mm == -INFINITY ? 1.f : sm.m[i][y] == -INFINITY ? (sm.l[i][y] == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(sm.m[i][y] - mm);
+        sum += sm.l[i][y] * w[i];
     }
-    float* o = a.o + rec * kPfDim + d;
-    *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(o + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    if (d == 0) a.ml[rec] = make_float2(M, L);
+#pragma unroll
+    for (int d = (threadIdx.x % T) * 4; d < kPfDim; d += 4 * T) {
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] += sm.o[i][y][d + e] * w[i];
+        *reinterpret_cast<float4*>(a.o + rec * kPfDim + d) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+    if (threadIdx.x % T == 0) a.ml[rec] = make_float2(mm, sum);
 }
 
 // ---------------------------------------------------------------------------------------------
-// Shared prefixes. Grid (kv head and key range, rounded up to 8, tile of 16 MT rows): the row tiles of one (head,
-// range) are 8 k workgroups apart, so one XCD's L2 serves them all. A tile's rows are taken in runs of sequences with
-// one prefix, in the smallest of 16, 32 or 64 rows that holds the run.
+// Shared prefixes. Block (kv head and key range, rounded up to 8, tile of MT rows): the row tiles of one (head, range)
+// are 8 k workgroups apart, so one XCD's L2 serves them all. A tile's rows are taken in runs of sequences with one
+// prefix, in the smallest of 16, 32 or 64 rows that holds the run.
 // ---------------------------------------------------------------------------------------------
-template <int KVQ, int QDT, int NT>
-__device__ __forceinline__ void pf_run(const PfArgs& a, PfShared& sm, int h, int z, int64_t ra, int64_t rb, int P, int owner, int k0, int k1) {
-    constexpr int NQ = QDT == DT_BF16 ? 1 : QDT == DT_F16 ? 2 : 3;
-    const int wave = threadIdx.x >> 6, l16 = threadIdx.x & 15;
-    PfState<NT, NQ, NQ> st;
+template <int QDT>
+constexpr int kPfTerms = QDT == DT_BF16 ? 1 : QDT == DT_F16 ? 2 : 3;
+
+template <int KVQ, int QDT, int W, int NT>
+__device__ __forceinline__ void pf_run(const PfArgs& a, void* lds, int h, int z, int64_t ra, int64_t rb, int P, int owner, int k0, int k1) {
+    constexpr int NQ = kPfTerms<QDT>;
+    using State = PfState<W, NT, NQ, NQ>;
+    State st;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int64_t r = min(ra + 16 * t + l16, rb - 1);
+        const int64_t r = min(ra + W * t + State::row(), rb - 1);
         const int b = (int)(r / a.G), g = (int)(r - (int64_t)b * a.G);
         const int64_t off = (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2);
         st.template load_q<QDT>(t, (const uint8_t*)a.q + off, a.neg, a.qvec);
     }
     st.clear();
     const int32_t* row = a.pt + owner * a.pts;
-    pf_walk<KVQ>(a, st, h * a.hs, k0 + wave, k1, [&](int k) { return row[k]; },
+    pf_walk<KVQ>(a, st, h * a.hs, k0 + (int)(threadIdx.x >> 6), k1, [&](int k) { return row[k]; },
                  [&](int k, int& lo, int& hi) { lo = 0, hi = P - k * kPfPage; });
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-        pf_merge(a, sm, st.acc[t], st.m[t], st.l[t], [&](int i16) -> int64_t {
-            const int64_t r = ra + 16 * t + i16;
+        pf_merge(a, *static_cast<PfShared<W>*>(lds), st.acc[t], st.m[t], st.l[t], [&](int i) -> int64_t {
+            const int64_t r = ra + W * t + i;
             if (r >= rb) return -1;
             const int64_t b = r / a.G;
             return (b * a.Hq + h * a.G + (r - b * a.G)) * (a.NP + a.NS) + z;
@@ -356,11 +406,10 @@ __device__ __forceinline__ void pf_run(const PfArgs& a, PfShared& sm, int h, int
 }
 
 template <int KVQ, int QDT, int MT>
-__global__ __launch_bounds__(256) void k_prefix(PfArgs a) {
-    __shared__ PfShared sm;
-    if ((int)blockIdx.x >= a.Hkv * a.NP) return;
-    const int h = blockIdx.x % a.Hkv, z = blockIdx.x / a.Hkv, lane = threadIdx.x & 63;
-    const int64_t r0 = (int64_t)blockIdx.y * (16 * MT), r1 = min(r0 + 16 * MT, (int64_t)a.B * a.G);
+__device__ void pf_prefix(const PfArgs& a, void* lds, int x, int tile) {
+    if (x >= a.Hkv * a.NP) return;
+    const int h = x % a.Hkv, z = x / a.Hkv, lane = threadIdx.x & 63;
+    const int64_t r0 = (int64_t)tile * MT, r1 = min(r0 + MT, (int64_t)a.B * a.G);
     const int b0 = (int)(r0 / a.G), b1 = (int)((r1 - 1) / a.G);  // sequences of the tile: at most 64
     // lane i: sequence b0 + i
     const int bl = b0 + lane <= b1 ? b0 + lane : -2;
@@ -378,45 +427,71 @@ __global__ __launch_bounds__(256) void k_prefix(PfArgs a) {
         const int k0 = z * per, k1 = min(k0 + per, tiles);
         if (k0 >= k1) continue;  // the whole workgroup
         const int64_t ra = max(r0, (int64_t)(b0 + i) * a.G), rb = min(r1, (int64_t)(b0 + j) * a.G);  // its rows
-        if (MT > 2 && rb - ra > 32) pf_run<KVQ, QDT, MT>(a, sm, h, z, ra, rb, P, owner, k0, k1);
-        else if (MT > 1 && rb - ra > 16) pf_run<KVQ, QDT, (MT > 1 ? 2 : 1)>(a, sm, h, z, ra, rb, P, owner, k0, k1);
-        else pf_run<KVQ, QDT, 1>(a, sm, h, z, ra, rb, P, owner, k0, k1);
+        if constexpr (MT > 32)
+            if (rb - ra > 32) {
+                pf_run<KVQ, QDT, 32, 2>(a, lds, h, z, ra, rb, P, owner, k0, k1);
+                continue;
+            }
+        if constexpr (MT > 16)
+            if (rb - ra > 16) {
+                pf_run<KVQ, QDT, 32, 1>(a, lds, h, z, ra, rb, P, owner, k0, k1);
+                continue;
+            }
+        pf_run<KVQ, QDT, 16, 1>(a, lds, h, z, ra, rb, P, owner, k0, k1);
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// The other keys. Grid (key range, kv head and tile of 16 of its heads, sequence).
+// The other keys. Block (key range z, kv head and tile of 16 of its heads, sequence).
 // ---------------------------------------------------------------------------------------------
 template <int KVQ, int QDT>
-__global__ __launch_bounds__(256) void k_suffix(PfArgs a) {
-    constexpr int NQ = QDT == DT_BF16 ? 1 : QDT == DT_F16 ? 2 : 3;
-    __shared__ PfShared sm;
-    const int z = blockIdx.x, ct = blockIdx.y / a.Hkv, h = blockIdx.y - ct * a.Hkv, b = blockIdx.z;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
+__device__ void pf_suffix(const PfArgs& a, void* lds, int z, int hc, int b) {
+    constexpr int NQ = kPfTerms<QDT>;
+    const int ct = hc / a.Hkv, h = hc - ct * a.Hkv;
     const PfSeq s = pf_seq(a, b);
     // tiles [0, n1) the owner's, below P; then its own from the tile that holds P on
     const int n1 = pf_shared(a, b, s) ? 0 : pf_tiles(s.P), first = s.P / kPfPage;
     const int tiles = s.L > s.P ? n1 + pf_tiles(s.L) - first : n1;
     const int per = pf_per(tiles, a.NS, kPfMinSuffix), k0 = z * per, k1 = min(k0 + per, tiles);
     if (k0 >= k1) return;
-    PfState<1, NQ, NQ> st;
+    using State = PfState<16, 1, NQ, NQ>;
+    State st;
     {
-        const int g = min(ct * 16 + l16, a.G - 1);
+        const int g = min(ct * 16 + State::row(), a.G - 1);
         const int64_t off = (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2);
         st.template load_q<QDT>(0, (const uint8_t*)a.q + off, a.neg, a.qvec);
     }
     st.clear();
-    pf_walk<KVQ>(a, st, h * a.hs, k0 + wave, k1,
+    pf_walk<KVQ>(a, st, h * a.hs, k0 + (int)(threadIdx.x >> 6), k1,
                  [&](int k) { return a.pt[(k < n1 ? s.owner : b) * a.pts + (k < n1 ? k : first + k - n1)]; },
                  [&](int k, int& lo, int& hi) {
                      const int at = (k < n1 ? k : first + k - n1) * kPfPage;
                      lo = k < n1 ? 0 : s.P - at;
                      hi = (k < n1 ? s.P : s.L) - at;
                  });
-    pf_merge(a, sm, st.acc[0], st.m[0], st.l[0], [&](int i16) -> int64_t {
+    pf_merge(a, *static_cast<PfShared<16>*>(lds), st.acc[0], st.m[0], st.l[0], [&](int i16) -> int64_t {
         const int g = ct * 16 + i16;
         return g < a.G ? ((int64_t)b * a.Hq + h * a.G + g) * (a.NP + a.NS) + a.NP + z : -1;
     });
+}
+
+// MT > 0: the prefixes, row tiles of MT, in the first np workgroups; SUF: the other keys in the rest.
+template <int KVQ, int QDT, int MT, bool SUF>
+__global__ __launch_bounds__(256, MT == 64 || (MT == 32 && QDT != DT_BF16) ? 1 : 2) void k_shared_prefix(PfArgs a, int np) {
+    __shared__ PfShared<(MT > 16 ? 32 : 16)> sm;
+    int x = blockIdx.x;
+    if constexpr (MT > 0) {
+        if (x < np) {
+            const int w = (a.Hkv * a.NP + 7) / 8 * 8;
+            pf_prefix<KVQ, QDT, MT>(a, &sm, x % w, x / w);
+            return;
+        }
+    }
+    if constexpr (SUF) {
+        x -= np;
+        const int hc = a.Hkv * ((a.G + 15) / 16), z = x % a.NS, y = x / a.NS;
+        pf_suffix<KVQ, QDT>(a, &sm, z, y % hc, y / hc);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -466,31 +541,37 @@ __global__ __launch_bounds__(256) void k_prefix_join(PfArgs a, int odt) {
 }
 
 struct PfPlan {
-    int MT, NP, NS, tiles;
+    int MT, NP, NS, np, ns;  // rows of a prefix workgroup, splits, workgroups
+    bool apart;              // the prefixes in a launch of their own
 };
 // Launch shape from what the host knows: rows, kv heads and the table's width (an upper bound of every length).
 static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
     const int64_t rows = (int64_t)B * (Hq / Hkv), groups = (Hq / Hkv + 15) / 16;
     PfPlan p;
-    // rows a workgroup shares a key among: 64, fewer when there are fewer, or when q's further terms take the registers
-    p.MT = rows <= 16 ? 1 : rows <= 32 || dt != DT_BF16 ? 2 : 4;
-    p.tiles = (int)((rows + 16 * p.MT - 1) / (16 * p.MT));
+    p.apart = rows > 32 && cols > PF_APART && dt == DT_BF16;
+    p.MT = rows <= 16 ? 16 : p.apart ? 64 : 32;
+    const int64_t tiles = (rows + p.MT - 1) / p.MT;
     auto clamp = [](int64_t v, int64_t hi) { return (int)max((int64_t)1, min(min(v, hi), (int64_t)kPfMaxRecords)); };
-    // a workgroup a CU for the prefix (its waves fill the register file), eight for the suffix
-    p.NP = clamp(256 / ((int64_t)p.tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
-    p.NS = clamp(2048 / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);
+    p.NP = clamp((p.apart ? 256 : PF_NP) / (tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
+    p.NS = clamp(PF_NS / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);
+    p.np = B > 1 ? (int)(((int64_t)Hkv * p.NP + 7) / 8 * 8 * tiles) : 0;  // one sequence shares nothing
+    p.ns = (int)(p.NS * Hkv * groups * B);
     return p;
 }
 
 template <int KVQ, int QDT>
 static void pf_launch(const PfArgs& a, const PfPlan& p, int odt, hipStream_t st) {
-    const dim3 grid((a.Hkv * a.NP + 7) / 8 * 8, p.tiles), block(256);
-    if (a.B > 1) {  // one sequence shares nothing
-        if (p.MT == 1) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 1>), grid, block, 0, st, a);
-        else if (p.MT == 2) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 2>), grid, block, 0, st, a);
-        else if constexpr (QDT == DT_BF16) hipLaunchKernelGGL((k_prefix<KVQ, QDT, 4>), grid, block, 0, st, a);
+    const dim3 block(256);
+    if (p.apart) {
+        if constexpr (QDT == DT_BF16) {
+            hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 64, false>), dim3(p.np), block, 0, st, a, p.np);
+            hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 0, true>), dim3(p.ns), block, 0, st, a, 0);
+        }
+    } else if (p.MT == 16) {
+        hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 16, true>), dim3(p.np + p.ns), block, 0, st, a, p.np);
+    } else {
+        hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 32, true>), dim3(p.np + p.ns), block, 0, st, a, p.np);
     }
-    hipLaunchKernelGGL((k_suffix<KVQ, QDT>), dim3(a.NS, a.Hkv * ((a.G + 15) / 16), a.B), block, 0, st, a);
     hipLaunchKernelGGL(k_prefix_join, dim3((unsigned)(((int64_t)a.B * a.Hq + 3) / 4)), block, 0, st, a, odt);
 }
 
