@@ -5,17 +5,18 @@
 // others on its own:  o = sum_j p_j v_j / l,  p_j = exp(scale q.k_j - m),  l = sum_j p_j,  lse = m + log l.
 // The softmax splits over any partition of the keys into records (m, l, unnormalised o) that a second launch joins.
 //
-//   k_prefix  keys [0, P) of neighbouring sequences with the same owner and P ("shared"): a workgroup takes up to 64
-//             query rows (sequence, head of the kv group) and a range of the keys; every wave takes every fourth
-//             32-key tile for ALL rows, so a K/V byte is loaded once per 64 rows, straight into registers.
-//   k_suffix  the other keys of a sequence (all of them where it shares with no neighbour): one kv head and a range of
-//             the keys a workgroup, the group's heads as the matrix's columns. Bound by memory.
-//   k_prefix_join  one wave a (sequence, head): its records, the division, the output type.
+//   prefix  keys [0, P) of neighbouring sequences with the same owner and P ("shared"): a workgroup takes up to 32 query
+//           rows (sequence, head of the kv group) and a range of the keys; every wave takes every fourth 32-key tile for
+//           ALL rows, so a K/V byte is loaded once per 32 rows, straight into registers.
+//   suffix  the other keys of a sequence (all of them where it shares with no neighbour): one kv head and a range of the
+//           keys a workgroup, the group's heads as the matrix's columns. Bound by HBM.
+//   join    one wave a (sequence, head): its records, the division, the output type.
+// Prefix and suffix are the two kinds of workgroup of one launch, the join is a second.
 //
-// Tiles: the pool's 32-key K / V layouts (wf_norm.h k_tile_off / v_tile_off) are the A operands of
-// v_mfma_f32_16x16x32_bf16 as they lie: S^T (16 keys x 16 rows) = K Q^T, two per tile, whose accumulator leaves
-// lane (row l16, quarter q4) with the scores of keys 8 q4 .. 8 q4 + 7 -- the B operand of O^T (16 dims x 16 rows) =
-// V^T P^T. Probabilities never leave their lane; no LDS and no barrier until the waves' records meet.
+// Tiles: the pool's 32-key K / V layouts (wf_norm.h k_tile_off / v_tile_off) are the A operands of the matrix cores as they
+// lie: S^T (keys x rows) = K Q^T, whose accumulator leaves a lane with groups of 8 neighbouring keys of one row -- the B
+// operand of O^T (dims x rows) = V^T P^T. Probabilities never leave their lane; no LDS and no barrier until the
+// waves' records meet.
 // The running max is raised only when a tile passes it by 2^8 (its exchange between the four lanes of a row and
 // the rescaling of o are rare then): p <= 2^8 is as exact in bf16 and 32 bits as p <= 1.
 //
@@ -32,18 +33,9 @@ typedef __bf16 pf_bf8 __attribute__((ext_vector_type(8)));
 typedef float pf_f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPfDim = 128, kPfPage = 32;
-constexpr int kPfMaxRecords = 64;          // splits of each part
-#ifndef PF_APART
-#define PF_APART 128
-#endif
-#ifndef PF_NP
-#define PF_NP 256
-#endif
-#ifndef PF_NS
-#define PF_NS 2048
-#endif
-constexpr int kPfMinTiles = 4;             // prefix: a tile a wave at least
-constexpr int kPfMinSuffix = 8;            // suffix: two
+constexpr int kPfMaxRecords = 64;          // splits of each part: a lane each in the join, twice
+constexpr int kPfMinTiles = 12;            // tiles of a prefix range: a record costs its write and read in the join (8: +20% behind 1024 keys)
+constexpr int kPfMinSuffix = 8;            // of a suffix range: two a wave
 constexpr float kPfLn2 = 0.69314718055994530942f;
 
 struct PfArgs {
@@ -374,7 +366,7 @@ __device__ __forceinline__ void pf_merge(const PfArgs& a, PfShared<W>& sm, const
 // ---------------------------------------------------------------------------------------------
 // Shared prefixes. Block (kv head and key range, rounded up to 8, tile of MT rows): the row tiles of one (head, range)
 // are 8 k workgroups apart, so one XCD's L2 serves them all. A tile's rows are taken in runs of sequences with one
-// prefix, in the smallest of 16, 32 or 64 rows that holds the run.
+// prefix, in 16 or 32 rows.
 // ---------------------------------------------------------------------------------------------
 template <int QDT>
 constexpr int kPfTerms = QDT == DT_BF16 ? 1 : QDT == DT_F16 ? 2 : 3;
@@ -427,11 +419,6 @@ __device__ void pf_prefix(const PfArgs& a, void* lds, int x, int tile) {
         const int k0 = z * per, k1 = min(k0 + per, tiles);
         if (k0 >= k1) continue;  // the whole workgroup
         const int64_t ra = max(r0, (int64_t)(b0 + i) * a.G), rb = min(r1, (int64_t)(b0 + j) * a.G);  // its rows
-        if constexpr (MT > 32)
-            if (rb - ra > 32) {
-                pf_run<KVQ, QDT, 32, 2>(a, lds, h, z, ra, rb, P, owner, k0, k1);
-                continue;
-            }
         if constexpr (MT > 16)
             if (rb - ra > 16) {
                 pf_run<KVQ, QDT, 32, 1>(a, lds, h, z, ra, rb, P, owner, k0, k1);
@@ -475,23 +462,20 @@ __device__ void pf_suffix(const PfArgs& a, void* lds, int z, int hc, int b) {
     });
 }
 
-// MT > 0: the prefixes, row tiles of MT, in the first np workgroups; SUF: the other keys in the rest.
-template <int KVQ, int QDT, int MT, bool SUF>
-__global__ __launch_bounds__(256, MT == 64 || (MT == 32 && QDT != DT_BF16) ? 1 : 2) void k_shared_prefix(PfArgs a, int np) {
-    __shared__ PfShared<(MT > 16 ? 32 : 16)> sm;
+// The first np workgroups the prefixes, in row tiles of MT; the others the other keys: the one part waits for the
+// matrix cores and L1, the other for HBM.
+template <int KVQ, int QDT, int MT>
+__global__ __launch_bounds__(256, MT == 32 && QDT != DT_BF16 ? 1 : 2) void k_shared_prefix(PfArgs a, int np) {
+    __shared__ PfShared<MT> sm;
     int x = blockIdx.x;
-    if constexpr (MT > 0) {
-        if (x < np) {
-            const int w = (a.Hkv * a.NP + 7) / 8 * 8;
-            pf_prefix<KVQ, QDT, MT>(a, &sm, x % w, x / w);
-            return;
-        }
+    if (x < np) {
+        const int w = (a.Hkv * a.NP + 7) / 8 * 8;
+        pf_prefix<KVQ, QDT, MT>(a, &sm, x % w, x / w);
+        return;
     }
-    if constexpr (SUF) {
-        x -= np;
-        const int hc = a.Hkv * ((a.G + 15) / 16), z = x % a.NS, y = x / a.NS;
-        pf_suffix<KVQ, QDT>(a, &sm, z, y % hc, y / hc);
-    }
+    x -= np;
+    const int hc = a.Hkv * ((a.G + 15) / 16), z = x % a.NS, y = x / a.NS;
+    pf_suffix<KVQ, QDT>(a, &sm, z, y % hc, y / hc);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -542,18 +526,17 @@ __global__ __launch_bounds__(256) void k_prefix_join(PfArgs a, int odt) {
 
 struct PfPlan {
     int MT, NP, NS, np, ns;  // rows of a prefix workgroup, splits, workgroups
-    bool apart;              // the prefixes in a launch of their own
 };
 // Launch shape from what the host knows: rows, kv heads and the table's width (an upper bound of every length).
 static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
     const int64_t rows = (int64_t)B * (Hq / Hkv), groups = (Hq / Hkv + 15) / 16;
     PfPlan p;
-    p.apart = rows > 32 && cols > PF_APART && dt == DT_BF16;
-    p.MT = rows <= 16 ? 16 : p.apart ? 64 : 32;
+    p.MT = rows <= 16 ? 16 : 32;
     const int64_t tiles = (rows + p.MT - 1) / p.MT;
     auto clamp = [](int64_t v, int64_t hi) { return (int)max((int64_t)1, min(min(v, hi), (int64_t)kPfMaxRecords)); };
-    p.NP = clamp((p.apart ? 256 : PF_NP) / (tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
-    p.NS = clamp(PF_NS / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);
+    // prefix ranges: as many workgroups as the device holds at once, two a CU (one where q's further terms take the registers)
+    p.NP = clamp((dt == DT_BF16 ? 512 : 256) / (tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
+    p.NS = clamp(512 / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);
     p.np = B > 1 ? (int)(((int64_t)Hkv * p.NP + 7) / 8 * 8 * tiles) : 0;  // one sequence shares nothing
     p.ns = (int)(p.NS * Hkv * groups * B);
     return p;
@@ -561,17 +544,9 @@ static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
 
 template <int KVQ, int QDT>
 static void pf_launch(const PfArgs& a, const PfPlan& p, int odt, hipStream_t st) {
-    const dim3 block(256);
-    if (p.apart) {
-        if constexpr (QDT == DT_BF16) {
-            hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 64, false>), dim3(p.np), block, 0, st, a, p.np);
-            hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 0, true>), dim3(p.ns), block, 0, st, a, 0);
-        }
-    } else if (p.MT == 16) {
-        hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 16, true>), dim3(p.np + p.ns), block, 0, st, a, p.np);
-    } else {
-        hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 32, true>), dim3(p.np + p.ns), block, 0, st, a, p.np);
-    }
+    const dim3 grid(p.np + p.ns), block(256);
+    if (p.MT == 16) hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 16>), grid, block, 0, st, a, p.np);
+    else hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 32>), grid, block, 0, st, a, p.np);
     hipLaunchKernelGGL(k_prefix_join, dim3((unsigned)(((int64_t)a.B * a.Hq + 3) / 4)), block, 0, st, a, odt);
 }
 
