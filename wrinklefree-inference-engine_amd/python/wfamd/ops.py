@@ -9,6 +9,7 @@ RuntimeError (KernelError) for HIP failures.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
@@ -408,30 +409,51 @@ def decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_st
 # Serving operators around the paged decode path: page plans, rotary positions, log probabilities.
 # Device tensors only, all on one device; they run on that device's current stream.
 # ---------------------------------------------------------------------------------------------
-def _serve_args(name: str, dev: torch.device, **tensors) -> None:
-    """ValueError unless every tensor is on `dev`, a HIP device."""
+# These run once a layer or once a token, where the host's time counts: arguments are looked over in one expression, and
+# what is wrong is worked out only when something is.
+def _one_device(name: str, **tensors) -> None:
+    """ValueError that says which tensor is not on the first one's device, or that this is not a HIP device."""
+    dev = next(iter(tensors.values())).device
     for what, t in tensors.items():
         if t is not None and t.device != dev:
             raise ValueError(f"{name}: {what} is on {t.device}, expected one HIP device ({dev})")
-    if dev.type != "cuda":
-        raise ValueError(f"{name}: device tensors only, got {dev}")
+    raise ValueError(f"{name}: device tensors only, got {dev}")
 
 
-def _int32_rows(name: str, what: str, t: torch.Tensor, n: Optional[int] = None) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
-        raise ValueError(f"{name}: {what} must be a contiguous int32 [{'n' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
+def _int32_rows(name: str, n, **tensors) -> None:
+    """ValueError unless every tensor is a contiguous int32 [n]."""
+    for what, t in tensors.items():
+        if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name}: {what} must be a contiguous int32 [{n}], got {t.dtype} {tuple(t.shape)}")
+
+
+def _is_rows(t: torch.Tensor, n: int) -> bool:
+    return t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous()
+
+
+def _table_stride(name: str, t: torch.Tensor, b: int) -> int:
+    """The row stride of an int32 [b, blocks] page table whose rows are contiguous."""
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != b or (b and t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: page_table must be int32 [{b}, blocks] with contiguous rows, got {t.dtype} {tuple(t.shape)}")
+    return t.stride(0) if b > 1 else t.shape[1]
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a torch.cuda.Stream around it (2 us)
 
 
-def _call_on(dev: torch.device, name: str, *args) -> None:
-    """Launch on dev's current stream, with dev current (kernels go to the device that is current)."""
-    if dev.index == torch.cuda.current_device():
-        call(name, *args, _raw_stream(dev.index))
+def _call_on(index: int, name: str, *args) -> None:
+    """Launch on the current stream of device `index`, with it current (kernels go to the device that is current)."""
+    if index == torch.cuda.current_device():
+        call(name, *args, _raw_stream(index))
         return
-    with torch.cuda.device(dev):
-        call(name, *args, _raw_stream(dev.index))
+    with torch.cuda.device(index):
+        call(name, *args, _raw_stream(index))
+
+
+@functools.lru_cache(maxsize=256)
+def _ws_bytes(name: str, *sizes: int) -> int:
+    """A workspace size: host arithmetic on sizes alone."""
+    return int(getattr(_lib.load(), name)(*sizes))
 
 
 class KVPagePlan(NamedTuple):
@@ -453,28 +475,30 @@ def kv_page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
     sizes the token arrays (the sum of new_lens, or a bound). `pages` / `slots` are what KVCacheManager.scatter_kv
     takes. The first counts[2] of free_pages are in use afterwards; a sequence that does not fit its table row or
     the free list is refused whole (counts[3]) and its tokens have page -1."""
-    dev = cached_lens.device
-    _serve_args("kv_page_plan", dev, new_lens=new_lens, free_pages=free_pages, page_table=page_table)
-    _int32_rows("kv_page_plan", "cached_lens", cached_lens)
-    b = cached_lens.shape[0]
-    _int32_rows("kv_page_plan", "new_lens", new_lens, b)
-    _int32_rows("kv_page_plan", "free_pages", free_pages)
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != b or (
-            b and page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError(f"kv_page_plan: page_table must be int32 [{b}, blocks] with contiguous rows, got {page_table.dtype} "
-                         f"{tuple(page_table.shape)}")
-    n, cols = int(num_tokens), page_table.shape[1]
+    index = cached_lens.get_device()
+    if not index == new_lens.get_device() == free_pages.get_device() == page_table.get_device() or index < 0:
+        _one_device("kv_page_plan", cached_lens=cached_lens, new_lens=new_lens, free_pages=free_pages, page_table=page_table)
+    b = cached_lens.numel()
+    free = free_pages.numel()
+    if not (_is_rows(cached_lens, b) and _is_rows(new_lens, b) and _is_rows(free_pages, free)):
+        _int32_rows("kv_page_plan", b, cached_lens=cached_lens, new_lens=new_lens)
+        _int32_rows("kv_page_plan", free, free_pages=free_pages)
+    ts = _table_stride("kv_page_plan", page_table, b)
+    n = int(num_tokens)
     if n < 0:
         raise ValueError(f"kv_page_plan: num_tokens {n} is negative")
-    pad = -n % 4  # every array begins on a 16-byte line
-    out = torch.empty(4 * (n + pad) + b + 5, dtype=torch.int32, device=dev)
-    pages, _, slots, _, rows, _, pos, _, counts, cu = out.split([n, pad, n, pad, n, pad, n, pad, 4, b + 1])
-    nws = int(_lib.load().wf_kv_page_plan_ws_bytes(b))
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    pad = -n % 4 if n > 4096 else 0  # large arrays begin on 16-byte lines
+    out = torch.empty(4 * (n + pad) + b + 5, dtype=torch.int32, device=cached_lens.device)
+    if pad:
+        pages, _, slots, _, rows, _, pos, _, counts, cu = out.split([n, pad, n, pad, n, pad, n, pad, 4, b + 1])
+    else:
+        pages, slots, rows, pos, counts, cu = out.split([n, n, n, n, 4, b + 1])
+    nws = _ws_bytes("wf_kv_page_plan_ws_bytes", b)
+    ws = torch.empty(nws, dtype=torch.uint8, device=out.device) if nws else None
     base, step = out.data_ptr(), 4 * (n + pad)
-    _call_on(dev, "wf_kv_page_plan", cached_lens.data_ptr(), new_lens.data_ptr(), b, free_pages.data_ptr(), free_pages.shape[0],
-             page_table.data_ptr(), max(page_table.stride(0), cols) if b < 2 else page_table.stride(0), cols, int(page_size), n, base,
-             base + step, base + 2 * step, base + 3 * step, base + 4 * step + 16, base + 4 * step, _ptr(ws))
+    _call_on(index, "wf_kv_page_plan", cached_lens.data_ptr(), new_lens.data_ptr(), b, free_pages.data_ptr(), free, page_table.data_ptr(),
+             ts, page_table.shape[1], int(page_size), n, base, base + step, base + 2 * step, base + 3 * step, base + 4 * step + 16,
+             base + 4 * step, _ptr(ws))
     return KVPagePlan(pages, slots, rows, pos, cu, counts)
 
 
@@ -513,13 +537,6 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: Optio
     return f.to(_device() if device is None else device), scale
 
 
-def _rotary_rows(what: str, t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
-    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or t.dtype != like.dtype:
-        raise ValueError(f"rotary_embed: {what} must be [tokens, heads, head_dim] like q in tokens, head_dim and dtype, got "
-                         f"{t.dtype} {tuple(t.shape)}")
-    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
-
-
 def _no_overlap(t: torch.Tensor) -> bool:
     """No element of a strided tensor shares its place with another (sizes 1 aside)."""
     reach = 1
@@ -536,31 +553,42 @@ def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     (include/wf_bitnet.h wf_rotary_embed). positions [T] int32 or int64; freqs, scale from rotary_frequencies: the first
     2 len(freqs) dims of a head are turned, the rest copied. Returns (q, k) turned: new tensors, or with
     inplace=True the given ones. Each result is rounded once, from 32 bits; the angle is formed in 64."""
-    dev = q.device
-    _serve_args("rotary_embed", dev, q=q, k=k, positions=positions, freqs=freqs)
+    index = q.get_device()
+    if not index == positions.get_device() == freqs.get_device() or index < 0 or (k is not None and k.get_device() != index):
+        _one_device("rotary_embed", q=q, k=k, positions=positions, freqs=freqs)
     code = _dtcode(q)
+    if q.dim() != 3:
+        raise ValueError(f"rotary_embed: q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
+    T, Hq, D = q.shape
+    if k is not None and (k.dim() != 3 or k.shape[0] != T or k.shape[2] != D or k.dtype is not q.dtype):
+        raise ValueError(f"rotary_embed: k must be [{T}, heads, {D}] {q.dtype} as q is, got {k.dtype} {tuple(k.shape)}")
+    if positions.shape != (T,) or positions.dtype not in (torch.int64, torch.int32) or not positions.is_contiguous():
+        raise ValueError(f"rotary_embed: positions must be a contiguous int32 or int64 [{T}], got {positions.dtype} {tuple(positions.shape)}")
+    r = 2 * freqs.numel()
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or not 0 < r <= D:
+        raise ValueError(f"rotary_embed: freqs must be a contiguous float64 [n], 0 < 2 n <= {D}, got {freqs.dtype} {tuple(freqs.shape)}")
     if inplace:
         for what, t in (("q", q), ("k", k)):
-            if t is not None and t.numel() and ((t.stride(-1) != 1 and t.shape[-1] > 1) or not _no_overlap(t)):
+            if t is not None and t.numel() and ((t.stride(-1) != 1 and D > 1) or not _no_overlap(t)):
                 raise ValueError(f"rotary_embed: {what} of strides {t.stride()} cannot be turned in place")
         if k is not None and k.numel() and k.data_ptr() == q.data_ptr():
             raise ValueError("rotary_embed: q and k are the same memory, turned in place it would be turned twice")
-    q = _rotary_rows("q", q, q)
-    T, Hq, D = q.shape
-    Hk = 0
-    if k is not None:
-        k = _rotary_rows("k", k, q)
-        Hk = k.shape[1]
-    if positions.dim() != 1 or positions.shape[0] != T or positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous():
-        raise ValueError(f"rotary_embed: positions must be a contiguous int32 or int64 [{T}], got {positions.dtype} {tuple(positions.shape)}")
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or not 0 < 2 * freqs.shape[0] <= D:
-        raise ValueError(f"rotary_embed: freqs must be a contiguous float64 [n], 0 < 2 n <= {D}, got {freqs.dtype} {tuple(freqs.shape)}")
-    qo = q if inplace else torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    ko = k if inplace or k is None else torch.empty((T, Hk, D), dtype=q.dtype, device=dev)
-    kk, kko = (q, qo) if k is None else (k, ko)
-    _call_on(dev, "wf_rotary_embed", q.data_ptr(), q.stride(0), q.stride(1), Hq, kk.data_ptr(), kk.stride(0), kk.stride(1), Hk, code,
-             positions.data_ptr(), int(positions.dtype == torch.int64), freqs.data_ptr(), T, D, 2 * freqs.shape[0], int(interleaved),
-             float(scale), qo.data_ptr(), qo.stride(0), qo.stride(1), kko.data_ptr(), kko.stride(0), kko.stride(1))
+        qo, ko = q, k
+    else:
+        qo = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        ko = None if k is None else torch.empty((T, k.shape[1], D), dtype=q.dtype, device=q.device)
+        if q.stride(2) != 1:
+            q = q.contiguous()
+        if k is not None and k.stride(2) != 1:
+            k = k.contiguous()
+    qs, qos = q.stride(), qo.stride()
+    if k is None:
+        kargs, koargs = (None, 0, 0, 0), (None, 0, 0)
+    else:
+        ks, kos = k.stride(), ko.stride()
+        kargs, koargs = (k.data_ptr(), ks[0], ks[1], k.shape[1]), (ko.data_ptr(), kos[0], kos[1])
+    _call_on(index, "wf_rotary_embed", q.data_ptr(), qs[0], qs[1], Hq, *kargs, code, positions.data_ptr(),
+             positions.dtype is torch.int64, freqs.data_ptr(), T, D, r, bool(interleaved), scale, qo.data_ptr(), qos[0], qos[1], *koargs)
     return qo, ko
 
 
@@ -579,9 +607,11 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     q's dtype, with return_lse=True also the log of the sum of exponentials [B, Hq] float32. A sequence of no keys
     gives zeros and -inf."""
     name = "shared_prefix_attention"
-    dev = q.device
-    _serve_args(name, dev, q=q, k_pool=k_pool, v_pool=v_pool, page_table=page_table, seq_lens=seq_lens, prefix_rows=prefix_rows,
-                prefix_lens=prefix_lens)
+    index = q.get_device()
+    if index < 0 or not index == k_pool.get_device() == v_pool.get_device() == page_table.get_device() == seq_lens.get_device() == \
+            prefix_rows.get_device() == prefix_lens.get_device():
+        _one_device(name, q=q, k_pool=k_pool, v_pool=v_pool, page_table=page_table, seq_lens=seq_lens, prefix_rows=prefix_rows,
+                    prefix_lens=prefix_lens)
     code = _dtcode(q)
     if kv_dtype not in _KV_QUANT:
         raise ValueError(f"{name}: kv_dtype must be 'bf16', 'fp8' or 'int8', got {kv_dtype!r}")
@@ -589,29 +619,28 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     if q.dim() != 3 or q.shape[2] != 128:
         raise ValueError(f"{name}: q must be [batch, heads, 128], got {tuple(q.shape)}")
     B, Hq, D = q.shape
-    if k_pool.dim() != 3 or k_pool.shape != v_pool.shape or k_pool.shape[2] != 32 * D or k_pool.dtype != kvt or v_pool.dtype != kvt or (
-            k_pool.stride() != v_pool.stride() or k_pool.stride(2) != 1):
+    ks = k_pool.stride()
+    if k_pool.dim() != 3 or k_pool.shape[2] != 4096 or k_pool.dtype is not kvt or v_pool.dtype is not kvt or (
+            k_pool.shape != v_pool.shape or ks != v_pool.stride() or ks[2] != 1):
         raise ValueError(f"{name}: k_pool / v_pool must be {kvt} [pages, kv_heads, {32 * D}] alike, got {k_pool.dtype} {tuple(k_pool.shape)} "
                          f"and {v_pool.dtype} {tuple(v_pool.shape)}")
-    pages, Hkv = k_pool.shape[:2]
+    pages, Hkv, _ = k_pool.shape
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError(f"{name}: {Hq} query heads for {Hkv} kv heads")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B or (
-            B and page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError(f"{name}: page_table must be int32 [{B}, blocks] with contiguous rows, got {page_table.dtype} {tuple(page_table.shape)}")
-    for what, t in (("seq_lens", seq_lens), ("prefix_rows", prefix_rows), ("prefix_lens", prefix_lens)):
-        _int32_rows(name, what, t, B)
-    if q.stride(2) != 1:
+    ts = _table_stride(name, page_table, B)
+    if not (_is_rows(seq_lens, B) and _is_rows(prefix_rows, B) and _is_rows(prefix_lens, B)):
+        _int32_rows(name, B, seq_lens=seq_lens, prefix_rows=prefix_rows, prefix_lens=prefix_lens)
+    qs = q.stride()
+    if qs[2] != 1:
         q = q.contiguous()
+        qs = q.stride()
     cols = page_table.shape[1]
-    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
-    ws = torch.empty(int(_lib.load().wf_shared_prefix_attention_ws_bytes(code, B, Hq, Hkv, cols)), dtype=torch.uint8, device=dev)
-    _call_on(dev, "wf_shared_prefix_attention", q.data_ptr(), code, q.stride(0), q.stride(1), k_pool.data_ptr(), v_pool.data_ptr(), quant,
-             k_pool.stride(0), k_pool.stride(1), pages, page_table.data_ptr(), max(page_table.stride(0), cols) if B < 2 else page_table.stride(0),
-             cols, seq_lens.data_ptr(), prefix_rows.data_ptr(), prefix_lens.data_ptr(), float(k_scale), float(v_scale),
-             float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(D), B, Hq, Hkv, D, out.data_ptr(), out.stride(0),
-             out.stride(1), _ptr(lse), ws.data_ptr())
+    out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    ws = torch.empty(_ws_bytes("wf_shared_prefix_attention_ws_bytes", code, B, Hq, Hkv, cols), dtype=torch.uint8, device=q.device)
+    _call_on(index, "wf_shared_prefix_attention", q.data_ptr(), code, qs[0], qs[1], k_pool.data_ptr(), v_pool.data_ptr(), quant, ks[0], ks[1],
+             pages, page_table.data_ptr(), ts, cols, seq_lens.data_ptr(), prefix_rows.data_ptr(), prefix_lens.data_ptr(), k_scale, v_scale,
+             D ** -0.5 if sm_scale is None else sm_scale, B, Hq, Hkv, D, out.data_ptr(), Hq * D, D, _ptr(lse), ws.data_ptr())
     return (out, lse) if return_lse else out
 
 
@@ -628,8 +657,9 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     """Log probability and rank of one given token a row, the row's entropy and its top_k (<= 64) alternatives,
     from logits [R, V] bf16 / f16 / f32 read once (include/wf_bitnet.h wf_token_logprobs, which also says what rows of
     -inf, NaN or +inf give). tokens [R] int32 or int64; a negative one asks for nothing. Equal logits rank by index."""
-    dev = logits.device
-    _serve_args("token_logprobs", dev, logits=logits, tokens=tokens)
+    index = logits.get_device()
+    if index < 0 or (tokens is not None and tokens.get_device() != index):
+        _one_device("token_logprobs", logits=logits, tokens=tokens)
     code = _dtcode(logits)
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"token_logprobs: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
@@ -637,22 +667,23 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     k = int(top_k)
     if not 0 <= k <= min(64, V):
         raise ValueError(f"token_logprobs: top_k {k} not in [0, {min(64, V)}]")
-    if V > 1 and logits.stride(1) != 1 or R > 1 and logits.stride(0) < V:
+    ld, step = logits.stride()
+    if V > 1 and step != 1 or R > 1 and ld < V:
         logits = logits.contiguous()
-    if tokens is not None and (tokens.dim() != 1 or tokens.shape[0] != R or tokens.dtype not in (torch.int32, torch.int64)
-                               or not tokens.is_contiguous()):
-        raise ValueError(f"token_logprobs: tokens must be a contiguous int32 or int64 [{R}], got {tokens.dtype} {tuple(tokens.shape)}")
+        ld = V
+    dev = logits.device
     lp = rank = None
     if tokens is not None:
+        if tokens.shape != (R,) or tokens.dtype not in (torch.int32, torch.int64) or not tokens.is_contiguous():
+            raise ValueError(f"token_logprobs: tokens must be a contiguous int32 or int64 [{R}], got {tokens.dtype} {tuple(tokens.shape)}")
         lp = torch.empty(R, dtype=torch.float32, device=dev)
         rank = torch.empty(R, dtype=torch.int32, device=dev)
     ent = torch.empty(R, dtype=torch.float32, device=dev)
     ids = torch.empty((R, k), dtype=torch.int32, device=dev)
     top = torch.empty((R, k), dtype=torch.float32, device=dev)
-    ws = torch.empty(int(_lib.load().wf_token_logprobs_ws_bytes(R, V, k)), dtype=torch.uint8, device=dev)
-    _call_on(dev, "wf_token_logprobs", logits.data_ptr(), code, logits.stride(0), R, V, _ptr(tokens),
-             int(tokens is not None and tokens.dtype == torch.int64), k, _ptr(lp), _ptr(rank), ent.data_ptr(), ids.data_ptr(),
-             top.data_ptr(), ws.data_ptr())
+    ws = torch.empty(_ws_bytes("wf_token_logprobs_ws_bytes", R, V, k), dtype=torch.uint8, device=dev)
+    _call_on(index, "wf_token_logprobs", logits.data_ptr(), code, ld, R, V, _ptr(tokens), tokens is not None and tokens.dtype is torch.int64,
+             k, _ptr(lp), _ptr(rank), ent.data_ptr(), ids.data_ptr(), top.data_ptr(), ws.data_ptr())
     return TokenLogprobs(lp, rank, ent, ids, top)
 
 
