@@ -48,4 +48,13 @@ __device__ __forceinline__ uint4 i8x8_to_bf16(uint2 r) {
     return make_uint4(i8x2_to_bf16(x, 0), i8x2_to_bf16(x, 16), i8x2_to_bf16(y, 0), i8x2_to_bf16(y, 16));
 }
 
+// The same with the byte picked and sign-extended by the conversion itself (one instruction a code, 12 for 8 codes
+// with the packing, against 22)
+__device__ __forceinline__ uint32_t i8x2_to_bf16_sext(uint32_t u, int sh) {
+    return pk_bf16((float)(int8_t)(u >> sh), (float)(int8_t)(u >> (sh + 8)));
+}
+__device__ __forceinline__ uint4 i8x8_to_bf16_sext(uint2 r) {
+    return make_uint4(i8x2_to_bf16_sext(r.x, 0), i8x2_to_bf16_sext(r.x, 16), i8x2_to_bf16_sext(r.y, 0), i8x2_to_bf16_sext(r.y, 16));
+}
+
 }  // namespace wf

@@ -91,7 +91,7 @@ struct PfFrag {
     static __device__ __forceinline__ uint4 bf(T t) {
         if constexpr (KVQ == 0) return t;
         else if constexpr (KVQ == 1) return fp8x8_to_bf16(t);
-        else return i8x8_to_bf16(t);
+        else return i8x8_to_bf16_sext(t);
     }
 };
 
