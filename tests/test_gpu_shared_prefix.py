@@ -335,3 +335,46 @@ def test_a_decode_step_from_lengths_to_log_probabilities():
     assert (lp.top_logprobs[:, 0].double() - ref.amax(1)).abs().max().item() <= 2.0 ** -24 * 300  # 300 roundings: 16 terms a lane, |log p| < 20
     best = lp.ranks == 1
     assert best.any() and torch.equal(lp.logprobs[best], lp.top_logprobs[:, 0][best])
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8", "fp8"])
+def test_decoder_reserves_a_batch_and_attends_over_its_pool(kv):
+    """BitNetDecoder.reserve_batch gives the pages that reserve gives one sequence after the other; its
+    shared_prefix_attention reads what a step's cache holds; token_logprobs is over the step's logits."""
+    from wfamd import ops
+    from wfamd.model import BitNetConfig, BitNetDecoder, synthetic_weights
+    cfg = BitNetConfig(hidden=512, layers=2, n_heads=4, n_kv_heads=2, head_dim=D, inter=768, vocab=1024, max_seq=256)
+    w = synthetic_weights(cfg)
+    a, b = (BitNetDecoder(cfg, w, batch=16, num_pages=96, page_seed=5, kv_dtype=kv, kv_scale=(0.05, 0.03) if kv != "bf16" else None)
+            for _ in range(2))
+    rng = torch.Generator().manual_seed(1)
+    for counts in (torch.randint(0, 70, (16,), generator=rng).tolist(), [0] * 16, torch.randint(40, 160, (16,), generator=rng).tolist()):
+        a.reserve_batch(counts)
+        for i, n in enumerate(counts):
+            b.reserve(i, n)
+        assert torch.equal(a.page_table, b.page_table) and all((x == y).all() for x, y in zip(a.seq_pages, b.seq_pages))
+    free = a.pool.num_free_pages()
+    with pytest.raises(RuntimeError):
+        a.reserve_batch([256] * 16)
+    assert a.pool.num_free_pages() == free
+    for bad in ([1] * 15, [257] + [1] * 15, [-1] + [1] * 15):
+        with pytest.raises(ValueError):
+            a.reserve_batch(bad)
+    pos = [len(p) * 32 - 1 for p in a.seq_pages]
+    k = torch.randn(16, 2, 160, D, generator=torch.Generator("cuda").manual_seed(2), device="cuda").bfloat16()
+    for layer in range(2):
+        a.load_kv(layer, k, -k, lengths=pos)
+    a.set_state(list(range(16)), [p - 1 for p in pos])
+    a.step(graph=False)
+    a.check()
+    p = a.token_logprobs(a.tokens, top_k=2)
+    assert (p.ranks == 1).all() and torch.equal(p.top_ids[:, 0], a.tokens)
+    ref = a.logits.double().log_softmax(1)
+    assert (p.logprobs.double() - ref.gather(1, a.tokens.long()[:, None])[:, 0]).abs().max().item() <= 2.0 ** -24 * 300
+    # the last layer's attention of the step, from the pool by this operator: within the two kernels' roundings of P and of the output
+    q = a.attention_records()[0]
+    got, want = a.shared_prefix_attention(1, q, i32(pos), i32([-1] * 16), i32([0] * 16)), a.attention_row()
+    assert (got.double() - want.double()).abs().max().item() <= 6 * 2.0 ** -8 * want.double().abs().max().item()
+    c = dict(q=q, k_pool=a.k_cache[1], v_pool=a.v_cache[1], page_table=a.page_table, seq_lens=i32(pos), prefix_rows=i32([0] * 16),
+             prefix_lens=i32([60] * 16), kv_dtype=kv, k_scale=0.05 if kv != "bf16" else 1.0, v_scale=0.03 if kv != "bf16" else 1.0)
+    assert torch.equal(a.shared_prefix_attention(1, q, c["seq_lens"], c["prefix_rows"], c["prefix_lens"]), check(c)[0])

@@ -28,6 +28,7 @@ struct PlanArgs {
     int cols, page, shift, T;  // shift: log2 of page, or -1
     int32_t *pages, *slots, *rows, *pos, *cu, *counts;
     int32_t *ws_off, *ws_cu;  // [B + 1] each, B > kPlanLdsSeqs only
+    int lens16;               // both length arrays are 16-byte aligned
 };
 
 // Lengths are clamped to >= 0; sums are 64 bits and saturate where they are stored as 32.
@@ -79,15 +80,22 @@ __device__ void plan_scan(const PlanArgs& a, int32_t* off, int32_t* cu, int32_t*
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (threadIdx.x == 0) sh_taken = sh_refused = 0;
     int64_t cn = 0, ct = 0;  // sums before this round
+    int taken = 0, refused = 0;
     for (int b0 = 0; b0 < a.B; b0 += kPlanThreads * E) {
         PlanSeq s[E];
         int64_t n = 0, t = 0;
         int c[E], f[E];
+        const int bt = b0 + E * threadIdx.x;
+        if (E == 4 && a.lens16 && bt + 4 <= a.B) {
+            const int4 v = *reinterpret_cast<const int4*>(a.cached + bt), w = *reinterpret_cast<const int4*>(a.fresh + bt);
+            c[0] = v.x, c[E / 4] = v.y, c[E / 2] = v.z, c[E - 1] = v.w;
+            f[0] = w.x, f[E / 4] = w.y, f[E / 2] = w.z, f[E - 1] = w.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int b = b0 + E * threadIdx.x + i;
-            c[i] = b < a.B ? a.cached[b] : 0;
-            f[i] = b < a.B ? a.fresh[b] : 0;
+            for (int i = 0; i < E; ++i) {
+                c[i] = bt + i < a.B ? a.cached[bt + i] : 0;
+                f[i] = bt + i < a.B ? a.fresh[bt + i] : 0;
+            }
         }
 #pragma unroll
         for (int i = 0; i < E; ++i) {
@@ -111,13 +119,20 @@ __device__ void plan_scan(const PlanArgs& a, int32_t* off, int32_t* cu, int32_t*
             if (b < a.B) {
                 off[b] = sat32(on), cu[b] = sat32(ot);
                 if (cl) cl[b] = c[i], nl[b] = f[i];
-                if (report) {
-                    if (!s[i].fit(on, a.F)) atomicAdd(&sh_refused, 1);
-                    else if (s[i].need) atomicMax(&sh_taken, (int)(on + s[i].need));
-                }
+                const bool fit = s[i].fit(on, a.F);
+                refused += !fit;
+                if (fit && s[i].need) taken = max(taken, (int)(on + s[i].need));
             }
             on += s[i].need;
             ot += s[i].n;
+        }
+    }
+    if (report) {  // one LDS atomic a wave: one a sequence kept the first workgroup 8 us behind the others at 1024 sequences
+        taken = wave_reduce(taken, [](int x, int y) { return max(x, y); }, 0);
+        refused = wave_sum_i(refused);
+        if (lane == 0) {
+            atomicMax(&sh_taken, taken);
+            atomicAdd(&sh_refused, refused);
         }
     }
     __syncthreads();
@@ -147,28 +162,10 @@ __device__ __forceinline__ int plan_find(const int32_t* at, int B, int v) {
     return lo;
 }
 
-// LDS: the sums in LDS, scanned here. N: tokens a thread takes.
-template <bool LDS, int N>
-__global__ __launch_bounds__(kPlanThreads) void k_page_plan(PlanArgs a) {
-    __shared__ int32_t sm[LDS ? 4 * (kPlanLdsSeqs + 1) : 1];
-    const int32_t *off = a.ws_off, *cu = a.ws_cu, *cl = a.cached, *nl = a.fresh;
-    if constexpr (LDS) {
-        constexpr int S = kPlanLdsSeqs + 1;
-        if (a.B <= kPlanThreads) plan_scan<1>(a, sm, sm + S, sm + 2 * S, sm + 3 * S, blockIdx.x == 0);
-        else plan_scan<4>(a, sm, sm + S, sm + 2 * S, sm + 3 * S, blockIdx.x == 0);
-        off = sm, cu = sm + S, cl = sm + 2 * S, nl = sm + 3 * S;
-    }
-    const int me = blockIdx.x * kPlanThreads + threadIdx.x, all = gridDim.x * kPlanThreads;
-    // the pages that are taken, one a thread: into their sequence's row
-    for (int i = me, n = min(off[a.B], a.F); i < n; i += all) {
-        const int b = plan_find(off, a.B, i);
-        const PlanSeq s = plan_seq(a, cl[b], nl[b]);
-        if (s.fit(off[b], a.F)) a.table[b * a.ts + s.have + (i - off[b])] = a.free_pages[i];
-    }
-    for (int b = me; b <= a.B; b += all) a.cu[b] = cu[b];
-    // the tokens
-    const int64_t t0 = (int64_t)me * N;
-    if (t0 >= a.T) return;
+// tokens t0 .. t0 + N - 1 (their sums and lengths in LDS or global memory)
+template <int N>
+__device__ __forceinline__ void plan_tokens(const PlanArgs& a, const int32_t* off, const int32_t* cu, const int32_t* cl, const int32_t* nl,
+                                            int64_t t0) {
     int pg[N], sl[N], rw[N], ps[N];
     int b = t0 < cu[a.B] ? plan_find(cu, a.B, (int)t0) : -1, known = -1;
     int64_t o = 0;
@@ -192,7 +189,12 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_plan(PlanArgs a) {
         if (!fit) continue;
         const uint32_t blk = plan_div(a, pos);
         sl[i] = (int)(pos - blk * (uint32_t)a.page);
-        pg[i] = blk < s.have ? a.table[b * a.ts + blk] : a.free_pages[o + blk - s.have];
+        if (i > 0 && sl[i] > 0 && rw[i - 1] == b) {  // the token before stands on the same page
+            pg[i] = pg[i - 1];
+        } else {
+            const int32_t* at = blk < s.have ? a.table + b * a.ts + blk : a.free_pages + (o + blk - s.have);
+            pg[i] = *at;
+        }
     }
     if constexpr (N == 4) {
         if (t0 + 4 <= a.T) {  // the launch saw to the arrays' alignment
@@ -213,11 +215,33 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_plan(PlanArgs a) {
     }
 }
 
+// LDS: the sums in LDS, scanned here. N: tokens a thread takes.
+template <bool LDS, int N>
+__global__ __launch_bounds__(kPlanThreads) void k_page_plan(PlanArgs a) {
+    __shared__ int32_t sm[LDS ? 4 * (kPlanLdsSeqs + 1) : 1];
+    const int32_t *off = a.ws_off, *cu = a.ws_cu, *cl = a.cached, *nl = a.fresh;
+    if constexpr (LDS) {
+        constexpr int S = kPlanLdsSeqs + 1;
+        if (a.B <= kPlanThreads) plan_scan<1>(a, sm, sm + S, sm + 2 * S, sm + 3 * S, blockIdx.x == 0);
+        else plan_scan<4>(a, sm, sm + S, sm + 2 * S, sm + 3 * S, blockIdx.x == 0);
+        off = sm, cu = sm + S, cl = sm + 2 * S, nl = sm + 3 * S;
+    }
+    const int me = blockIdx.x * kPlanThreads + threadIdx.x, all = gridDim.x * kPlanThreads;
+    // the pages that are taken, one a thread: into their sequence's row
+    for (int64_t i = me, n = min(off[a.B], a.F); i < n; i += all) {
+        const int b = plan_find(off, a.B, (int)i);
+        const PlanSeq s = plan_seq(a, cl[b], nl[b]);
+        if (s.fit(off[b], a.F)) a.table[b * a.ts + s.have + (i - off[b])] = a.free_pages[i];
+    }
+    for (int b = me; b <= a.B; b += all) a.cu[b] = cu[b];
+    if ((int64_t)me * N < a.T) plan_tokens<N>(a, off, cu, cl, nl, (int64_t)me * N);
+}
+
 template <bool LDS>
 static void plan_launch(const PlanArgs& a, hipStream_t st) {
     const bool wide = a.T >= kPlanWide && aligned16(a.pages) && aligned16(a.slots) && aligned16(a.rows) && aligned16(a.pos);
     const int each = kPlanThreads * (wide ? 4 : 1);
-    // a thread for every token; at least one for every second sequence up to 64 workgroups (the table's entries)
+    // a thread for every token (or four); at least a workgroup for every 512 sequences (the table's entries)
     const int grid = max(max((a.T + each - 1) / each, min((a.B + 511) / 512, 64)), 1);
     if (wide) hipLaunchKernelGGL((k_page_plan<LDS, 4>), dim3(grid), dim3(kPlanThreads), 0, st, a);
     else hipLaunchKernelGGL((k_page_plan<LDS, 1>), dim3(grid), dim3(kPlanThreads), 0, st, a);
@@ -248,7 +272,7 @@ int wf_kv_page_plan(const int32_t* cached_lens, const int32_t* new_lens, int B, 
     WF_REQUIRE(num_tokens <= 0x7fffffff - 4096, "kv_page_plan: too many tokens");
     PlanArgs a{cached_lens, new_lens, B, free_pages, num_free, page_table, table_stride, max_blocks, page_size,
                page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size), num_tokens, pages, slots, rows, positions, cu_tokens, counts,
-               nullptr, nullptr};
+               nullptr, nullptr, aligned16(cached_lens) && aligned16(new_lens)};
     hipStream_t st = as_stream(stream);
     if (B <= kPlanLdsSeqs) {
         plan_launch<true>(a, st);

@@ -362,6 +362,34 @@ class BitNetDecoder:
         self._pt_host[b, :len(self.seq_pages[b])] = self.seq_pages[b]
         self.page_table[b].copy_(torch.from_numpy(self._pt_host[b]))
 
+    def reserve_batch(self, n_tokens) -> None:
+        """reserve() for the whole batch: n_tokens[b] is sequence b's token count (0: as it is). The page table's rows are
+        filled by one device launch (ops.kv_page_plan) instead of a host copy per sequence; pages go to the
+        sequences in slot order."""
+        if not self.paged:
+            raise ValueError("reserve_batch needs a paged decoder (num_pages > 0)")
+        want = [int(n) for n in n_tokens]
+        if len(want) != self.batch or min(want) < 0 or max(want) > self.cfg.max_seq:
+            raise ValueError(f"reserve_batch: {self.batch} token counts of 0 .. {self.cfg.max_seq} expected")
+        held = [len(p) for p in self.seq_pages]
+        need = [max(0, (n + 31) // 32 - h) for n, h in zip(want, held)]
+        total = sum(need)
+        if total == 0:
+            return
+        got = self.pool.allocate_pages(total)
+        if len(got) != total:
+            raise RuntimeError(f"KV page pool exhausted ({self.pool.num_free_pages()} free, {total} needed)")
+        at = 0
+        for b, n in enumerate(need):
+            if n:
+                self.seq_pages[b] = np.concatenate([self.seq_pages[b], got[at:at + n]])
+                self._pt_host[b, :len(self.seq_pages[b])] = self.seq_pages[b]
+                at += n
+        # one transfer: tokens held, tokens to come (whole pages of both), the pages in order
+        host = torch.from_numpy(np.concatenate([32 * np.asarray(held), 32 * np.asarray(need), got]).astype(np.int32))
+        held_d, need_d, got_d = host.to(self.dev).split([self.batch, self.batch, total])
+        ops.kv_page_plan(held_d, need_d, got_d, self.page_table, 0)
+
     def map_pages(self, b: int, pages) -> None:
         """Point sequence b's 32-token blocks at `pages` (block j -> pages[j]): pages a caller allocated
         from this decoder's pool itself, e.g. through sgl_kernel.kvcache.KVCacheManager(backing=self),
@@ -568,6 +596,21 @@ class BitNetDecoder:
             raise ValueError("q must be [batch, n_heads, head_dim] bf16 on the decoder's device")
         q = q.contiguous()
         ops.device_copy(v.q, q.data_ptr(), q.numel() * 2)
+
+    def token_logprobs(self, tokens: Optional[torch.Tensor] = None, top_k: int = 0) -> "ops.TokenLogprobs":
+        """Log probability and rank of one token per sequence (e.g. self.tokens, the greedy choices), entropy and the
+        top_k alternatives of the last step's logits (ops.token_logprobs)."""
+        return ops.token_logprobs(self.logits, tokens, top_k)
+
+    def shared_prefix_attention(self, layer: int, q: torch.Tensor, seq_lens: torch.Tensor, prefix_rows: torch.Tensor,
+                                prefix_lens: torch.Tensor, page_table: Optional[torch.Tensor] = None, **kw):
+        """ops.shared_prefix_attention over a layer of this decoder's paged pool (its K/V type and scales): q [B, Hq, 128],
+        one token per row of page_table (default: the decoder's own table)."""
+        if not self.paged:
+            raise ValueError("shared_prefix_attention needs a paged decoder (num_pages > 0)")
+        ks, vs = (float(x) for x in self.kv_scale[layer]) if self.kv_fp8 else (1.0, 1.0)
+        return ops.shared_prefix_attention(q, self.k_cache[layer], self.v_cache[layer], self.page_table if page_table is None else page_table,
+                                           seq_lens, prefix_rows, prefix_lens, kv_dtype=self.kv_dtype, k_scale=ks, v_scale=vs, **kw)
 
     @property
     def weight_bytes(self) -> int:
