@@ -427,10 +427,6 @@ def _int32_rows(name: str, n, **tensors) -> None:
             raise ValueError(f"{name}: {what} must be a contiguous int32 [{n}], got {t.dtype} {tuple(t.shape)}")
 
 
-def _is_rows(t: torch.Tensor, n: int) -> bool:
-    return t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous()
-
-
 def _table_stride(name: str, t: torch.Tensor, b: int) -> int:
     """The row stride of an int32 [b, blocks] page table whose rows are contiguous."""
     if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != b or (b and t.shape[1] > 1 and t.stride(1) != 1):
@@ -441,13 +437,14 @@ def _table_stride(name: str, t: torch.Tensor, b: int) -> int:
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a torch.cuda.Stream around it (2 us)
 
 
-def _call_on(index: int, name: str, *args) -> None:
+def _call_on(index: int, name: str, args: tuple) -> None:
     """Launch on the current stream of device `index`, with it current (kernels go to the device that is current)."""
-    if index == torch.cuda.current_device():
-        call(name, *args, _raw_stream(index))
-        return
-    with torch.cuda.device(index):
-        call(name, *args, _raw_stream(index))
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _call_on(index, name, args)
+    rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 @functools.lru_cache(maxsize=256)
@@ -480,7 +477,8 @@ def kv_page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
         _one_device("kv_page_plan", cached_lens=cached_lens, new_lens=new_lens, free_pages=free_pages, page_table=page_table)
     b = cached_lens.numel()
     free = free_pages.numel()
-    if not (_is_rows(cached_lens, b) and _is_rows(new_lens, b) and _is_rows(free_pages, free)):
+    if not (cached_lens.dtype is new_lens.dtype is free_pages.dtype is torch.int32 and cached_lens.shape == (b,) == new_lens.shape and
+            free_pages.shape == (free,) and cached_lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous()):
         _int32_rows("kv_page_plan", b, cached_lens=cached_lens, new_lens=new_lens)
         _int32_rows("kv_page_plan", free, free_pages=free_pages)
     ts = _table_stride("kv_page_plan", page_table, b)
@@ -496,9 +494,9 @@ def kv_page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
     nws = _ws_bytes("wf_kv_page_plan_ws_bytes", b)
     ws = torch.empty(nws, dtype=torch.uint8, device=out.device) if nws else None
     base, step = out.data_ptr(), 4 * (n + pad)
-    _call_on(index, "wf_kv_page_plan", cached_lens.data_ptr(), new_lens.data_ptr(), b, free_pages.data_ptr(), free, page_table.data_ptr(),
+    _call_on(index, "wf_kv_page_plan", (cached_lens.data_ptr(), new_lens.data_ptr(), b, free_pages.data_ptr(), free, page_table.data_ptr(),
              ts, page_table.shape[1], int(page_size), n, base, base + step, base + 2 * step, base + 3 * step, base + 4 * step + 16,
-             base + 4 * step, _ptr(ws))
+             base + 4 * step, _ptr(ws)))
     return KVPagePlan(pages, slots, rows, pos, cu, counts)
 
 
@@ -587,8 +585,8 @@ def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     else:
         ks, kos = k.stride(), ko.stride()
         kargs, koargs = (k.data_ptr(), ks[0], ks[1], k.shape[1]), (ko.data_ptr(), kos[0], kos[1])
-    _call_on(index, "wf_rotary_embed", q.data_ptr(), qs[0], qs[1], Hq, *kargs, code, positions.data_ptr(),
-             positions.dtype is torch.int64, freqs.data_ptr(), T, D, r, bool(interleaved), scale, qo.data_ptr(), qos[0], qos[1], *koargs)
+    _call_on(index, "wf_rotary_embed", (q.data_ptr(), qs[0], qs[1], Hq, *kargs, code, positions.data_ptr(),
+             positions.dtype is torch.int64, freqs.data_ptr(), T, D, r, bool(interleaved), scale, qo.data_ptr(), qos[0], qos[1], *koargs))
     return qo, ko
 
 
@@ -628,7 +626,9 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError(f"{name}: {Hq} query heads for {Hkv} kv heads")
     ts = _table_stride(name, page_table, B)
-    if not (_is_rows(seq_lens, B) and _is_rows(prefix_rows, B) and _is_rows(prefix_lens, B)):
+    if not (seq_lens.dtype is prefix_rows.dtype is prefix_lens.dtype is torch.int32 and
+            seq_lens.shape == (B,) == prefix_rows.shape == prefix_lens.shape and seq_lens.is_contiguous() and
+            prefix_rows.is_contiguous() and prefix_lens.is_contiguous()):
         _int32_rows(name, B, seq_lens=seq_lens, prefix_rows=prefix_rows, prefix_lens=prefix_lens)
     qs = q.stride()
     if qs[2] != 1:
@@ -638,9 +638,9 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     ws = torch.empty(_ws_bytes("wf_shared_prefix_attention_ws_bytes", code, B, Hq, Hkv, cols), dtype=torch.uint8, device=q.device)
-    _call_on(index, "wf_shared_prefix_attention", q.data_ptr(), code, qs[0], qs[1], k_pool.data_ptr(), v_pool.data_ptr(), quant, ks[0], ks[1],
+    _call_on(index, "wf_shared_prefix_attention", (q.data_ptr(), code, qs[0], qs[1], k_pool.data_ptr(), v_pool.data_ptr(), quant, ks[0], ks[1],
              pages, page_table.data_ptr(), ts, cols, seq_lens.data_ptr(), prefix_rows.data_ptr(), prefix_lens.data_ptr(), k_scale, v_scale,
-             D ** -0.5 if sm_scale is None else sm_scale, B, Hq, Hkv, D, out.data_ptr(), Hq * D, D, _ptr(lse), ws.data_ptr())
+             D ** -0.5 if sm_scale is None else sm_scale, B, Hq, Hkv, D, out.data_ptr(), Hq * D, D, _ptr(lse), ws.data_ptr()))
     return (out, lse) if return_lse else out
 
 
@@ -682,8 +682,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     ids = torch.empty((R, k), dtype=torch.int32, device=dev)
     top = torch.empty((R, k), dtype=torch.float32, device=dev)
     ws = torch.empty(_ws_bytes("wf_token_logprobs_ws_bytes", R, V, k), dtype=torch.uint8, device=dev)
-    _call_on(index, "wf_token_logprobs", logits.data_ptr(), code, ld, R, V, _ptr(tokens), tokens is not None and tokens.dtype is torch.int64,
-             k, _ptr(lp), _ptr(rank), ent.data_ptr(), ids.data_ptr(), top.data_ptr(), ws.data_ptr())
+    _call_on(index, "wf_token_logprobs", (logits.data_ptr(), code, ld, R, V, _ptr(tokens), tokens is not None and tokens.dtype is torch.int64,
+             k, _ptr(lp), _ptr(rank), ent.data_ptr(), ids.data_ptr(), top.data_ptr(), ws.data_ptr()))
     return TokenLogprobs(lp, rank, ent, ids, top)
 
 
