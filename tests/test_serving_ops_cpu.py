@@ -171,3 +171,18 @@ def test_shared_prefix_attention_refusals():
     assert lib.wf_shared_prefix_attention(*{**good, "B": 0}.values()) == _lib.WF_OK
     assert lib.wf_shared_prefix_attention_ws_bytes(1, 0, 4, 1, 8) == 0 and lib.wf_shared_prefix_attention_ws_bytes(1, 2, 4, 3, 8) == 0
     assert lib.wf_shared_prefix_attention_ws_bytes(1, 2, 4, 1, 8) >= 2 * 4 * 2 * 520
+
+
+def test_launch_sizes_refused():
+    """A grid's threads are counted in 32 bits: sizes past that are refused before the launch."""
+    plan = [P, P, 4, P, 8, P, 16, 16, 32, 8, P, P, P, P, P, P, P, None]
+    for at, v in ((2, (1 << 24) + 1), (2, 0x7fffffff), (9, 0x7ffff800)):
+        refused("wf_kv_page_plan", plan[:at] + [v] + plan[at + 1:], "too many")
+    rope = [P, 512, 128, 4, P, 128, 128, 1, 1, P, 0, P, 2, 128, 128, 0, 1.0, P, 512, 128, P, 128, 128, None]
+    for at, v in ((12, 1 << 24), (12, 0x7fffffff), (3, 65536), (7, 0x7fffffff)):
+        refused("wf_rotary_embed", rope[:at] + [v] + rope[at + 1:], "too many")
+    refused("wf_token_logprobs", [P, 1, 100, 1 << 26, 100, P, 0, 5, P, P, P, P, P, P, None], "too many rows")
+    pre = dict(q=P, dt=1, qsb=512, qsh=128, k=P, v=P, kvq=0, pgs=4096, hs=4096, pages=4, pt=P, pts=8, cols=8, lens=P, rows=P, plens=P,
+               ks=1.0, vs=1.0, sm=0.1, B=2, hq=4, hkv=1, D=128, out=P, osb=512, osh=128, lse=None, ws=P, st=None)
+    for kw in ({"B": 65535, "hq": 65535, "hkv": 65535}, {"B": 65535, "hq": 512, "hkv": 512}, {"B": 65535, "hq": 2048, "hkv": 128}):
+        refused("wf_shared_prefix_attention", list({**pre, **kw}.values()), "too many")

@@ -17,6 +17,9 @@ inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Workgroups of 256 threads in one grid dimension: its threads are counted in 32 bits.
+constexpr int64_t kMaxWgs256 = (1 << 24) - 1;
+
 inline int check_launch(const char* what) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) {

@@ -501,7 +501,7 @@ int wf_token_logprobs(const void* logits, int dtype, int64_t ld, int R, int V, c
     WF_REQUIRE(!tokens || (logprobs && ranks), "token_logprobs: null logprobs / ranks");
     WF_REQUIRE(top_k == 0 || (top_ids && top_logprobs), "token_logprobs: null top_ids / top_logprobs");
     const int S = lp_splits(R, V);
-    WF_REQUIRE((int64_t)R * S <= 0x7fffffff - 4, "token_logprobs: too many rows");
+    WF_REQUIRE((int64_t)R * S <= 4 * kMaxWgs256, "token_logprobs: too many rows (%d)", R);
     const int chunk = (int)((((int64_t)V + S - 1) / S + 31) / 32 * 32);
     LpPart* part = reinterpret_cast<LpPart*>(ws);
     LpArgs a{logits, ld, R, V, S, chunk, tokens, tokens64, top_k, part, reinterpret_cast<double*>(part + (int64_t)R * S), logprobs, entropy, top_logprobs, ranks, top_ids};

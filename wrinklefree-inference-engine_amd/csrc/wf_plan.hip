@@ -269,7 +269,8 @@ int wf_kv_page_plan(const int32_t* cached_lens, const int32_t* new_lens, int B, 
     WF_REQUIRE(B == 0 || (cached_lens && new_lens && (page_table || max_blocks == 0)), "kv_page_plan: null lengths / table");
     WF_REQUIRE(num_free == 0 || free_pages, "kv_page_plan: null free list");
     WF_REQUIRE(num_tokens == 0 || (pages && slots && rows && positions), "kv_page_plan: null token arrays");
-    WF_REQUIRE(num_tokens <= 0x7fffffff - 4096, "kv_page_plan: too many tokens");
+    WF_REQUIRE(B <= 1 << 24, "kv_page_plan: too many sequences (%d)", B);
+    WF_REQUIRE(num_tokens <= 0x7fffffff - 4096, "kv_page_plan: too many tokens (%d)", num_tokens);
     PlanArgs a{cached_lens, new_lens, B, free_pages, num_free, page_table, table_stride, max_blocks, page_size,
                page_size & (page_size - 1) ? -1 : __builtin_ctz(page_size), num_tokens, pages, slots, rows, positions, cu_tokens, counts,
                nullptr, nullptr, aligned16(cached_lens) && aligned16(new_lens)};

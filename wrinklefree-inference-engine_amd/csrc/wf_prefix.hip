@@ -75,7 +75,7 @@ __device__ __forceinline__ PfSeq pf_seq(const PfArgs& a, int b) {
     s.P = owner >= 0 && owner < a.B ? min(max(plen, 0), s.L) : 0;
     return s;
 }
-// Whether b's prefix is read together with a neighbour's (all three launches ask this).
+// Whether b's prefix is read together with a neighbour's (both launches ask this).
 __device__ __forceinline__ bool pf_shared(const PfArgs& a, int b, const PfSeq& s) {
     return s.same(pf_seq(a, b - 1)) || s.same(pf_seq(a, b + 1));
 }
@@ -402,7 +402,7 @@ __device__ void pf_prefix(const PfArgs& a, void* lds, int x, int tile) {
     if (x >= a.Hkv * a.NP) return;
     const int h = x % a.Hkv, z = x / a.Hkv, lane = threadIdx.x & 63;
     const int64_t r0 = (int64_t)tile * MT, r1 = min(r0 + MT, (int64_t)a.B * a.G);
-    const int b0 = (int)(r0 / a.G), b1 = (int)((r1 - 1) / a.G);  // sequences of the tile: at most 64
+    const int b0 = (int)(r0 / a.G), b1 = (int)((r1 - 1) / a.G);  // sequences of the tile: at most MT <= 32
     // lane i: sequence b0 + i
     const int bl = b0 + lane <= b1 ? b0 + lane : -2;
     const PfSeq me = pf_seq(a, bl), before = pf_seq(a, bl - 1), after = pf_seq(a, bl + 1);
@@ -525,7 +525,8 @@ __global__ __launch_bounds__(256) void k_prefix_join(PfArgs a, int odt) {
 }
 
 struct PfPlan {
-    int MT, NP, NS, np, ns;  // rows of a prefix workgroup, splits, workgroups
+    int MT, NP, NS;  // rows of a prefix workgroup, splits
+    int64_t np, ns;  // workgroups
 };
 // Launch shape from what the host knows: rows, kv heads and the table's width (an upper bound of every length).
 static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
@@ -537,16 +538,16 @@ static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
     // prefix ranges: as many workgroups as the device holds at once, two a CU (one where q's further terms take the registers)
     p.NP = clamp((dt == DT_BF16 ? 512 : 256) / (tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
     p.NS = clamp(512 / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);
-    p.np = B > 1 ? (int)(((int64_t)Hkv * p.NP + 7) / 8 * 8 * tiles) : 0;  // one sequence shares nothing
-    p.ns = (int)(p.NS * Hkv * groups * B);
+    p.np = B > 1 ? ((int64_t)Hkv * p.NP + 7) / 8 * 8 * tiles : 0;  // one sequence shares nothing
+    p.ns = p.NS * Hkv * groups * B;
     return p;
 }
 
 template <int KVQ, int QDT>
 static void pf_launch(const PfArgs& a, const PfPlan& p, int odt, hipStream_t st) {
-    const dim3 grid(p.np + p.ns), block(256);
-    if (p.MT == 16) hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 16>), grid, block, 0, st, a, p.np);
-    else hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 32>), grid, block, 0, st, a, p.np);
+    const dim3 grid((unsigned)(p.np + p.ns)), block(256);
+    if (p.MT == 16) hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 16>), grid, block, 0, st, a, (int)p.np);
+    else hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 32>), grid, block, 0, st, a, (int)p.np);
     hipLaunchKernelGGL(k_prefix_join, dim3((unsigned)(((int64_t)a.B * a.Hq + 3) / 4)), block, 0, st, a, odt);
 }
 
@@ -593,6 +594,8 @@ int wf_shared_prefix_attention(const void* q, int dtype, int64_t q_sb, int64_t q
                "shared_prefix_attention: null pointer");
     WF_REQUIRE(aligned16(k_pool) && aligned16(v_pool) && aligned16(ws), "shared_prefix_attention: pools and workspace must be 16-byte aligned");
     const PfPlan p = pf_plan(dtype, B, Hq, Hkv, max_blocks);
+    WF_REQUIRE(p.np + p.ns <= kMaxWgs256 && (int64_t)B * Hq <= 4 * kMaxWgs256, "shared_prefix_attention: batch %d with heads %d / %d too many", B, Hq,
+               Hkv);
     const int64_t recs = (int64_t)B * Hq * (p.NP + p.NS);
     float* o = reinterpret_cast<float*>(ws);
     const int per16 = dtype == WF_F32 ? 4 : 8;

@@ -132,6 +132,7 @@ int wf_rotary_embed(const void* q, int64_t q_st, int64_t q_sh, int Hq, const voi
                     float scale, void* q_out, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh, void* stream) {
     WF_REQUIRE(dtype == WF_F32 || dtype == WF_BF16 || dtype == WF_F16, "rotary_embed: bad dtype %d", dtype);
     WF_REQUIRE(T >= 0 && Hq >= 0 && Hk >= 0, "rotary_embed: negative size (T %d, heads %d / %d)", T, Hq, Hk);
+    WF_REQUIRE(T <= kMaxWgs256 && Hq <= 65535 && Hk <= 65535, "rotary_embed: too many tokens or heads (T %d, heads %d / %d)", T, Hq, Hk);
     WF_REQUIRE(D > 0 && D <= kRopeMaxDim, "rotary_embed: head_dim %d not in [1, %d]", D, kRopeMaxDim);
     WF_REQUIRE(rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= D, "rotary_embed: rotary_dim %d must be even, in [2, %d]",
                rotary_dim, D);
