@@ -186,3 +186,42 @@ def test_launch_sizes_refused():
                ks=1.0, vs=1.0, sm=0.1, B=2, hq=4, hkv=1, D=128, out=P, osb=512, osh=128, lse=None, ws=P, st=None)
     for kw in ({"B": 65535, "hq": 65535, "hkv": 65535}, {"B": 65535, "hq": 512, "hkv": 512}, {"B": 65535, "hq": 2048, "hkv": 128}):
         refused("wf_shared_prefix_attention", list({**pre, **kw}.values()), "too many")
+
+
+def _places(t):
+    return set((t.data_ptr() + t.element_size() * (t.stride(0) * i + t.stride(1) * h + d)) for i in range(t.shape[0]) for h in range(t.shape[1])
+               for d in range(t.shape[2]))
+
+
+def test_apart():
+    """_apart never calls overlapping tensors apart, and knows the arrangements that q and k come in."""
+    from wfamd.ops import _apart
+    x = torch.zeros(4096, dtype=torch.bfloat16)
+    D = 4
+    row = x[:5 * 32].view(5, 8, D)           # heads of one row: q, k, v slices
+    groups = x[:5 * 48].view(5, 3, 4, D)     # kv groups of (q, q, k, v)
+    three = x[:5 * 24].view(5, 6, D)         # q and k heads in turn
+    yes = [(row[:, :4], row[:, 4:6]), (row[:, 4:6], row[:, :4]), (three[:, 0::2], three[:, 1::2]), (row[:1, :3], row[:1, 3:]),
+           (groups[:, :, 0], groups[:, :, 2]), (x[:160].view(5, 8, D), x[160:240].view(5, 4, D)), (row[:2], row[2:4]),
+           (row[:1, :, :2].as_strided((1, 4, D), (0, 8, 1)), row[:1].as_strided((1, 4, D), (0, 8, 1), D))]
+    no = [(row, row), (row[:, :4], row[:, 3:6]), (row[:, :4], row[:, :2]), (row[:2], row[1:3]), (three[:, 0::2], three[:, 2::2]),
+          (row[:, :4], x[130:130 + 5 * 32].view(5, 8, D)[:, :4]), (groups[:, :, 0], groups[:, :, 0])]
+    for a, b in yes:
+        assert not _places(a) & _places(b)
+        assert _apart(a, b) and _apart(b, a), (a.stride(), b.stride())
+    for a, b in no:
+        assert _places(a) & _places(b)
+        assert not _apart(a, b) and not _apart(b, a), (a.stride(), b.stride())
+    g = torch.Generator().manual_seed(0)
+    for _ in range(4000):  # any two views: a 'yes' is one
+        def view():
+            h, t = torch.randint(1, 4, (2,), generator=g).tolist()
+            sh = D + int(torch.randint(0, 10, (1,), generator=g))
+            st = (h - 1) * sh + D + int(torch.randint(0, 40, (1,), generator=g)) if torch.rand((), generator=g) < .5 else sh * (h + 2)
+            return x.as_strided((t, h, D), (st, sh, 1), int(torch.randint(0, 120, (1,), generator=g)))
+        a, b = view(), view()
+        if torch.rand((), generator=g) < .5:
+            b = x.as_strided(b.shape, a.stride(), b.storage_offset())
+        from wfamd.ops import _no_overlap
+        if _no_overlap(a) and _no_overlap(b) and _apart(a, b):
+            assert not _places(a) & _places(b), (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())

@@ -545,12 +545,29 @@ def _no_overlap(t: torch.Tensor) -> bool:
     return True
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """No place of a [T, H, D] is one of b's (same type, dims contiguous, neither overlaps itself): they end before each other, or
+    are slices of one tensor's rows, or of its heads."""
+    (na, ha, D), (at, ah, _), (nb, hb, _), (bt, bh, _) = a.shape, a.stride(), b.shape, b.stride()
+    wa, wb = (ha - 1) * ah + D, (hb - 1) * bh + D  # places a token reaches over
+    d, es = b.data_ptr() - a.data_ptr(), a.element_size()
+    if d >= ((na - 1) * at + wa) * es or -d >= ((nb - 1) * bt + wb) * es:
+        return True
+    if d % es:
+        return False
+    d //= es
+    if at == bt > 0 and wa <= d % at <= at - wb:  # rows at one stride, b behind a in each
+        return True
+    # heads in turn: different places of one head stride, which divides the token strides
+    return ah == bh > 0 and (na == 1 or at % ah == 0) and (nb == 1 or bt % bh == 0) and D <= d % ah <= ah - D
+
+
 def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, *,
                  interleaved: bool = False, scale: float = 1.0, inplace: bool = False):
     """Rotary positions on q [T, Hq, D] and k [T, Hk, D] (or None), bf16 / f16 / f32, any token and head strides
     (include/wf_bitnet.h wf_rotary_embed). positions [T] int32 or int64; freqs, scale from rotary_frequencies: the first
     2 len(freqs) dims of a head are turned, the rest copied. Returns (q, k) turned: new tensors, or with
-    inplace=True the given ones. Each result is rounded once, from 32 bits; the angle is formed in 64."""
+    inplace=True the given ones (slices of one tensor, but sharing no place). Each result is rounded once, from 32 bits; the angle is formed in 64."""
     index = q.get_device()
     if not index == positions.get_device() == freqs.get_device() or index < 0 or (k is not None and k.get_device() != index):
         _one_device("rotary_embed", q=q, k=k, positions=positions, freqs=freqs)
@@ -569,8 +586,8 @@ def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         for what, t in (("q", q), ("k", k)):
             if t is not None and t.numel() and ((t.stride(-1) != 1 and D > 1) or not _no_overlap(t)):
                 raise ValueError(f"rotary_embed: {what} of strides {t.stride()} cannot be turned in place")
-        if k is not None and k.numel() and k.data_ptr() == q.data_ptr():
-            raise ValueError("rotary_embed: q and k are the same memory, turned in place it would be turned twice")
+        if k is not None and k.numel() and q.numel() and not _apart(q, k):
+            raise ValueError("rotary_embed: q and k share memory, turned in place it would be turned twice")
         qo, ko = q, k
     else:
         qo = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
