@@ -535,8 +535,9 @@ static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
     p.MT = rows <= 16 ? 16 : 32;
     const int64_t tiles = (rows + p.MT - 1) / p.MT;
     auto clamp = [](int64_t v, int64_t hi) { return (int)max((int64_t)1, min(min(v, hi), (int64_t)kPfMaxRecords)); };
-    // prefix ranges: as many workgroups as the device holds at once, two a CU (one where q's further terms take the registers)
-    p.NP = clamp((dt == DT_BF16 ? 512 : 256) / (tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
+    // prefix ranges: one workgroup a CU. A second one reads no faster (L1, below), and its place goes to a suffix
+    // workgroup, whose time is HBM's: 32768 shared keys 102 us, 118 with two.
+    p.NP = clamp(256 / (tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
     p.NS = clamp(512 / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);
     p.np = B > 1 ? ((int64_t)Hkv * p.NP + 7) / 8 * 8 * tiles : 0;  // one sequence shares nothing
     p.ns = p.NS * Hkv * groups * B;
