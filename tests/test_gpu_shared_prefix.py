@@ -93,12 +93,14 @@ def check(c, sm_scale=None):
     out, lse = ops.shared_prefix_attention(**c, sm_scale=sm_scale, return_lse=True)
     want, wlse, mean, top, size, keys = reference(**c, sm_scale=sm_scale)
     t = c["q"].dtype
-    terms = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}[t]
+    half = t == torch.float16 and c["kv_dtype"] != "bf16"  # f16 products: q as it is, p rounded once to f16
+    terms = {torch.bfloat16: 1, torch.float16: 2 - half, torch.float32: 3}[t]
     u = 2.0 ** -24
     # a score: 128 products and sums for each term of q, the scale's 3 roundings, the exponent's and exp2's (64 + 4)
     ds = u * ((128 * terms + 8) * size + 3 * top + 68)
-    # p: 2^-8 for each of its terms, twice the score's error; l and o: a sum over the keys, 24 more of the joins
-    rel = 2.0 ** -(8 * terms) + 2 * ds + u * (keys + 24)
+    # p: 2^-8 for each of its bf16 terms, 2^-11 for one of f16 (and 2^-32 of the row's largest where it is below 2^-21 of
+    # it, less than its share of the sum's u); twice the score's error; l and o: a sum over the keys, 24 more of the joins
+    rel = (2.0 ** -11 if half else 2.0 ** -(8 * terms)) + 2 * ds + u * (keys + 24)
     tol = mean * rel[..., None] + torch.finfo(t).eps / 2 * want.abs() + (2.0 ** -25 if t == torch.float16 else 1e-37)
     assert out.dtype == t and torch.isfinite(out).all()
     assert ((out.double().cpu() - want).abs() / tol).max().item() <= 1.0
@@ -203,6 +205,36 @@ def test_extreme_scores():
     c["q"].fill_(math.nan)
     out, lse = ops.shared_prefix_attention(**c, return_lse=True)
     assert out.isnan().all() and lse.isnan().all()
+
+
+@pytest.mark.parametrize("kv", ["fp8", "int8"])
+def test_f16_over_one_byte_pools(kv):
+    """f16 products: flat and steep rows, a rising score, every code, what is masked."""
+    from wfamd import ops
+    shape = (6, 1, 4, [150, 150, 97, 150, 0, 101], [0] * 6, [100] * 6, kv, "f16")
+    for size in (0.0, 1.0, 30.0, 300.0):
+        check(case(*shape, seed=20, size=size))
+    check(case(*shape, seed=21), sm_scale=-0.3)
+    # scores that rise by a little with every tile: the frame is raised time and again, or (0.02) not at all
+    for step in (0.02, 1.5):
+        c = case(40, 1, 2, [640] * 40, [0] * 40, [600] * 40, kv, "f16", seed=22)
+        c["q"].zero_()
+        c["q"][..., 0] = step / c["k_scale"] * D ** 0.5
+        for j in range(20):
+            level = torch.tensor([float(j)], device="cuda")
+            code = level.to(torch.float8_e4m3fn).view(torch.uint8).item() if kv == "fp8" else j
+            for b in (range(40) if j > 17 else (0,)):
+                c["k_pool"][int(c["page_table"][b, j])] = code
+        check(c)
+    # a sequence of one key gives its values: all codes that are numbers
+    codes = torch.arange(256, device="cuda").to(torch.uint8)
+    if kv == "fp8":
+        codes = torch.where(codes & 0x7f == 0x7f, 0, codes).to(torch.uint8)
+    c = case(2, 1, 1, [1, 1], [-1, -1], [0, 0], kv, "f16", seed=23)
+    for i in range(2):
+        c["v_pool"][int(c["page_table"][i, 0])][0, V_AT[0].cuda()] = codes[128 * i:128 * i + 128]
+    c["v_scale"] = 1.0
+    assert torch.equal(ops.shared_prefix_attention(**c).reshape(-1), widen(codes, kv).half())
 
 
 def test_strides_layers_and_offsets_past_32_bits():

@@ -1,4 +1,4 @@
-// wf_kv.h -- one-byte K/V codes (OCP e4m3fn, int8) to bf16 in registers, for the attention kernels.
+// wf_kv.h -- one-byte K/V codes (OCP e4m3fn, int8) to bf16 or f16 in registers, for the attention kernels.
 #pragma once
 #include "wf_device.h"
 
@@ -55,6 +55,26 @@ __device__ __forceinline__ uint32_t i8x2_to_bf16_sext(uint32_t u, int sh) {
 }
 __device__ __forceinline__ uint4 i8x8_to_bf16_sext(uint2 r) {
     return make_uint4(i8x2_to_bf16_sext(r.x, 0), i8x2_to_bf16_sext(r.x, 16), i8x2_to_bf16_sext(r.y, 0), i8x2_to_bf16_sext(r.y, 16));
+}
+
+// The same codes as f16 (exact too). int8: the byte, biased to unsigned, is the mantissa of 1024 + code + 128, a subtraction
+// away from the code: 10 instructions for 8 codes.
+typedef _Float16 v2h_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t i8x2_to_f16(uint32_t biased, uint32_t sel) {
+    const v2h_t h = __builtin_bit_cast(v2h_t, __builtin_amdgcn_perm(0x64646464u, biased, sel));
+    return __builtin_bit_cast(uint32_t, h - v2h_t{(_Float16)1152.f, (_Float16)1152.f});
+}
+__device__ __forceinline__ uint4 i8x8_to_f16(uint2 r) {
+    const uint32_t x = r.x ^ 0x80808080u, y = r.y ^ 0x80808080u;
+    return make_uint4(i8x2_to_f16(x, 0x04010400u), i8x2_to_f16(x, 0x04030402u), i8x2_to_f16(y, 0x04010400u), i8x2_to_f16(y, 0x04030402u));
+}
+__device__ __forceinline__ uint4 fp8x8_to_f16(uint2 r) {
+    const v2h_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(r.x, 1.0f, false);
+    const v2h_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(r.x, 1.0f, true);
+    const v2h_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(r.y, 1.0f, false);
+    const v2h_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(r.y, 1.0f, true);
+    return make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
+                      __builtin_bit_cast(uint32_t, d));
 }
 
 }  // namespace wf

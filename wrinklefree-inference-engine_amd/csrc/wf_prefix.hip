@@ -20,16 +20,17 @@
 // The running max is raised only when a tile passes it by 2^8 (its exchange between the four lanes of a row and
 // the rescaling of o are rare then): p <= 2^8 is as exact in bf16 and 32 bits as p <= 1.
 //
-// Rounding: scores, max, sums and o in 32 bits. A q of f16 / f32 enters as the exact sum of two / three bf16 terms.
-// P is rounded to bf16 for bf16 outputs (2^-9 a term, as much as the output's own rounding); f16 and f32 outputs take
-// two and three terms of it.
+// Operands and rounding: scores, max, sums and o in 32 bits. The matrices are bf16, and f16 where q is f16 and the pool holds
+// one-byte codes (all of them f16 values). Where the pool is bf16, an f16 q enters as the exact sum of two bf16 terms;
+// an f32 q as three. P is rounded once to the output's type where that is the matrices' (bf16 2^-8, f16 2^-11 a
+// term at most, as much as the output's own rounding; f16 with the exponents 7 higher, so that only p < 2^-21 lose bits,
+// 2^-32 at most); else it has as many terms as q.
 #include "wf_common.h"
 #include "wf_device.h"
 #include "wf_kv.h"
 
 namespace wf {
 
-typedef __bf16 pf_bf8 __attribute__((ext_vector_type(8)));
 typedef float pf_f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPfDim = 128, kPfPage = 32;
@@ -83,32 +84,43 @@ __device__ __forceinline__ bool pf_shared(const PfArgs& a, int b, const PfSeq& s
 __device__ __forceinline__ int pf_per(int tiles, int splits, int least) { return max((tiles + splits - 1) / splits, least); }
 __device__ __forceinline__ int pf_tiles(int keys) { return (keys + kPfPage - 1) / kPfPage; }
 
-// 8 elements of a tile's fragment as bf16
-template <int KVQ>
-struct PfFrag {
+// The matrices' elements for a pool and q, and how many of them make up a q (and a p)
+template <int KVQ, int QDT>
+struct PfType {
+    static constexpr bool kHalf = QDT == DT_F16 && KVQ != 0;
+    static constexpr int kTerms = QDT == DT_BF16 || kHalf ? 1 : QDT == DT_F16 ? 2 : 3;
+    using E = typename std::conditional<kHalf, _Float16, __bf16>::type;
+    typedef E V8 __attribute__((ext_vector_type(8)));
+    // 8 elements of a tile's fragment
     static constexpr int kBytes = KVQ == 0 ? 2 : 1;
     using T = typename std::conditional<KVQ == 0, uint4, uint2>::type;
-    static __device__ __forceinline__ uint4 bf(T t) {
+    static __device__ __forceinline__ uint4 wide(T t) {
         if constexpr (KVQ == 0) return t;
-        else if constexpr (KVQ == 1) return fp8x8_to_bf16(t);
-        else return i8x8_to_bf16_sext(t);
+        else if constexpr (KVQ == 1) return kHalf ? fp8x8_to_f16(t) : fp8x8_to_bf16(t);
+        else return kHalf ? i8x8_to_f16(t) : i8x8_to_bf16_sext(t);
     }
 };
 
-// NT column tiles of W query rows: the q fragments, running max, sum and output of one wave. A K or V tile is 8 fragments
+// W query rows: the q fragments, running max, sum and output of one wave. A K or V tile is 8 fragments
 // of 8 elements a lane, and either way the accumulator of S^T leaves a lane with the keys that it needs in P^T:
-//   W = 16 (v_mfma_f32_16x16x32_bf16): lane (l = row, g = quarter); scores of keys 8 g + e, e = 0..7;
-//   W = 32 (v_mfma_f32_32x32x16_bf16, 1.7 times the rate: 32 cycles to 2 x 27 measured): lane (l = row, g = half); scores of
+//   W = 16 (16x16x32 products): lane (l = row, g = quarter); scores of keys 8 g + e, e = 0..7;
+//   W = 32 (32x32x16, 1.7 times the rate: 32 cycles to 2 x 27 measured): lane (l = row, g = half); scores of
 //          keys 16 j + 8 g + e, j = 0, 1 -- K's 32 rows are the two 16-row halves of the tile one after the other.
-template <int W, int NT, int NQ, int NPT>
+template <int W, int KVQ, int QDT>
 struct PfState {
+    using Type = PfType<KVQ, QDT>;
+    using E = typename Type::E;
+    using V8 = typename Type::V8;
+    using T = typename Type::T;
+    static constexpr int N = Type::kTerms;
     static constexpr int J = W / 16;            // groups of 8 keys a lane
-    static constexpr int M = kPfDim / W;        // accumulators of a column tile
+    static constexpr int M = kPfDim / W;        // accumulators
     static constexpr int S = W == 16 ? 4 : 8;   // dim steps of a score
+    static constexpr float kUp = Type::kHalf ? 7.f : 0.f;  // the exponents' frame lies this much below the max: p < 2^(8 + 7), and normal in f16 from 2^-21 on
     typedef float Acc __attribute__((ext_vector_type(W == 16 ? 4 : 16)));
-    pf_bf8 q[NT][NQ][S];
-    Acc acc[NT][M];
-    float m[NT], f[NT], l[NT];  // max (log2 domain), the frame of the exponents (m, or 0 while it is -inf), sum
+    V8 q[N][S];
+    Acc acc[M];
+    float m, f, l;  // max (log2 domain), the frame of the exponents (m - kUp, or 0 while it is -inf), sum
 
     static __device__ __forceinline__ int row() { return threadIdx.x & (W - 1); }
     static __device__ __forceinline__ int group() { return (threadIdx.x & 63) / W; }
@@ -121,22 +133,20 @@ struct PfState {
         if constexpr (W == 16) return i * 512 + (threadIdx.x & 63) * 8;
         else return (i >> 1) * 1024 + (row() >> 4) * 512 + (i & 1) * 256 + group() * 128 + (row() & 15) * 8;  // i = 2 m + j
     }
-    static __device__ __forceinline__ Acc mfma(pf_bf8 x, pf_bf8 y, Acc c) {
-        if constexpr (W == 16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+    static __device__ __forceinline__ Acc mfma(V8 x, V8 y, Acc c) {
+        if constexpr (W == 16 && Type::kHalf) return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+        else if constexpr (W == 16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+        else if constexpr (Type::kHalf) return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
         else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
     }
 
     __device__ __forceinline__ void clear() {
+        m = -INFINITY, f = 0.f, l = 0.f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            m[t] = -INFINITY, f[t] = 0.f, l[t] = 0.f;
-#pragma unroll
-            for (int n = 0; n < M; ++n) acc[t][n] = Acc{};
-        }
+        for (int n = 0; n < M; ++n) acc[n] = Acc{};
     }
-    // tile t's row; fragment c: its dims 8 (64 / W c + g) ..; vec: the row is 16-byte aligned
-    template <int QDT>
-    __device__ __forceinline__ void load_q(int t, const uint8_t* row, float neg, bool vec) {
+    // this lane's row; fragment c: its dims 8 (64 / W c + g) ..; vec: the row is 16-byte aligned
+    __device__ __forceinline__ void load_q(const uint8_t* row, float neg, bool vec) {
         constexpr int G = 64 / W, V = QDT == DT_F32 ? 2 : 1;
 #pragma unroll
         for (int c = 0; c < S; ++c) {
@@ -160,92 +170,76 @@ struct PfState {
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] *= neg;
 #pragma unroll
-            for (int k = 0; k < NQ; ++k) {
-                pf_bf8 v;
+            for (int k = 0; k < N; ++k)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[e] = (__bf16)x[e];
-                    x[e] -= (float)v[e];
+                    q[k][c][e] = (E)x[e];
+                    if (k + 1 < N) x[e] -= (float)q[k][c][e];
                 }
-                q[t][k][c] = v;
-            }
         }
     }
-    using Scores = float[NT][8 * J];
-    using Probs = pf_bf8[NT][NPT][J];
-    // scores of a 32-key tile: s[t][8 j + e] for key 8 (64 / W j + g) + e
-    template <int KVQ>
-    __device__ __forceinline__ void scores(const typename PfFrag<KVQ>::T (&kf)[8], Scores& s) {
-        Acc c[NT][W == 16 ? 2 : 1];
+    using Scores = float[8 * J];
+    using Probs = V8[N][J];
+    // scores of a 32-key tile: s[8 j + e] for key 8 (64 / W j + g) + e
+    __device__ __forceinline__ void scores(const T (&kf)[8], Scores& s) {
+        Acc c[W == 16 ? 2 : 1];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int h = 0; h < (W == 16 ? 2 : 1); ++h) c[t][h] = Acc{};
+        for (int h = 0; h < (W == 16 ? 2 : 1); ++h) c[h] = Acc{};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int step = W == 16 ? i >> 1 : i, h = W == 16 ? i & 1 : 0;
-            const pf_bf8 kb = __builtin_bit_cast(pf_bf8, PfFrag<KVQ>::bf(kf[W == 16 ? 4 * h + step : i]));
+            const V8 kb = __builtin_bit_cast(V8, Type::wide(kf[W == 16 ? 4 * h + step : i]));
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int k = NQ - 1; k >= 0; --k) c[t][h] = mfma(kb, q[t][k][step], c[t][h]);
+            for (int k = N - 1; k >= 0; --k) c[h] = mfma(kb, q[k][step], c[h]);
         }
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 8 * J; ++e)
-                s[t][e] = W == 16 ? c[t][(e >> 2) & (W == 16)][e & 3] : c[t][0][(8 * ((e >> 2) & 1) + 4 * (e >> 3) + (e & 3)) & (W / 2 - 1)];
+        for (int e = 0; e < 8 * J; ++e)
+            s[e] = W == 16 ? c[(e >> 2) & (W == 16)][e & 3] : c[0][(8 * ((e >> 2) & 1) + 4 * (e >> 3) + (e & 3)) & (W / 2 - 1)];
     }
     static __device__ __forceinline__ int key(int j) { return 8 * (64 / W * j + group()); }
     // scores -> probabilities in the rows' frames; keys outside [lo, hi) of the tile are masked
-    __device__ __forceinline__ void softmax(Scores& s, pf_bf8 (&p)[NT][NPT][J], int lo, int hi, float sc) {
-        const bool whole = lo <= 0 && hi >= kPfPage;
+    __device__ __forceinline__ void softmax(Scores& x, Probs& p, int lo, int hi, float sc) {
+        if (!(lo <= 0 && hi >= kPfPage)) {
+            asm volatile("");  // a branch, not selects on every tile
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float (&x)[8 * J] = s[t];
-            if (!whole) {
-                asm volatile("");  // a branch, not selects on every tile
-#pragma unroll
-                for (int e = 0; e < 8 * J; ++e) x[e] = key(e >> 3) + (e & 7) >= lo && key(e >> 3) + (e & 7) < hi ? x[e] : -INFINITY;
-            }
-            float mx = x[0];
-#pragma unroll
-            for (int e = 1; e < 8 * J; ++e) mx = fmaxf(mx, x[e]);
-            mx *= sc;
-            if (__any(mx > m[t] + 8.f)) {
-                if constexpr (W == 16) mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m[t]);
-                const float nf = mx == -INFINITY ? 0.f : mx;
-                // (an empty sum stays, also when it is NaN: it holds no finite score to rescale)
-                const float r = m[t] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(f[t] - nf);
-                l[t] *= r;
-#pragma unroll
-                for (int n = 0; n < M; ++n) acc[t][n] *= r;
-                m[t] = mx;
-                f[t] = nf;
-            }
-#pragma unroll
-            for (int e = 0; e < 8 * J; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], sc, -f[t]));
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const float* y = x + 8 * j;
-                l[t] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
-            }
-#pragma unroll
-            for (int k = 0; k < NPT; ++k)
-#pragma unroll
-                for (int e = 0; e < 8 * J; ++e) {
-                    p[t][k][e >> 3][e & 7] = (__bf16)x[e];
-                    if (k + 1 < NPT) x[e] -= (float)p[t][k][e >> 3][e & 7];
-                }
+            for (int e = 0; e < 8 * J; ++e) x[e] = key(e >> 3) + (e & 7) >= lo && key(e >> 3) + (e & 7) < hi ? x[e] : -INFINITY;
         }
+        float mx = x[0];
+#pragma unroll
+        for (int e = 1; e < 8 * J; ++e) mx = fmaxf(mx, x[e]);
+        mx *= sc;
+        if (__any(mx > m + 8.f)) {
+            if constexpr (W == 16) mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m);
+            const float nf = mx == -INFINITY ? 0.f : mx - kUp;
+            // (an empty sum stays, also when it is NaN: it holds no finite score to rescale)
+            const float r = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(f - nf);
+            l *= r;
+#pragma unroll
+            for (int n = 0; n < M; ++n) acc[n] *= r;
+            m = mx;
+            f = nf;
+        }
+#pragma unroll
+        for (int e = 0; e < 8 * J; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], sc, -f));
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const float* y = x + 8 * j;
+            l += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int e = 0; e < 8 * J; ++e) {
+                p[k][e >> 3][e & 7] = (E)x[e];
+                if (k + 1 < N) x[e] -= (float)p[k][e >> 3][e & 7];
+            }
     }
     // o += P V
-    template <int KVQ>
-    __device__ __forceinline__ void values(const typename PfFrag<KVQ>::T (&vf)[8], const pf_bf8 (&p)[NT][NPT][J], int lo, int hi) {
+    __device__ __forceinline__ void values(const T (&vf)[8], const Probs& p, int lo, int hi) {
         uint4 v[8];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) v[n] = PfFrag<KVQ>::bf(vf[n]);
+        for (int n = 0; n < 8; ++n) v[n] = Type::wide(vf[n]);
         if (!(lo <= 0 && hi >= kPfPage)) {  // a masked key's V may hold anything: 0 x NaN is NaN
             asm volatile("");
 #pragma unroll
@@ -262,11 +256,9 @@ struct PfState {
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
-            const pf_bf8 vb = __builtin_bit_cast(pf_bf8, v[n]);
+            const V8 vb = __builtin_bit_cast(V8, v[n]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int k = NPT - 1; k >= 0; --k) acc[t][n / J] = mfma(vb, p[t][k][n % J], acc[t][n / J]);
+            for (int k = N - 1; k >= 0; --k) acc[n / J] = mfma(vb, p[k][n % J], acc[n / J]);
         }
     }
 };
@@ -275,9 +267,9 @@ struct PfState {
 // range(k, lo, hi) its valid keys. 64 page ids are fetched at a time, a lane each. The next tile's K is under way from
 // the moment this one's scores are done, its V from the moment this one's products are: one set of registers,
 // and half a tile's work over each load's latency.
-template <int KVQ, class State, class Page, class Range>
+template <class State, class Page, class Range>
 __device__ __forceinline__ void pf_walk(const PfArgs& a, State& st, int64_t head, int k0, int k1, Page page, Range range) {
-    using T = typename PfFrag<KVQ>::T;
+    using T = typename State::T;
     const int lane = threadIdx.x & 63, n = (k1 - k0 + 3) / 4;
     if (n <= 0) return;
     T kf[8], vf[8];
@@ -294,7 +286,7 @@ __device__ __forceinline__ void pf_walk(const PfArgs& a, State& st, int64_t head
     auto load = [&](int id, const uint8_t* pool, T (&f)[8], bool v) {
         const uint8_t* p = pool + max(id, 0) * a.pgs + head;  // no such page: page 0, masked
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = *reinterpret_cast<const T*>(p + (v ? State::v_at(e) : State::k_at(e)) * PfFrag<KVQ>::kBytes);
+        for (int e = 0; e < 8; ++e) f[e] = *reinterpret_cast<const T*>(p + (v ? State::v_at(e) : State::k_at(e)) * State::Type::kBytes);
     };
     int id = find(0);
     load(id, a.K, kf, false);
@@ -307,28 +299,28 @@ __device__ __forceinline__ void pf_walk(const PfArgs& a, State& st, int64_t head
         id = i + 1 < n ? find(i + 1) : -1;
         typename State::Scores s;
         typename State::Probs p;
-        st.template scores<KVQ>(kf, s);
+        st.scores(kf, s);
         load(id, a.K, kf, false);
         st.softmax(s, p, lo, hi, a.sc);
-        st.template values<KVQ>(vf, p, lo, hi);
+        st.values(vf, p, lo, hi);
         load(id, a.V, vf, true);
     }
 }
 
-// The four waves' states of one column tile -> one record a row.
+// The four waves' states -> one record a row.
 constexpr int kPfRow = kPfDim + 4;
 template <int W>
 struct __attribute__((aligned(16))) PfShared {
     float o[4][W][kPfRow];
     float m[4][W], l[4][W];
 };
-// row(i): the record's place in ml / o for row i of the column tile, or < 0
+// row(i): the record's place in ml / o for row i of the wave's, or < 0; m: the frame of l and o, -inf where no score was finite
 template <int W, class Acc, int M, class Row>
 __device__ __forceinline__ void pf_merge(const PfArgs& a, PfShared<W>& sm, const Acc (&acc)[M], float m, float l, Row row) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & (W - 1), g = lane / W;
     if constexpr (W == 16) l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    __syncthreads();  // the last column tile's record has been read
+    __syncthreads();  // the last run's records have been read
     // accumulator n, registers 4 i ..: dims W n + 8 i + 4 g .. (W = 16: i = 0)
 #pragma unroll
     for (int n = 0; n < M; ++n)
@@ -368,33 +360,21 @@ __device__ __forceinline__ void pf_merge(const PfArgs& a, PfShared<W>& sm, const
 // are 8 k workgroups apart, so one XCD's L2 serves them all. A tile's rows are taken in runs of sequences with one
 // prefix, in 16 or 32 rows.
 // ---------------------------------------------------------------------------------------------
-template <int QDT>
-constexpr int kPfTerms = QDT == DT_BF16 ? 1 : QDT == DT_F16 ? 2 : 3;
-
-template <int KVQ, int QDT, int W, int NT>
+template <int KVQ, int QDT, int W>
 __device__ __forceinline__ void pf_run(const PfArgs& a, void* lds, int h, int z, int64_t ra, int64_t rb, int P, int owner, int k0, int k1) {
-    constexpr int NQ = kPfTerms<QDT>;
-    using State = PfState<W, NT, NQ, NQ>;
-    State st;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int64_t r = min(ra + W * t + State::row(), rb - 1);
-        const int b = (int)(r / a.G), g = (int)(r - (int64_t)b * a.G);
-        const int64_t off = (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2);
-        st.template load_q<QDT>(t, (const uint8_t*)a.q + off, a.neg, a.qvec);
-    }
+    PfState<W, KVQ, QDT> st;
+    const int64_t r = min(ra + st.row(), rb - 1);
+    const int b = (int)(r / a.G), g = (int)(r - (int64_t)b * a.G);
+    st.load_q((const uint8_t*)a.q + (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2), a.neg, a.qvec);
     st.clear();
     const int32_t* row = a.pt + owner * a.pts;
-    pf_walk<KVQ>(a, st, h * a.hs, k0 + (int)(threadIdx.x >> 6), k1, [&](int k) { return row[k]; },
-                 [&](int k, int& lo, int& hi) { lo = 0, hi = P - k * kPfPage; });
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-        pf_merge(a, *static_cast<PfShared<W>*>(lds), st.acc[t], st.m[t], st.l[t], [&](int i) -> int64_t {
-            const int64_t r = ra + W * t + i;
-            if (r >= rb) return -1;
-            const int64_t b = r / a.G;
-            return (b * a.Hq + h * a.G + (r - b * a.G)) * (a.NP + a.NS) + z;
-        });
+    pf_walk(a, st, h * a.hs, k0 + (int)(threadIdx.x >> 6), k1, [&](int k) { return row[k]; },
+            [&](int k, int& lo, int& hi) { lo = 0, hi = P - k * kPfPage; });
+    pf_merge(a, *static_cast<PfShared<W>*>(lds), st.acc, st.m - st.kUp, st.l, [&](int i) -> int64_t {
+        if (ra + i >= rb) return -1;
+        const int64_t b = (ra + i) / a.G;
+        return (b * a.Hq + h * a.G + (ra + i - b * a.G)) * (a.NP + a.NS) + z;
+    });
 }
 
 template <int KVQ, int QDT, int MT>
@@ -421,10 +401,10 @@ __device__ void pf_prefix(const PfArgs& a, void* lds, int x, int tile) {
         const int64_t ra = max(r0, (int64_t)(b0 + i) * a.G), rb = min(r1, (int64_t)(b0 + j) * a.G);  // its rows
         if constexpr (MT > 16)
             if (rb - ra > 16) {
-                pf_run<KVQ, QDT, 32, 1>(a, lds, h, z, ra, rb, P, owner, k0, k1);
+                pf_run<KVQ, QDT, 32>(a, lds, h, z, ra, rb, P, owner, k0, k1);
                 continue;
             }
-        pf_run<KVQ, QDT, 16, 1>(a, lds, h, z, ra, rb, P, owner, k0, k1);
+        pf_run<KVQ, QDT, 16>(a, lds, h, z, ra, rb, P, owner, k0, k1);
     }
 }
 
@@ -433,7 +413,6 @@ __device__ void pf_prefix(const PfArgs& a, void* lds, int x, int tile) {
 // ---------------------------------------------------------------------------------------------
 template <int KVQ, int QDT>
 __device__ void pf_suffix(const PfArgs& a, void* lds, int z, int hc, int b) {
-    constexpr int NQ = kPfTerms<QDT>;
     const int ct = hc / a.Hkv, h = hc - ct * a.Hkv;
     const PfSeq s = pf_seq(a, b);
     // tiles [0, n1) the owner's, below P; then its own from the tile that holds P on
@@ -441,22 +420,18 @@ __device__ void pf_suffix(const PfArgs& a, void* lds, int z, int hc, int b) {
     const int tiles = s.L > s.P ? n1 + pf_tiles(s.L) - first : n1;
     const int per = pf_per(tiles, a.NS, kPfMinSuffix), k0 = z * per, k1 = min(k0 + per, tiles);
     if (k0 >= k1) return;
-    using State = PfState<16, 1, NQ, NQ>;
-    State st;
-    {
-        const int g = min(ct * 16 + State::row(), a.G - 1);
-        const int64_t off = (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2);
-        st.template load_q<QDT>(0, (const uint8_t*)a.q + off, a.neg, a.qvec);
-    }
+    PfState<16, KVQ, QDT> st;
+    const int g = min(ct * 16 + st.row(), a.G - 1);
+    st.load_q((const uint8_t*)a.q + (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2), a.neg, a.qvec);
     st.clear();
-    pf_walk<KVQ>(a, st, h * a.hs, k0 + (int)(threadIdx.x >> 6), k1,
-                 [&](int k) { return a.pt[(k < n1 ? s.owner : b) * a.pts + (k < n1 ? k : first + k - n1)]; },
-                 [&](int k, int& lo, int& hi) {
-                     const int at = (k < n1 ? k : first + k - n1) * kPfPage;
-                     lo = k < n1 ? 0 : s.P - at;
-                     hi = (k < n1 ? s.P : s.L) - at;
-                 });
-    pf_merge(a, *static_cast<PfShared<16>*>(lds), st.acc[0], st.m[0], st.l[0], [&](int i16) -> int64_t {
+    pf_walk(a, st, h * a.hs, k0 + (int)(threadIdx.x >> 6), k1,
+            [&](int k) { return a.pt[(k < n1 ? s.owner : b) * a.pts + (k < n1 ? k : first + k - n1)]; },
+            [&](int k, int& lo, int& hi) {
+                const int at = (k < n1 ? k : first + k - n1) * kPfPage;
+                lo = k < n1 ? 0 : s.P - at;
+                hi = (k < n1 ? s.P : s.L) - at;
+            });
+    pf_merge(a, *static_cast<PfShared<16>*>(lds), st.acc, st.m - st.kUp, st.l, [&](int i16) -> int64_t {
         const int g = ct * 16 + i16;
         return g < a.G ? ((int64_t)b * a.Hq + h * a.G + g) * (a.NP + a.NS) + a.NP + z : -1;
     });
@@ -465,7 +440,9 @@ __device__ void pf_suffix(const PfArgs& a, void* lds, int z, int hc, int b) {
 // The first np workgroups the prefixes, in row tiles of MT; the others the other keys: the one part waits for the
 // matrix cores and L1, the other for HBM.
 template <int KVQ, int QDT, int MT>
-__global__ __launch_bounds__(256, MT == 32 && QDT != DT_BF16 ? 1 : 2) void k_shared_prefix(PfArgs a, int np) {
+constexpr int kPfWgs = MT == 32 && PfType<KVQ, QDT>::kTerms > 1 ? 1 : 2;  // a CU: a q of several terms takes the registers
+template <int KVQ, int QDT, int MT>
+__global__ __launch_bounds__(256, (kPfWgs<KVQ, QDT, MT>)) void k_shared_prefix(PfArgs a, int np) {
     __shared__ PfShared<MT> sm;
     int x = blockIdx.x;
     if (x < np) {
