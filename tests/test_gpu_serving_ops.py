@@ -349,6 +349,36 @@ def test_logprobs_awkward_rows(kind, dtype):
     check_logprobs(x[:, 1:], [0, 776, V - 2, 4, 1, 2], 64)  # rows that begin off any 16-byte line
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,vocab,k", [(600, 32000, 20), (600, 32000, 33), (90, 20000, 32), (3, 20000, 32)])
+def test_logprobs_long_and_short_chunks(rows, vocab, k, dtype):
+    """Chunks that stay in registers and chunks that do not; the greatest logits spread out, and all in a few lanes."""
+    g = torch.Generator("cuda").manual_seed(3)
+    x = torch.randn(rows, vocab, generator=g, device="cuda")
+    x[1::2] += 8.0 * (torch.arange(vocab, device="cuda") // 8 % 64 < 19)
+    x[2::4] += 8.0 * (torch.arange(vocab, device="cuda") // 4 % 64 == 5)
+    check_logprobs(x.to(DT[dtype]), torch.randint(0, vocab, (rows,), generator=g, device="cuda").tolist(), k)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_logprobs_alternatives_among_nan_of_both_signs(dtype):
+    from wfamd import ops
+    g = torch.Generator("cuda").manual_seed(4)
+    for vocab in (50, 700, 20000):
+        x = torch.randn(5, vocab, generator=g, device="cuda").to(DT[dtype])
+        bits = x.view(torch.int32 if dtype == "f32" else torch.int16)
+        bad = torch.rand(5, vocab, generator=g, device="cuda") < 0.5
+        neg = torch.rand(5, vocab, generator=g, device="cuda") < 0.5
+        nan = torch.full((), math.nan, dtype=DT[dtype], device="cuda").view(bits.dtype)
+        bits[bad] = nan & (2 ** (31 if dtype == "f32" else 15) - 1)
+        bits[bad & neg] |= -2 ** (31 if dtype == "f32" else 15)
+        assert (x.isnan() == bad).all()
+        p = ops.token_logprobs(x, top_k=20)
+        want = torch.sort(x.float().nan_to_num(-math.inf), dim=1, descending=True, stable=True).indices[:, :20]
+        want[torch.arange(20, device="cuda") >= (~bad).sum(1, keepdim=True)] = -1  # fewer than 20 numbers in the row
+        assert torch.equal(p.top_ids.long(), want) and p.top_logprobs.isnan().all() and p.entropy.isnan().all()
+
+
 def test_logprobs_nan_and_infinity():
     from wfamd import ops
     x = torch.randn(4, 5000, device="cuda")

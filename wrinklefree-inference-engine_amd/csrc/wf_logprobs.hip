@@ -3,18 +3,21 @@
 // Row x of V logits, m = max x, Z = sum exp(x - m):
 //     log p_t = x_t - m - log Z,     H = log Z - sum (x - m) exp(x - m) / Z,
 //     rank of t = 1 + #{j : x_j > x_t} + #{j < t : x_j = x_t},  top k by value, the lower index first.
-// Each logit has to be read once (2 bytes bf16), some 10 VALU cycles a logit and SIMD: bound by memory for
-// many rows, by latency for few. One wave takes a chunk of one row and never meets another wave: no LDS,
-// no barrier, no atomics, so results do not depend on timing. Per lane it keeps a running max and sums in
+// Each logit has to be read once (2 bytes bf16), some 14 VALU cycles a logit and SIMD: bound by memory for
+// many rows, by latency for few. One wave takes a chunk of one row and never meets another wave: no
+// barrier, no atomics, so results do not depend on timing. Per lane it keeps a running max and sums in
 // the log2 domain, y = (x - max) log2e, e = 2^y, sum e and sum y e, rescaled when the lane's max rises.
-//
-// The top k without a data-dependent buffer: the chunk is cut into groups of four neighbouring 16-byte
-// vectors (the four lanes of a quad); each group's max comes from the softmax's own max and two DPP steps.
-// The k first groups, by (max, lower group first), hold the chunk's k first elements: an element of a
-// later group is preceded by the maxima of k groups, each greater, or equal and further left. The wave
-// keeps the k best groups sorted across its lanes (insertion: ballot, popcount, one lane shift), and reads
-// just those k groups again at the end for the elements themselves. k <= 64 is the wave's width.
 // A second launch, a wave per row, joins the chunks' sums and sorted lists.
+//
+// The top k without a data-dependent buffer, from maxima that the sums need anyway:
+//   short chunks (two tiles, few rows) stay in registers. The k-th greatest of the 64 lanes' maxima bounds the k-th
+//     logit from below; what reaches it (some 64 ln(64 / (64 - k)) logits) is packed by ballots and ordered once.
+//   long chunks are cut into groups of four neighbouring 16-byte vectors (the four lanes of a quad), each group's max two
+//     DPP steps more. The k first groups, by (max, lower group first), hold the chunk's k first elements: an
+//     element of a later group is preceded by the maxima of k groups, each greater, or equal and further left. The
+//     wave keeps the k best groups sorted across its lanes and reads just those again at the end. k <= 64 is the wave's width.
+// Measured, vocabulary 128256 in bf16: 2048 rows with 5 alternatives 119 us, 4.4 TB/s (97 us, 5.4 TB/s, without any); 128 rows
+// with 20: 17.5 us and 5 of the join (the reading and summing alone 11.7); one row 7 + 4 us, latencies.
 #include "wf_common.h"
 #include "wf_device.h"
 
@@ -22,6 +25,7 @@ namespace wf {
 
 constexpr int kLpMaxTop = 64;
 constexpr int kLpUnroll = 4;        // 16-byte vectors a lane holds of a tile
+constexpr int kLpHeld = 2;          // tiles of a chunk that stay in registers
 constexpr int kLpMaxSplits = 64;    // chunks of a row: a lane each in the join
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
@@ -125,16 +129,52 @@ struct LpQueue {
         const int lane = threadIdx.x & 63;
         const double c = lane < n ? q[lane] : 0.;
         meet();
+        if (!(l.last(1) > 0.)) {  // into an empty list: a key's place is the number of greater ones
+            int at = 0;
+            if (lane >= n) q[lane] = 0.;
+            meet();
+#pragma unroll 1
+            for (int i = 0; i < n; i += 8)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) at += q[i + e] > c;
+            meet();
+            if (lane < n) q[at] = c;
+            meet();
+            l.v = lane < n ? q[lane] : 0.;
+            meet();
+            n = 0;
+            return;
+        }
         n = 0;
         l.add(c, k);
+    }
+    // the place of this lane's key among those of `in`
+    __device__ __forceinline__ int place(uint64_t in) const {
+        return n + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
     }
     // the lanes' keys where `in`
     __device__ __forceinline__ void push(uint64_t in, double c, LpList& l, int k) {
         if (n + __builtin_popcountll(in) > 64) flush(l, k);
-        if (in >> (threadIdx.x & 63) & 1) q[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0))] = c;
+        if (in >> (threadIdx.x & 63) & 1) q[place(in)] = c;
         n += __builtin_popcountll(in);
     }
 };
+
+// dword i of a lane's vectors (registers: a tree of selects)
+template <int U>
+__device__ __forceinline__ uint32_t lp_dword(const uint4 (&w)[U], int i) {
+    uint32_t d[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t lo = i & 1 ? w[u].y : w[u].x, hi = i & 1 ? w[u].w : w[u].z;
+        d[u] = i & 2 ? hi : lo;
+    }
+#pragma unroll
+    for (int n = U, b = 4; n > 1; n /= 2, b *= 2)
+#pragma unroll
+        for (int u = 0; u < n / 2; ++u) d[u] = i & b ? d[2 * u + 1] : d[2 * u];
+    return d[0];
+}
 
 template <int DT>
 struct LpElem;  // logit type, logits of a 16-byte vector
@@ -150,6 +190,9 @@ struct LpElem<DT_F32> {
         w = make_uint4(w.y, w.z, w.w, 0);
         return x;
     }
+    // logit p of the lane's U vectors
+    template <int U>
+    static __device__ __forceinline__ float pick(const uint4 (&w)[U], int p) { return __uint_as_float(lp_dword(w, p)); }
     static __device__ __forceinline__ void unpack(uint4 w, float (&x)[N]) {
         x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
     }
@@ -165,6 +208,12 @@ struct LpElem<DT_BF16> {
         w = make_uint4(__builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16), __builtin_amdgcn_alignbit(w.w, w.z, 16),
                        w.w >> 16);
         return x;
+    }
+    // logit p of the lane's U vectors
+    template <int U>
+    static __device__ __forceinline__ float pick(const uint4 (&w)[U], int p) {
+        const uint32_t d = lp_dword(w, p >> 1);
+        return p & 1 ? bf_hi(d) : bf_lo(d);
     }
     static __device__ __forceinline__ void unpack(uint4 w, float (&x)[N]) {
         const uint32_t d[4] = {w.x, w.y, w.z, w.w};
@@ -183,6 +232,12 @@ struct LpElem<DT_F16> {
         w = make_uint4(__builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16), __builtin_amdgcn_alignbit(w.w, w.z, 16),
                        w.w >> 16);
         return x;
+    }
+    // logit p of the lane's U vectors
+    template <int U>
+    static __device__ __forceinline__ float pick(const uint4 (&w)[U], int p) {
+        const uint32_t d = lp_dword(w, p >> 1);
+        return h2f(p & 1 ? d >> 16 : d & 0xffffu);
     }
     static __device__ __forceinline__ void unpack(uint4 w, float (&x)[N]) {
         const uint32_t d[4] = {w.x, w.y, w.z, w.w};
@@ -206,7 +261,9 @@ struct LpArgs {
 // The row's token, -1 when there is none to look for (no tokens asked, or outside [0, V)).
 __device__ __forceinline__ int64_t lp_token(const LpArgs& a, int r) {
     if (!a.tok) return -1;
-    return a.tok64 ? ((const int64_t*)a.tok)[r] : (int64_t)((const int32_t*)a.tok)[r];
+    typedef const __attribute__((address_space(4))) int32_t* P;  // constant while the kernel runs: a scalar load
+    const P p = (P)(uintptr_t)a.tok;
+    return a.tok64 ? (int64_t)((uint64_t)(uint32_t)p[2 * (int64_t)r + 1] << 32 | (uint32_t)p[2 * (int64_t)r]) : (int64_t)p[r];
 }
 
 // the next float above x: v >= above(x) exactly if v > x (NaN where nothing is above)
@@ -270,7 +327,21 @@ struct LpSums {
     }
 };
 
-template <int DT, bool TOP, bool TOK>
+// At most the k-th greatest of the lanes' values (no NaN), to 16 bits of it
+__device__ __forceinline__ float lp_kth(float v, int k) {
+    const uint32_t b = __float_as_uint(v), o = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);  // in the values' order
+    uint32_t at = 0;
+#pragma unroll
+    for (int i = 31; i >= 16; --i) {
+        const uint32_t up = at | 1u << i;
+        if (__builtin_popcountll(__ballot(o >= up)) >= k) at = up;
+    }
+    at = max(at, 0x007fffffu);  // -inf
+    return __uint_as_float(at & 0x80000000u ? at ^ 0x80000000u : ~at);
+}
+
+// HELD (TOP): the chunk has at most kLpHeld tiles, which stay in registers.
+template <int DT, bool TOP, bool TOK, bool HELD>
 __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     using E = LpElem<DT>;
     constexpr int N = E::N, U = kLpUnroll;
@@ -283,6 +354,20 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     // whole 16-byte vectors of [lo, hi): [lo + head, lo + head + N nv); the rest (< 2 N logits) one a lane
     const int mis = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(typename E::T));
     const int head = min(mis ? N - mis : 0, hi - lo), nv = (hi - lo - head) / N, v0 = lo + head, tail = v0 + nv * N;
+    LpSums sum;
+    LpQueue queue(places[threadIdx.x >> 6]);
+    int rank = 0;  // of the wave, in a scalar
+    const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
+    auto load = [&](int base, uint4 (&to)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (base + u * 64 + lane < nv) to[u] = ldg_nt(reinterpret_cast<const uint8_t*>(vec + base + u * 64 + lane));
+    };
+    // Loads return in order: the first tile, the token's logit, what is left of the chunk, so that nothing waits for more than
+    // it needs. The token itself comes through the scalar cache.
+    constexpr int H = HELD ? kLpHeld : 1;
+    uint4 held[H][U];
+    load(0, held[0]);
     int tok = -1;
     float xt = 0.f, gt = NAN;
     if constexpr (TOK) {
@@ -293,46 +378,30 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
             gt = lp_above(xt);
         }
     }
-    LpSums sum;
-    LpList groups;
-    LpQueue queue(places[threadIdx.x >> 6]);
-    int rank = 0;  // of the wave, in a scalar
     // head and tail logits
     const int edge = lane < head ? lo + lane : lane < head + hi - tail ? tail + lane - head : -1;
     typename E::T edge_x = 0;
-    {
-        const int j = edge;
-        if (j >= 0) edge_x = row[j];
-        const float x = j >= 0 ? E::up(edge_x) : -INFINITY;
-        sum.raise(x);
-        const float one[1] = {x};
-        sum.add(one);
-        if constexpr (TOK) rank += __builtin_popcountll(__ballot(tok >= 0 && j >= 0 && (x > xt || (x == xt && j < tok))));
-    }
-    const uint4* vec = reinterpret_cast<const uint4*>(row + v0);
-    uint4 nx[U];
+    if (edge >= 0) edge_x = row[edge];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (u * 64 + lane < nv) nx[u] = ldg_nt(reinterpret_cast<const uint8_t*>(vec + u * 64 + lane));
-    for (int base = 0; base < nv; base += 64 * U) {
-        uint4 cur[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) cur[u] = nx[u];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {  // the next tile's vectors are under way while this one is summed
-            const int i = base + (U + u) * 64 + lane;
-            if (i < nv) nx[u] = ldg_nt(reinterpret_cast<const uint8_t*>(vec + i));  // read once
-        }
-        float x[U][N], vm[U], tm = -INFINITY;
+    for (int t = 1; t < H; ++t) load(64 * U * t, held[t]);
+    // a tile's logits, -inf behind the chunk's last
+    auto unpack = [&](int base, const uint4 (&from)[U], float (&x)[U][N]) {
         const bool whole = base + 64 * U <= nv;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            E::unpack(cur[u], x[u]);
+            E::unpack(from[u], x[u]);
             if (!whole) {
                 const bool in = base + u * 64 + lane < nv;
 #pragma unroll
                 for (int e = 0; e < N; ++e) x[u][e] = in ? x[u][e] : -INFINITY;
             }
+        }
+    };
+    // the sums and the rank over a tile; vm: its vectors' maxima
+    auto take = [&](int base, const float (&x)[U][N], float (&vm)[U]) {
+        float tm = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
             vm[u] = x[u][0];
 #pragma unroll
             for (int e = 1; e < N; ++e) vm[u] = fmaxf(vm[u], x[u][e]);
@@ -358,57 +427,144 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
                 }
             }
         }
-        if constexpr (TOP) {
-            // lane 4 g + u of a quad takes group g of vectors [64 u, 64 u + 64)
-            float gm = 0.f;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float m = fmaxf(vm[u], dpp_f<DPP_QP_1032>(vm[u]));
-                m = fmaxf(m, dpp_f<DPP_QP_2301>(m));
-                if ((lane & 3) == u) gm = m;
-            }
-            const int g = (base >> 2) + (lane & 3) * 16 + (lane >> 2);
-            const double c = 4 * g < nv ? lp_key(gm, g) : 0.;
-            const uint64_t in = __ballot(c > groups.last(a.k));
-            if (in) queue.push(in, c, groups, a.k);
-        }
-    }
-    sum.join();
+        return tm;
+    };
     const int64_t at = (int64_t)r * a.S + s;
-    if (lane == 0) a.part[at] = LpPart{sum.m, sum.z, sum.t, rank};
-    if constexpr (TOP) {
-        // the k best groups again, a vector a lane, 16 groups a load, and before them the head and tail logits; one copy of
-        // the list's code in a rolled loop: unrolled, fetching instructions took longer than running them
-        queue.flush(groups, a.k);
-        // k maxima reach the k-th: nothing below it is among the k first
-        const double kth = groups.last(a.k);
-        const float least = kth > 0. ? lp_value(kth) : -INFINITY;
+    if constexpr (HELD) {
+        float x[U][N], vm[U], most = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < H; ++t) {
+            if (64 * U * t >= nv) break;
+            unpack(64 * U * t, held[t], x);
+            most = fmaxf(most, take(64 * U * t, x, vm));
+        }
+        // k lanes' maxima reach the k-th of them: nothing below it is among the k first. What reaches it, usually little
+        // more than k, is packed into the queue's places.
+        const float least = lp_kth(most, a.k);
+        if (least == -INFINITY) queue.n = 65;  // also logits of -inf, whose difference has no sign
         LpList elems;
-        auto fetch = [&](int i, uint4& w, int& j) {
-            const int e = 16 * i + (lane >> 2);
-            const double c = __shfl(groups.v, e, 64);
-            const int vi = 4 * lp_index(c) + (lane & 3);
-            j = e < a.k && c > 0. && vi < nv ? v0 + vi * N : -1;
-            if (j >= 0) w = vec[vi];
-        };
-        uint4 w = make_uint4(E::bits(edge_x), 0, 0, 0), w1 = w;
-        int j = edge, n = 1, j1;
-        fetch(0, w1, j1);
-#pragma unroll 1
-        for (int i = 1;; ++i) {
-#pragma unroll 1
-            for (int e = 0; e < n; ++e) {
-                const float x = E::pop(w);
-                const uint64_t in = __ballot(j >= 0 && x >= least);
-                if (in) queue.push(in, lp_key(x, j + e), elems, a.k);
+        auto pack = [&](bool in, float v, int j) {
+            const uint64_t go = __ballot(in);
+            if (go) {
+                const int to = queue.place(go);
+                if (in && to < 64) queue.q[to] = lp_key(v, j);
+                queue.n += __builtin_popcountll(go);
             }
-            if (16 * (i - 1) >= a.k) break;
-            w = w1, j = j1, n = N;
-            if (16 * i < a.k) fetch(i, w1, j1);
+        };
+        {
+            const float v = edge >= 0 ? E::up(edge_x) : 0.f;
+            pack(edge >= 0 && v >= least, v, edge);
+        }
+#pragma unroll
+        for (int t = 0; t < H; ++t) {
+            if (64 * U * t >= nv || queue.n > 64) break;
+            unpack(64 * U * t, held[t], x);
+            // which of the lane's U N logits reach it, the first at the top: the differences' signs, two instructions a logit (a
+            // NaN's sign may be either: its key is that of no entry)
+            uint32_t mine = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < N; ++e) mine = __builtin_amdgcn_alignbit(mine, __float_as_uint(x[u][e] - least), 31);
+            mine = ~mine << (32 - U * N);
+            const int there = (nv - 64 * U * t - lane + 63) / 64 * N;  // the lane's logits up to the chunk's end
+            if (there < U * N) mine &= there > 0 ? ~(0xffffffffu >> there) : 0u;
+            while (queue.n <= 64 && __any(mine)) {
+                const int p = __builtin_clz(mine | 1u), j = v0 + (64 * (U * t + p / N) + lane) * N + p % N;
+                pack(mine != 0, E::pick(held[t], p), j);
+                mine &= ~(0x80000000u >> p);
+            }
+        }
+        if (queue.n > 64) {  // many equal ones, or the greatest in few lanes: again, a full queue's at a time, from memory
+            queue.n = 0;
+            uint4 w = make_uint4(E::bits(edge_x), 0, 0, 0);
+            int j = edge, n = 1;
+#pragma unroll 1
+            for (int b = 0;; b += 64) {
+#pragma unroll 1
+                for (int e = 0; e < n; ++e) {
+                    const float v = E::pop(w);
+                    const double c = lp_key(v, j + e);
+                    const uint64_t in = __ballot(j >= 0 && v >= least && c > elems.last(a.k));
+                    if (in) queue.push(in, c, elems, a.k);
+                }
+                if (b >= nv) break;
+                n = N;
+                j = b + lane < nv ? v0 + (b + lane) * N : -1;
+                if (j >= 0) w = vec[b + lane];
+            }
         }
         queue.flush(elems, a.k);
         if (lane < a.k) a.list[at * a.k + lane] = elems.v;
+    } else {
+        LpList groups;
+        uint4 (&nx)[U] = held[0];
+        for (int base = 0; base < nv; base += 64 * U) {
+            uint4 cur[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) cur[u] = nx[u];
+            load(base + 64 * U, nx);  // under way while this tile is summed
+            float x[U][N], vm[U];
+            unpack(base, cur, x);
+            take(base, x, vm);
+            if constexpr (TOP) {
+                // lane 4 g + u of a quad takes group g of vectors [64 u, 64 u + 64)
+                float gm = 0.f;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float m = fmaxf(vm[u], dpp_f<DPP_QP_1032>(vm[u]));
+                    m = fmaxf(m, dpp_f<DPP_QP_2301>(m));
+                    if ((lane & 3) == u) gm = m;
+                }
+                const int g = (base >> 2) + (lane & 3) * 16 + (lane >> 2);
+                const double c = 4 * g < nv ? lp_key(gm, g) : 0.;
+                const uint64_t in = __ballot(c > groups.last(a.k));
+                if (in) queue.push(in, c, groups, a.k);
+            }
+        }
+        if constexpr (TOP) {
+            // the k best groups again, a vector a lane, 16 groups a load, and before them the head and tail logits; one copy of
+            // the list's code in a rolled loop: unrolled, fetching instructions took longer than running them
+            queue.flush(groups, a.k);
+            // k maxima reach the k-th: nothing below it is among the k first
+            const double kth = groups.last(a.k);
+            const float least = kth > 0. ? lp_value(kth) : -INFINITY;
+            LpList elems;
+            auto fetch = [&](int i, uint4& w, int& j) {
+                const int e = 16 * i + (lane >> 2);
+                const double c = __shfl(groups.v, e, 64);
+                const int vi = 4 * lp_index(c) + (lane & 3);
+                j = e < a.k && c > 0. && vi < nv ? v0 + vi * N : -1;
+                if (j >= 0) w = vec[vi];
+            };
+            uint4 w = make_uint4(E::bits(edge_x), 0, 0, 0), w1 = w;
+            int j = edge, n = 1, j1;
+            fetch(0, w1, j1);
+#pragma unroll 1
+            for (int i = 1;; ++i) {
+#pragma unroll 1
+                for (int e = 0; e < n; ++e) {
+                    const float x = E::pop(w);
+                    const uint64_t in = __ballot(j >= 0 && x >= least);
+                    if (in) queue.push(in, lp_key(x, j + e), elems, a.k);
+                }
+                if (16 * (i - 1) >= a.k) break;
+                w = w1, j = j1, n = N;
+                if (16 * i < a.k) fetch(i, w1, j1);
+            }
+            queue.flush(elems, a.k);
+            if (lane < a.k) a.list[at * a.k + lane] = elems.v;
+        }
     }
+    {  // the head and tail logits
+        const float x = edge >= 0 ? E::up(edge_x) : -INFINITY;
+        sum.raise(x);
+        const float one[1] = {x};
+        sum.add(one);
+        if constexpr (TOK) rank += __builtin_popcountll(__ballot(tok >= 0 && edge >= 0 && (x > xt || (x == xt && edge < tok))));
+    }
+    sum.join();
+    if (lane == 0) a.part[at] = LpPart{sum.m, sum.z, sum.t, rank};
 }
 
 template <int DT>
@@ -420,6 +576,10 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     const int64_t at = (int64_t)r * a.S;
     LpPart p{-INFINITY, 0.f, 0.f, 0};
     if (lane < a.S) p = a.part[at + lane];
+    // the chunks' sorted lists, a lane each
+    const double* list = a.list + (at + lane) * a.k;
+    auto fetch = [&](int i) { return lane < a.S && i < a.k ? list[i] : 0.; };
+    double c0 = fetch(0), c1 = fetch(1), c2 = fetch(2);
     LpSums sum;
     sum.m = p.m, sum.z = p.z, sum.t = p.t;
     sum.join();
@@ -437,18 +597,15 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
         }
     }
     if (a.k == 0) return;
-    // the chunks' sorted lists, a lane each, from the front until no front can enter
+    // The heads first: of what follows in the lists only what comes before the k-th so far can enter, from the fronts until
+    // no front can.
     LpList top;
-    const double* list = a.list + (at + lane) * a.k;
-    auto fetch = [&](int i) { return lane < a.S && i < a.k ? list[i] : 0.; };
-    double c0 = fetch(0), c1 = fetch(1), c2 = fetch(2);
-    // the heads first; what comes before the k-th of them is all that can still enter, and it stands at the lists' fronts
-    top.add(c0, a.k);
-    const double least = top.last(a.k);
     LpQueue queue(places[threadIdx.x >> 6]);
+    queue.push(__ballot(c0 > 0.), c0, top, a.k);
+    queue.flush(top, a.k);
 #pragma unroll 1
     for (int i = 1; i < a.k; ++i) {
-        const uint64_t in = __ballot(c1 > least);
+        const uint64_t in = __ballot(c1 > top.last(a.k));
         if (!in) break;
         queue.push(in, c1, top, a.k);
         c1 = c2;
@@ -469,12 +626,14 @@ static int lp_splits(int R, int V) {
 }
 
 template <int DT>
-static void lp_launch(const LpArgs& a, hipStream_t st) {
+static void lp_launch(const LpArgs& a, bool held, hipStream_t st) {
     const dim3 grid((unsigned)(((int64_t)a.R * a.S + 3) / 4)), block(256);
-    if (a.k && a.tok) hipLaunchKernelGGL((k_logprobs_part<DT, true, true>), grid, block, 0, st, a);
-    else if (a.k) hipLaunchKernelGGL((k_logprobs_part<DT, true, false>), grid, block, 0, st, a);
-    else if (a.tok) hipLaunchKernelGGL((k_logprobs_part<DT, false, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((k_logprobs_part<DT, false, false>), grid, block, 0, st, a);
+    if (a.k && a.tok && held) hipLaunchKernelGGL((k_logprobs_part<DT, true, true, true>), grid, block, 0, st, a);
+    else if (a.k && held) hipLaunchKernelGGL((k_logprobs_part<DT, true, false, true>), grid, block, 0, st, a);
+    else if (a.k && a.tok) hipLaunchKernelGGL((k_logprobs_part<DT, true, true, false>), grid, block, 0, st, a);
+    else if (a.k) hipLaunchKernelGGL((k_logprobs_part<DT, true, false, false>), grid, block, 0, st, a);
+    else if (a.tok) hipLaunchKernelGGL((k_logprobs_part<DT, false, true, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((k_logprobs_part<DT, false, false, false>), grid, block, 0, st, a);
     hipLaunchKernelGGL((k_logprobs_join<DT>), dim3((a.R + 3) / 4), block, 0, st, a);
 }
 
@@ -500,15 +659,16 @@ int wf_token_logprobs(const void* logits, int dtype, int64_t ld, int R, int V, c
     WF_REQUIRE(logits && ws && aligned16(ws), "token_logprobs: null logits, or a workspace that is null or not 16-byte aligned");
     WF_REQUIRE(!tokens || (logprobs && ranks), "token_logprobs: null logprobs / ranks");
     WF_REQUIRE(top_k == 0 || (top_ids && top_logprobs), "token_logprobs: null top_ids / top_logprobs");
-    const int S = lp_splits(R, V);
+    const int S = lp_splits(R, V), chunk = (int)((((int64_t)V + S - 1) / S + 31) / 32 * 32);
+    // k past 32: what reaches the k-th of 64 maxima is 64 ln(64 / (64 - k)) logits, more than a queue's places
+    const bool held = top_k <= 32 && chunk <= kLpHeld * 64 * kLpUnroll * (dtype == WF_F32 ? 4 : 8);
     WF_REQUIRE((int64_t)R * S <= 4 * kMaxWgs256, "token_logprobs: too many rows (%d)", R);
-    const int chunk = (int)((((int64_t)V + S - 1) / S + 31) / 32 * 32);
     LpPart* part = reinterpret_cast<LpPart*>(ws);
     LpArgs a{logits, ld, R, V, S, chunk, tokens, tokens64, top_k, part, reinterpret_cast<double*>(part + (int64_t)R * S), logprobs, entropy, top_logprobs, ranks, top_ids};
     hipStream_t st = as_stream(stream);
-    if (dtype == WF_F32) lp_launch<DT_F32>(a, st);
-    else if (dtype == WF_BF16) lp_launch<DT_BF16>(a, st);
-    else lp_launch<DT_F16>(a, st);
+    if (dtype == WF_F32) lp_launch<DT_F32>(a, held, st);
+    else if (dtype == WF_BF16) lp_launch<DT_BF16>(a, held, st);
+    else lp_launch<DT_F16>(a, held, st);
     return check_launch("token_logprobs");
 }
 
