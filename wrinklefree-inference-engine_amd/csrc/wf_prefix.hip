@@ -463,36 +463,47 @@ __global__ __launch_bounds__(256) void k_prefix_join(PfArgs a, int odt) {
     const int lane = threadIdx.x & 63;
     if (row >= (int64_t)a.B * a.Hq) return;
     const int b = (int)(row / a.Hq), hq = (int)(row - (int64_t)b * a.Hq);
+    // Records of a row stand at fixed places, NP of the prefix's ranges and NS of the suffix's: their sums and the first records
+    // are under way before the lengths say which of them were written.
+    const int R = a.NP + a.NS;
+    const float2* ml = a.ml + row * R;
+    const float2* o = reinterpret_cast<const float2*>(a.o + row * R * kPfDim) + lane;
+    const float2 none = make_float2(-INFINITY, 0.f);
+    float2 e0 = lane < R ? ml[lane] : none, e1 = lane + 64 < R ? ml[lane + 64] : none;
+    const float2 o_prefix = o[0], o_suffix = o[a.NP * (kPfDim / 2)];
     const PfSeq s = pf_seq(a, b);
     const bool sh = pf_shared(a, b, s);
     const int tp = sh ? pf_tiles(s.P) : 0, pp = pf_per(tp, a.NP, kPfMinTiles), np = (tp + pp - 1) / pp;
     const int n1 = sh ? 0 : pf_tiles(s.P), ts = s.L > s.P ? n1 + pf_tiles(s.L) - s.P / kPfPage : n1;
     const int ps = pf_per(ts, a.NS, kPfMinSuffix), ns = (ts + ps - 1) / ps;
-    const float2* ml = a.ml + row * (a.NP + a.NS);
-    const float2* o = reinterpret_cast<const float2*>(a.o + row * (a.NP + a.NS) * kPfDim) + lane;
-    // lane i: the max and sum of records i and i + 64 (2 kPfMaxRecords at most)
-    const int n = np + ns;
-    auto place = [&](int i) { return i < np ? i : a.NP + i - np; };
-    const float2 none = make_float2(-INFINITY, 0.f);
-    const float2 e0 = lane < n ? ml[place(lane)] : none, e1 = lane + 64 < n ? ml[place(lane + 64)] : none;
+    auto written = [&](int i) { return i < a.NP ? i < np : i - a.NP < ns; };
+    e0 = written(lane) ? e0 : none;
+    e1 = written(lane + 64) ? e1 : none;
     const float M = wave_max(fmaxf(e0.x, e1.x));
     auto weight = [&](float2 e) {
         return M == -INFINITY ? 1.f : e.x == -INFINITY ? (e.y == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(e.x - M);
     };
     const float w0 = weight(e0), w1 = weight(e1), L = wave_sum(e0.y * w0 + e1.y * w1);
     float x = 0.f, y = 0.f;
-    for (int i = 0; i < n; i += 4) {
-        float2 v[4];
+    auto add = [&](int i, float2 v) {
+        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(i < 64 ? w0 : w1), i & 63));
+        x += v.x * w;
+        y += v.y * w;
+    };
+    auto part = [&](int first, int n, float2 v0) {
+        if (n > 0) add(first, v0);
+        for (int i = 1; i < n; i += 4) {
+            float2 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = i + k < n ? o[place(i + k) * (kPfDim / 2)] : make_float2(0.f, 0.f);
+            for (int k = 0; k < 4; ++k)
+                if (i + k < n) v[k] = o[(first + i + k) * (kPfDim / 2)];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float wk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(i + k < 64 ? w0 : w1), (i + k) & 63));
-            const float w = i + k < n ? wk : 0.f;
-            x += v[k].x * w;
-            y += v[k].y * w;
+            for (int k = 0; k < 4; ++k)
+                if (i + k < n) add(first + i + k, v[k]);
         }
-    }
+    };
+    part(0, np, o_prefix);
+    part(a.NP, ns, o_suffix);
     // no key, or none with a score above -inf: zeros
     const float inv = L == 0.f ? 0.f : a.vs / L;
     const int64_t at = b * a.o_sb + hq * a.o_sh + 2 * lane;
