@@ -20,6 +20,11 @@
 // The running max is raised only when a tile passes it by 2^8 (its exchange between the four lanes of a row and
 // the rescaling of o are rare then): p <= 2^8 is as exact in bf16 and 32 bits as p <= 1.
 //
+// What bounds it: a wave loads 16 KiB (bf16) a tile for 32 rows, through the 64 bytes a cycle of its CU's L1: some 2000 cycles
+// a tile for four waves, twice the matrix and softmax work. Suffixes run at HBM's rate beside them. Measured a call, 20 query and 5 kv
+// heads, bf16, batch 128: 1024 shared keys and suffixes to 512 (88 MB) 31 us; 32768 and suffixes to 1024 (253 MB) 101 us; no
+// sharing, 1024 keys each (335 MB) 59 us, 5.6 TB/s.
+//
 // Operands and rounding: scores, max, sums and o in 32 bits. The matrices are bf16, and f16 where q is f16 and the pool holds
 // one-byte codes (all of them f16 values). Where the pool is bf16, an f16 q enters as the exact sum of two bf16 terms;
 // an f32 q as three. P is rounded once to the output's type where that is the matrices' (bf16 2^-8, f16 2^-11 a
