@@ -472,3 +472,75 @@ def test_serving_ops_in_a_graph_and_on_another_stream():
     torch.cuda.synchronize()
     for i, p in enumerate(both):
         assert torch.equal(p.top_ids, want[i % 2].top_ids) and torch.equal(p.top_logprobs, want[i % 2].top_logprobs)
+
+
+def test_offsets_past_32_bits():
+    """Rows 2^30 elements apart: the third begins at element 2^31."""
+    from wfamd import ops
+    base = torch.empty((1 << 31) + 4096, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator("cuda").manual_seed(6)
+    x = base.as_strided((3, 1000), (1 << 30, 1))
+    x.copy_(torch.randn(3, 1000, generator=g, device="cuda"))
+    a, b = ops.token_logprobs(x, torch.tensor([3, 4, 5], device="cuda"), 20), ops.token_logprobs(x.contiguous(), torch.tensor([3, 4, 5], device="cuda"), 20)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    q = base.as_strided((3, 4, 64), (1 << 30, 128, 1))
+    k = base.as_strided((3, 4, 64), (1 << 30, 128, 1), 64)
+    q.copy_(torch.randn(3, 4, 64, generator=g, device="cuda"))
+    k.copy_(torch.randn(3, 4, 64, generator=g, device="cuda"))
+    pos = torch.tensor([5, 0, 70000], device="cuda")
+    freqs, _ = ops.rotary_frequencies(64)
+    want = ops.rotary_embed(q.contiguous(), k.contiguous(), pos, freqs)
+    got = ops.rotary_embed(q, k, pos, freqs)
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
+    got = ops.rotary_embed(q, k, pos, freqs, inplace=True)  # heads of q and k in turn
+    assert got[0] is q and got[1] is k and torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+def test_rotary_in_place_on_slices_of_one_projection():
+    from wfamd import ops
+    g = torch.Generator("cuda").manual_seed(7)
+    qkv = torch.randn(9, 12, 64, generator=g, device="cuda")
+    pos = torch.arange(9, device="cuda", dtype=torch.int32) * 100
+    freqs, _ = ops.rotary_frequencies(64)
+    before = qkv.clone()
+    q, k = ops.rotary_embed(before[:, :8], before[:, 8:10], pos, freqs)
+    ops.rotary_embed(qkv[:, :8], qkv[:, 8:10], pos, freqs, inplace=True)
+    assert torch.equal(qkv[:, :8], q) and torch.equal(qkv[:, 8:10], k) and torch.equal(qkv[:, 10:], before[:, 10:])
+    for bad in (qkv[:, 7:9], qkv[:, :2], qkv[:, 4:8]):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.rotary_embed(qkv[:, :8], bad, pos, freqs, inplace=True)
+
+
+def test_two_graphs_of_each_operator_replayed_in_turn():
+    """Workspaces and results of two captured calls of one operator stay their own."""
+    from wfamd import ops
+    g = torch.Generator("cuda").manual_seed(8)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    x = [torch.randn(130, 9000, generator=g, device="cuda").bfloat16() for _ in range(2)]
+    lens = [torch.randint(0, 40, (3000,), generator=g, device="cuda", dtype=torch.int32) for _ in range(2)]
+    free, tables = torch.arange(9000, device="cuda", dtype=torch.int32), [torch.zeros(3000, 8, dtype=torch.int32, device="cuda") for _ in range(2)]
+    q, pos = [torch.randn(50, 4, 64, generator=g, device="cuda") for _ in range(2)], i32(list(range(50)))
+    freqs, _ = ops.rotary_frequencies(64)
+    calls = [lambda i: ops.token_logprobs(x[i], None, 20), lambda i: ops.kv_page_plan(lens[i], lens[1 - i], free, tables[i], 60000),
+             lambda i: (ops.rotary_embed(q[i], None, pos, freqs)[0],)]
+    for call in calls:
+        want = [[t.clone() for t in call(i) if t is not None] for i in range(2)]
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            call(0)
+        s.synchronize()
+        graphs = []
+        for i in range(2):
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr):
+                out = call(i)
+            graphs.append((gr, [t for t in out if t is not None]))
+        for _ in range(3):
+            for gr, _out in graphs:
+                gr.replay()
+            torch.cuda.synchronize()
+            for (_gr, out), w in zip(graphs, want):
+                assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(out, w))
+            call(0)  # the program's own work in between
+            torch.cuda.synchronize()
