@@ -273,15 +273,17 @@ struct PfState {
 // the moment this one's scores are done, its V from the moment this one's products are: one set of registers,
 // and half a tile's work over each load's latency.
 template <class State, class Page, class Range>
-__device__ __forceinline__ void pf_walk(const PfArgs& a, State& st, int64_t head, int k0, int k1, Page page, Range range) {
+__device__ __forceinline__ void pf_walk(const PfArgs& a, State& st, const uint8_t* q, int64_t head, int k0, int k1, Page page, Range range) {
     using T = typename State::T;
     const int lane = threadIdx.x & 63, n = (k1 - k0 + 3) / 4;
     if (n <= 0) return;
     T kf[8], vf[8];
-    int ids = -1;
+    int ids = k0 + 4 * lane < k1 ? page(k0 + 4 * lane) : -1;
+    st.load_q(q, a.neg, a.qvec);  // beside the ids' latency, not before it
+    ids = ids < a.np ? ids : -1;
     // the id of tile number i (0, 1, ..) of the walk; < 0 where the pool has no such page
     auto find = [&](int i) {
-        if ((i & 63) == 0) {
+        if (i > 0 && (i & 63) == 0) {
             const int k = k0 + 4 * (i + lane);
             ids = k < k1 ? page(k) : -1;
             ids = ids < a.np ? ids : -1;
@@ -370,10 +372,10 @@ __device__ __forceinline__ void pf_run(const PfArgs& a, void* lds, int h, int z,
     PfState<W, KVQ, QDT> st;
     const int64_t r = min(ra + st.row(), rb - 1);
     const int b = (int)(r / a.G), g = (int)(r - (int64_t)b * a.G);
-    st.load_q((const uint8_t*)a.q + (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2), a.neg, a.qvec);
+    const uint8_t* q = (const uint8_t*)a.q + (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2);
     st.clear();
     const int32_t* row = a.pt + owner * a.pts;
-    pf_walk(a, st, h * a.hs, k0 + (int)(threadIdx.x >> 6), k1, [&](int k) { return row[k]; },
+    pf_walk(a, st, q, h * a.hs, k0 + (int)(threadIdx.x >> 6), k1, [&](int k) { return row[k]; },
             [&](int k, int& lo, int& hi) { lo = 0, hi = P - k * kPfPage; });
     pf_merge(a, *static_cast<PfShared<W>*>(lds), st.acc, st.m - st.kUp, st.l, [&](int i) -> int64_t {
         if (ra + i >= rb) return -1;
@@ -427,9 +429,9 @@ __device__ void pf_suffix(const PfArgs& a, void* lds, int z, int hc, int b) {
     if (k0 >= k1) return;
     PfState<16, KVQ, QDT> st;
     const int g = min(ct * 16 + st.row(), a.G - 1);
-    st.load_q((const uint8_t*)a.q + (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2), a.neg, a.qvec);
+    const uint8_t* q = (const uint8_t*)a.q + (b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh) * (QDT == DT_F32 ? 4 : 2);
     st.clear();
-    pf_walk(a, st, h * a.hs, k0 + (int)(threadIdx.x >> 6), k1,
+    pf_walk(a, st, q, h * a.hs, k0 + (int)(threadIdx.x >> 6), k1,
             [&](int k) { return a.pt[(k < n1 ? s.owner : b) * a.pts + (k < n1 ? k : first + k - n1)]; },
             [&](int k, int& lo, int& hi) {
                 const int at = (k < n1 ? k : first + k - n1) * kPfPage;
