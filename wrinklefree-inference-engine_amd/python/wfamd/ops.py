@@ -435,14 +435,20 @@ def _table_stride(name: str, t: torch.Tensor, b: int) -> int:
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a torch.cuda.Stream around it (2 us)
+_current_device = torch._C._cuda_getDevice  # what torch.cuda.current_device() returns once there is a device tensor
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    return getattr(_lib.load(), name)
 
 
 def _call_on(index: int, name: str, args: tuple) -> None:
     """Launch on the current stream of device `index`, with it current (kernels go to the device that is current)."""
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         with torch.cuda.device(index):
             return _call_on(index, name, args)
-    rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
+    rc = _entry(name)(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, name)
 
@@ -450,7 +456,7 @@ def _call_on(index: int, name: str, args: tuple) -> None:
 @functools.lru_cache(maxsize=256)
 def _ws_bytes(name: str, *sizes: int) -> int:
     """A workspace size: host arithmetic on sizes alone."""
-    return int(getattr(_lib.load(), name)(*sizes))
+    return int(_entry(name)(*sizes))
 
 
 class KVPagePlan(NamedTuple):
@@ -486,11 +492,11 @@ def kv_page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
     if n < 0:
         raise ValueError(f"kv_page_plan: num_tokens {n} is negative")
     pad = -n % 4 if n > 4096 else 0  # large arrays begin on 16-byte lines
-    out = torch.empty(4 * (n + pad) + b + 5, dtype=torch.int32, device=cached_lens.device)
+    out = cached_lens.new_empty(4 * (n + pad) + b + 5)
     if pad:
-        pages, _, slots, _, rows, _, pos, _, counts, cu = out.split([n, pad, n, pad, n, pad, n, pad, 4, b + 1])
+        pages, _, slots, _, rows, _, pos, _, counts, cu = out.split_with_sizes([n, pad, n, pad, n, pad, n, pad, 4, b + 1])
     else:
-        pages, slots, rows, pos, counts, cu = out.split([n, n, n, n, 4, b + 1])
+        pages, slots, rows, pos, counts, cu = out.split_with_sizes([n, n, n, n, 4, b + 1])
     nws = _ws_bytes("wf_kv_page_plan_ws_bytes", b)
     ws = torch.empty(nws, dtype=torch.uint8, device=out.device) if nws else None
     base, step = out.data_ptr(), 4 * (n + pad)
@@ -590,8 +596,8 @@ def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
             raise ValueError("rotary_embed: q and k share memory, turned in place it would be turned twice")
         qo, ko = q, k
     else:
-        qo = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty((T, k.shape[1], D), dtype=q.dtype, device=q.device)
+        qo = q.new_empty((T, Hq, D))
+        ko = None if k is None else q.new_empty((T, k.shape[1], D))
         if q.stride(2) != 1:
             q = q.contiguous()
         if k is not None and k.stride(2) != 1:
@@ -652,9 +658,9 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
         q = q.contiguous()
         qs = q.stride()
     cols = page_table.shape[1]
-    out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+    out = q.new_empty((B, Hq, D))
     lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-    ws = torch.empty(_ws_bytes("wf_shared_prefix_attention_ws_bytes", code, B, Hq, Hkv, cols), dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(_ws_bytes("wf_shared_prefix_attention_ws_bytes", code, B, Hq, Hkv, cols), dtype=torch.uint8)
     _call_on(index, "wf_shared_prefix_attention", (q.data_ptr(), code, qs[0], qs[1], k_pool.data_ptr(), v_pool.data_ptr(), quant, ks[0], ks[1],
              pages, page_table.data_ptr(), ts, cols, seq_lens.data_ptr(), prefix_rows.data_ptr(), prefix_lens.data_ptr(), k_scale, v_scale,
              D ** -0.5 if sm_scale is None else sm_scale, B, Hq, Hkv, D, out.data_ptr(), Hq * D, D, _ptr(lse), ws.data_ptr()))
@@ -688,17 +694,17 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     if V > 1 and step != 1 or R > 1 and ld < V:
         logits = logits.contiguous()
         ld = V
-    dev = logits.device
+    new = logits.new_empty
     lp = rank = None
     if tokens is not None:
         if tokens.shape != (R,) or tokens.dtype not in (torch.int32, torch.int64) or not tokens.is_contiguous():
             raise ValueError(f"token_logprobs: tokens must be a contiguous int32 or int64 [{R}], got {tokens.dtype} {tuple(tokens.shape)}")
-        lp = torch.empty(R, dtype=torch.float32, device=dev)
-        rank = torch.empty(R, dtype=torch.int32, device=dev)
-    ent = torch.empty(R, dtype=torch.float32, device=dev)
-    ids = torch.empty((R, k), dtype=torch.int32, device=dev)
-    top = torch.empty((R, k), dtype=torch.float32, device=dev)
-    ws = torch.empty(_ws_bytes("wf_token_logprobs_ws_bytes", R, V, k), dtype=torch.uint8, device=dev)
+        lp = new(R, dtype=torch.float32)
+        rank = new(R, dtype=torch.int32)
+    ent = new(R, dtype=torch.float32)
+    ids = new((R, k), dtype=torch.int32)
+    top = new((R, k), dtype=torch.float32)
+    ws = new(_ws_bytes("wf_token_logprobs_ws_bytes", R, V, k), dtype=torch.uint8)
     _call_on(index, "wf_token_logprobs", (logits.data_ptr(), code, ld, R, V, _ptr(tokens), tokens is not None and tokens.dtype is torch.int64,
              k, _ptr(lp), _ptr(rank), ent.data_ptr(), ids.data_ptr(), top.data_ptr(), ws.data_ptr()))
     return TokenLogprobs(lp, rank, ent, ids, top)
