@@ -26,6 +26,8 @@ namespace wf {
 constexpr int kLpMaxTop = 64;
 constexpr int kLpUnroll = 4;        // 16-byte vectors a lane holds of a tile
 constexpr int kLpHeld = 2;          // tiles of a chunk that stay in registers
+constexpr int kLpPlaces = 128;      // places for what may be among their alternatives
+constexpr int kLpMergeLists = 16;   // chunks of a row up to which the join merges whole lists
 constexpr int kLpMaxSplits = 64;    // chunks of a row: a lane each in the join
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
@@ -88,6 +90,11 @@ struct LpList {
         step<31, 16>(v), clean<8>(v);
         step<63, 32>(v), clean<16>(v);
     }
+    // with another sorted list
+    __device__ __forceinline__ void merge(double c) {
+        v = __builtin_fmax(v, lp_xor<63>(c));  // the first 64 of both, a bitonic sequence
+        clean<32>(v);
+    }
     static __device__ __forceinline__ double lane(double v, int l) {
         return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l));
     }
@@ -99,8 +106,7 @@ struct LpList {
         if (__builtin_popcountll(todo) > 8) {
             c = todo >> (threadIdx.x & 63) & 1 ? c : 0.;
             sort(c);
-            v = __builtin_fmax(v, lp_xor<63>(c));  // the first 64 of both lists, a bitonic sequence
-            clean<32>(v);
+            merge(c);
             return;
         }
         while (todo) {
@@ -116,35 +122,59 @@ struct LpList {
 
 // Candidates on their way to a list: packed into the wave's 64 places in LDS by a ballot and a lane count each, taken in
 // together when the places are full or at the end.
+// LDS of one wave: its accesses are in order, the compiler's too
+__device__ __forceinline__ void lp_meet() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// The first 64 of the n <= P keys in the wave's P places (P = 64, 128), a lane each: a key's place is the number of greater ones.
+template <int P>
+__device__ __forceinline__ double lp_order(double* q, int n) {
+    const int lane = threadIdx.x & 63;
+    lp_meet();
+    double c[P / 64];
+    int at[P / 64], keys = 0;  // keys: without those of no entry
+#pragma unroll
+    for (int h = 0; h < P / 64; ++h) {
+        c[h] = lane + 64 * h < n ? q[lane + 64 * h] : 0.;
+        at[h] = 0;
+        keys += __builtin_popcountll(__ballot(c[h] > 0.));
+    }
+    lp_meet();
+#pragma unroll
+    for (int h = 0; h < P / 64; ++h) q[lane + 64 * h] = c[h];
+    lp_meet();
+#pragma unroll 1
+    for (int i = 0; i < n; i += 8)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const double k = q[i + e];
+#pragma unroll
+            for (int h = 0; h < P / 64; ++h) at[h] += k > c[h];
+        }
+    lp_meet();
+#pragma unroll
+    for (int h = 0; h < P / 64; ++h)
+        if (c[h] > 0. && at[h] < 64) q[at[h]] = c[h];
+    lp_meet();
+    const double v = lane < keys ? q[lane] : 0.;
+    lp_meet();
+    return v;
+}
+
 struct LpQueue {
     double* q;
     int n;  // of the wave, in a scalar
     __device__ __forceinline__ explicit LpQueue(double* places) : q(places), n(0) {}
-    static __device__ __forceinline__ void meet() {  // LDS of one wave: its accesses are in order, the compiler's too
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    }
     __device__ __forceinline__ void flush(LpList& l, int k) {
-        meet();
-        const int lane = threadIdx.x & 63;
-        const double c = lane < n ? q[lane] : 0.;
-        meet();
-        if (!(l.last(1) > 0.)) {  // into an empty list: a key's place is the number of greater ones
-            int at = 0;
-            if (lane >= n) q[lane] = 0.;
-            meet();
-#pragma unroll 1
-            for (int i = 0; i < n; i += 8)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) at += q[i + e] > c;
-            meet();
-            if (lane < n) q[at] = c;
-            meet();
-            l.v = lane < n ? q[lane] : 0.;
-            meet();
+        if (!(l.last(1) > 0.)) {
+            l.v = lp_order<64>(q, n);
             n = 0;
             return;
         }
+        lp_meet();
+        const double c = (int)(threadIdx.x & 63) < n ? q[threadIdx.x & 63] : 0.;
+        lp_meet();
         n = 0;
         l.add(c, k);
     }
@@ -327,14 +357,21 @@ struct LpSums {
     }
 };
 
-// At most the k-th greatest of the lanes' values (no NaN), to 16 bits of it
-__device__ __forceinline__ float lp_kth(float v, int k) {
-    const uint32_t b = __float_as_uint(v), o = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);  // in the values' order
-    uint32_t at = 0;
+// At most the k-th greatest of the lanes' M values each (no NaN), to 16 bits of it
+template <int M>
+__device__ __forceinline__ float lp_kth(const float (&v)[M], int k) {
+    uint32_t o[M], at = 0;
 #pragma unroll
-    for (int i = 31; i >= 16; --i) {
-        const uint32_t up = at | 1u << i;
-        if (__builtin_popcountll(__ballot(o >= up)) >= k) at = up;
+    for (int m = 0; m < M; ++m) {
+        const uint32_t b = __float_as_uint(v[m]);
+        o[m] = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);  // in the values' order
+    }
+#pragma unroll 1
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+        int n = 0;
+#pragma unroll
+        for (int m = 0; m < M; ++m) n += __builtin_popcountll(__ballot(o[m] >= (at | bit)));
+        if (n >= k) at |= bit;
     }
     at = max(at, 0x007fffffu);  // -inf
     return __uint_as_float(at & 0x80000000u ? at ^ 0x80000000u : ~at);
@@ -345,7 +382,7 @@ template <int DT, bool TOP, bool TOK, bool HELD>
 __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     using E = LpElem<DT>;
     constexpr int N = E::N, U = kLpUnroll;
-    __shared__ double places[4][64];
+    __shared__ double places[4][HELD ? kLpPlaces : 64];
     const int w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
     if (w >= a.R * a.S) return;
     const int r = w / a.S, s = w - r * a.S;
@@ -431,23 +468,28 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     };
     const int64_t at = (int64_t)r * a.S + s;
     if constexpr (HELD) {
-        float x[U][N], vm[U], most = -INFINITY;
+        float x[U][N], vm[H * U], most[1] = {-INFINITY};
+#pragma unroll
+        for (int v = 0; v < H * U; ++v) vm[v] = -INFINITY;
 #pragma unroll
         for (int t = 0; t < H; ++t) {
             if (64 * U * t >= nv) break;
             unpack(64 * U * t, held[t], x);
-            most = fmaxf(most, take(64 * U * t, x, vm));
+            float tv[U];
+            most[0] = fmaxf(most[0], take(64 * U * t, x, tv));
+#pragma unroll
+            for (int u = 0; u < U; ++u) vm[U * t + u] = fmaxf(-INFINITY, tv[u]);
         }
-        // k lanes' maxima reach the k-th of them: nothing below it is among the k first. What reaches it, usually little
-        // more than k, is packed into the queue's places.
-        const float least = lp_kth(most, a.k);
-        if (least == -INFINITY) queue.n = 65;  // also logits of -inf, whose difference has no sign
+        // k lanes' maxima reach the k-th of them: nothing below it is among the k first. What reaches it is packed into the
+        // queue's places: some 64 ln(64 / (64 - k)) logits; beyond k = 32, of the vectors' maxima, little more than k.
+        const float least = a.k <= 32 ? lp_kth(most, a.k) : lp_kth(vm, a.k);
+        if (least == -INFINITY) queue.n = kLpPlaces + 1;  // also logits of -inf, whose difference has no sign
         LpList elems;
         auto pack = [&](bool in, float v, int j) {
             const uint64_t go = __ballot(in);
             if (go) {
                 const int to = queue.place(go);
-                if (in && to < 64) queue.q[to] = lp_key(v, j);
+                if (in && to < kLpPlaces) queue.q[to] = lp_key(v, j);
                 queue.n += __builtin_popcountll(go);
             }
         };
@@ -457,7 +499,7 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
         }
 #pragma unroll
         for (int t = 0; t < H; ++t) {
-            if (64 * U * t >= nv || queue.n > 64) break;
+            if (64 * U * t >= nv || queue.n > kLpPlaces) break;
             unpack(64 * U * t, held[t], x);
             // which of the lane's U N logits reach it, the first at the top: the differences' signs, two instructions a logit (a
             // NaN's sign may be either: its key is that of no entry)
@@ -469,13 +511,15 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
             mine = ~mine << (32 - U * N);
             const int there = (nv - 64 * U * t - lane + 63) / 64 * N;  // the lane's logits up to the chunk's end
             if (there < U * N) mine &= there > 0 ? ~(0xffffffffu >> there) : 0u;
-            while (queue.n <= 64 && __any(mine)) {
+            while (queue.n <= kLpPlaces && __any(mine)) {
                 const int p = __builtin_clz(mine | 1u), j = v0 + (64 * (U * t + p / N) + lane) * N + p % N;
                 pack(mine != 0, E::pick(held[t], p), j);
                 mine &= ~(0x80000000u >> p);
             }
         }
-        if (queue.n > 64) {  // many equal ones, or the greatest in few lanes: again, a full queue's at a time, from memory
+        if (queue.n <= kLpPlaces) {
+            elems.v = queue.n > 64 ? lp_order<kLpPlaces>(queue.q, queue.n) : lp_order<64>(queue.q, queue.n);
+        } else {  // many equal ones, or the greatest in few lanes: again, a full queue's at a time, from memory
             queue.n = 0;
             uint4 w = make_uint4(E::bits(edge_x), 0, 0, 0);
             int j = edge, n = 1;
@@ -493,8 +537,8 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
                 j = b + lane < nv ? v0 + (b + lane) * N : -1;
                 if (j >= 0) w = vec[b + lane];
             }
+            queue.flush(elems, a.k);
         }
-        queue.flush(elems, a.k);
         if (lane < a.k) a.list[at * a.k + lane] = elems.v;
     } else {
         LpList groups;
@@ -580,6 +624,7 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     const double* list = a.list + (at + lane) * a.k;
     auto fetch = [&](int i) { return lane < a.S && i < a.k ? list[i] : 0.; };
     double c0 = fetch(0), c1 = fetch(1), c2 = fetch(2);
+    auto whole = [&](int i) { return lane < a.k && i < a.S ? a.list[(at + i) * a.k + lane] : 0.; };
     LpSums sum;
     sum.m = p.m, sum.z = p.z, sum.t = p.t;
     sum.join();
@@ -601,17 +646,29 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     // no front can.
     LpList top;
     LpQueue queue(places[threadIdx.x >> 6]);
-    queue.push(__ballot(c0 > 0.), c0, top, a.k);
-    queue.flush(top, a.k);
+    if (a.S > kLpMergeLists) {
+        queue.push(__ballot(c0 > 0.), c0, top, a.k);
+        queue.flush(top, a.k);
 #pragma unroll 1
-    for (int i = 1; i < a.k; ++i) {
-        const uint64_t in = __ballot(c1 > top.last(a.k));
-        if (!in) break;
-        queue.push(in, c1, top, a.k);
-        c1 = c2;
-        c2 = fetch(i + 2);
+        for (int i = 1; i < a.k; ++i) {
+            const uint64_t in = __ballot(c1 > top.last(a.k));
+            if (!in) break;
+            queue.push(in, c1, top, a.k);
+            c1 = c2;
+            c2 = fetch(i + 2);
+        }
+        queue.flush(top, a.k);
+    } else {
+        // few lists go deep: merged one after the other
+        top.v = whole(0);
+        double next = whole(1);
+#pragma unroll 1
+        for (int i = 1; i < a.S; ++i) {
+            const double c = next;
+            next = whole(i + 1);
+            top.merge(c);
+        }
     }
-    queue.flush(top, a.k);
     if (lane < a.k) {
         const bool in = top.v > 0.;  // no: fewer than k logits of the row are numbers
         a.top_i[(int64_t)r * a.k + lane] = in ? lp_index(top.v) : -1;
@@ -660,8 +717,7 @@ int wf_token_logprobs(const void* logits, int dtype, int64_t ld, int R, int V, c
     WF_REQUIRE(!tokens || (logprobs && ranks), "token_logprobs: null logprobs / ranks");
     WF_REQUIRE(top_k == 0 || (top_ids && top_logprobs), "token_logprobs: null top_ids / top_logprobs");
     const int S = lp_splits(R, V), chunk = (int)((((int64_t)V + S - 1) / S + 31) / 32 * 32);
-    // k past 32: what reaches the k-th of 64 maxima is 64 ln(64 / (64 - k)) logits, more than a queue's places
-    const bool held = top_k <= 32 && chunk <= kLpHeld * 64 * kLpUnroll * (dtype == WF_F32 ? 4 : 8);
+    const bool held = chunk <= kLpHeld * 64 * kLpUnroll * (dtype == WF_F32 ? 4 : 8);
     WF_REQUIRE((int64_t)R * S <= 4 * kMaxWgs256, "token_logprobs: too many rows (%d)", R);
     LpPart* part = reinterpret_cast<LpPart*>(ws);
     LpArgs a{logits, ld, R, V, S, chunk, tokens, tokens64, top_k, part, reinterpret_cast<double*>(part + (int64_t)R * S), logprobs, entropy, top_logprobs, ranks, top_ids};
