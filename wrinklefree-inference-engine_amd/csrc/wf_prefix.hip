@@ -385,8 +385,8 @@ __device__ __forceinline__ void pf_run(const PfArgs& a, void* lds, int h, int z,
 }
 
 template <int KVQ, int QDT, int MT>
-__device__ void pf_prefix(const PfArgs& a, void* lds, int x, int tile) {
-    if (x >= a.Hkv * a.NP) return;
+__device__ void pf_prefix(const PfArgs& a, void* lds, int x, int tile, int turn, int turns) {
+    if (x >= a.Hkv * a.NP) return;  // turn of turns: which of the tile's runs are this workgroup's
     const int h = x % a.Hkv, z = x / a.Hkv, lane = threadIdx.x & 63;
     const int64_t r0 = (int64_t)tile * MT, r1 = min(r0 + MT, (int64_t)a.B * a.G);
     const int b0 = (int)(r0 / a.G), b1 = (int)((r1 - 1) / a.G);  // sequences of the tile: at most MT <= 32
@@ -404,6 +404,11 @@ __device__ void pf_prefix(const PfArgs& a, void* lds, int x, int tile) {
         const int P = __builtin_amdgcn_readlane(me.P, i), owner = __builtin_amdgcn_readlane(me.owner, i);
         const int tiles = pf_tiles(P), per = pf_per(tiles, a.NP, kPfMinTiles);
         const int k0 = z * per, k1 = min(k0 + per, tiles);
+        if (turn != 0) {  // another workgroup's run
+            --turn;
+            continue;
+        }
+        turn = turns - 1;
         if (k0 >= k1) continue;  // the whole workgroup
         const int64_t ra = max(r0, (int64_t)(b0 + i) * a.G), rb = min(r1, (int64_t)(b0 + j) * a.G);  // its rows
         if constexpr (MT > 16)
@@ -449,12 +454,13 @@ __device__ void pf_suffix(const PfArgs& a, void* lds, int z, int hc, int b) {
 template <int KVQ, int QDT, int MT>
 constexpr int kPfWgs = MT == 32 && PfType<KVQ, QDT>::kTerms > 1 ? 1 : 2;  // a CU: a q of several terms takes the registers
 template <int KVQ, int QDT, int MT>
-__global__ __launch_bounds__(256, (kPfWgs<KVQ, QDT, MT>)) void k_shared_prefix(PfArgs a, int np) {
+__global__ __launch_bounds__(256, (kPfWgs<KVQ, QDT, MT>)) void k_shared_prefix(PfArgs a, int np, int turns) {
     __shared__ PfShared<MT> sm;
     int x = blockIdx.x;
     if (x < np) {
         const int w = (a.Hkv * a.NP + 7) / 8 * 8;
-        pf_prefix<KVQ, QDT, MT>(a, &sm, x % w, x / w);
+        const int tile = x / w / turns;
+        pf_prefix<KVQ, QDT, MT>(a, &sm, x % w, tile, x / w - tile * turns, turns);
         return;
     }
     x -= np;
@@ -521,6 +527,7 @@ __global__ __launch_bounds__(256) void k_prefix_join(PfArgs a, int odt) {
 
 struct PfPlan {
     int MT, NP, NS;  // rows of a prefix workgroup, splits
+    int turns;       // workgroups of a row tile and range, which take its runs in turn
     int64_t np, ns;  // workgroups
 };
 // Launch shape from what the host knows: rows, kv heads and the table's width (an upper bound of every length).
@@ -534,7 +541,10 @@ static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
     // workgroup, whose time is HBM's: 32768 shared keys 102 us, 118 with two.
     p.NP = clamp(256 / (tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
     p.NS = clamp(512 / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);
-    p.np = B > 1 ? ((int64_t)Hkv * p.NP + 7) / 8 * 8 * tiles : 0;  // one sequence shares nothing
+    // runs of a tile on workgroups of their own while there are CUs for them (half of them where one workgroup fills a CU and the
+    // suffixes need the others): 30 sequences in 4 groups 27 -> 16 us, 19 in 8 20 -> 16
+    p.turns = (int)max((int64_t)1, min((dt == DT_BF16 ? 256 : 128) / (tiles * Hkv * p.NP), (int64_t)min(B / 2, 8)));
+    p.np = B > 1 ? ((int64_t)Hkv * p.NP + 7) / 8 * 8 * tiles * p.turns : 0;  // one sequence shares nothing
     p.ns = p.NS * Hkv * groups * B;
     return p;
 }
@@ -542,8 +552,8 @@ static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
 template <int KVQ, int QDT>
 static void pf_launch(const PfArgs& a, const PfPlan& p, int odt, hipStream_t st) {
     const dim3 grid((unsigned)(p.np + p.ns)), block(256);
-    if (p.MT == 16) hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 16>), grid, block, 0, st, a, (int)p.np);
-    else hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 32>), grid, block, 0, st, a, (int)p.np);
+    if (p.MT == 16) hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 16>), grid, block, 0, st, a, (int)p.np, p.turns);
+    else hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 32>), grid, block, 0, st, a, (int)p.np, p.turns);
     hipLaunchKernelGGL(k_prefix_join, dim3((unsigned)(((int64_t)a.B * a.Hq + 3) / 4)), block, 0, st, a, odt);
 }
 
