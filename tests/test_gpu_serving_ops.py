@@ -544,3 +544,27 @@ def test_two_graphs_of_each_operator_replayed_in_turn():
                 assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(out, w))
             call(0)  # the program's own work in between
             torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim,rdim", [(80, 80), (96, 58), (128, 40), (67, 66), (24, 22)])
+def test_rotary_off_any_alignment(dim, rdim, dtype):
+    """Heads that begin at any element, odd strides: the same bits as from contiguous rows, in place too."""
+    from wfamd import ops
+    g = torch.Generator("cuda").manual_seed(dim)
+    base = torch.randn(40 * (5 * dim + 9) + 8, generator=g, device="cuda").to(DT[dtype])
+    pos = torch.randint(0, 5000, (40,), generator=g, device="cuda")
+    freqs, _ = ops.rotary_frequencies(rdim)
+    for first, th, hh in ((1, 5 * dim + 9, dim + 1), (3, 5 * dim + 1, dim), (0, 5 * dim + 8, dim + 2)):
+        for inter in (False, True):
+            x = base.clone()
+            q, k = x.as_strided((40, 3, dim), (th, hh, 1), first), x.as_strided((40, 1, dim), (th, hh, 1), first + 3 * hh)
+            before = x.clone()
+            want = ops.rotary_embed(q.contiguous(), k.contiguous(), pos, freqs, interleaved=inter)
+            got = ops.rotary_embed(q, k, pos, freqs, interleaved=inter)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(x, before)
+            ops.rotary_embed(q, k, pos, freqs, interleaved=inter, inplace=True)
+            assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+            q.copy_(before.as_strided(q.shape, q.stride(), first))
+            k.copy_(before.as_strided(k.shape, k.stride(), first + 3 * hh))
+            assert torch.equal(x, before)  # nothing beside the heads was written

@@ -8,11 +8,12 @@
 // in [-1/2, 1/2] goes to 32 bits (2^-25 of a half turn) and to sincospif. x is widened to 32 bits and each
 // result rounded once. A call reads and writes every element once and is bound by that.
 //
-// A workgroup takes kRopeTokens tokens (one in short calls): its threads first put the tokens' cos and sin
+// A workgroup takes four tokens (one in short calls): its threads first put the tokens' cos and sin
 // in LDS, one sincos per (token, pair) for all heads, then walk the heads with two 16-byte loads and
-// stores an item (VEC pairs). VEC = 1 takes any stride, alignment and r.
+// stores an item, whatever the strides, alignment and r; what r and D leave over goes one by one.
 // Measured: 16384 tokens, 20 + 5 heads of 128, bf16: 45 us, 4.65 TB/s (a large copy: 4.90); 128 tokens 3.7 us on the
-// device, latencies; 4097 tokens, 8 + 2 heads of 96, f32, interleaved 9.3 us.
+// device, latencies; 4097 tokens, 8 + 2 heads of 96, f32, interleaved 9.3 us; 10746
+// tokens, 16 heads of 128 of which 58 turn, bf16: 33 us (76 element by element), of 80 with 40: 19 us (50).
 #include "wf_common.h"
 #include "wf_device.h"
 
@@ -54,15 +55,21 @@ struct RopeElem<DT_F16> {
     static __device__ __forceinline__ T down(float v) { return f2h(v); }
 };
 
-template <class T, int N>
-struct __attribute__((aligned(sizeof(T) * N))) RopeVec {
+// 16 bytes of a head, aligned as its elements are (global memory takes such accesses)
+template <class T>
+struct RopeVec {
+    static constexpr int N = 16 / sizeof(T);
     T v[N];
+    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(v, p, 16); }
+    __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, v, 16); }
 };
 
-template <int DT, int VEC, bool INTER, int TOK>
+template <int DT, bool INTER, int TOK>
 __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs a) {
     using E = RopeElem<DT>;
-    using V = RopeVec<typename E::T, VEC>;
+    using T = typename E::T;
+    using V = RopeVec<T>;
+    constexpr int N = V::N;
     __shared__ float2 cs[TOK][kRopeMaxDim / 2];
     const int half = a.r >> 1, t0 = blockIdx.x * TOK, nt = min(TOK, a.T - t0);
     for (int i = threadIdx.x; i < nt * half; i += kRopeThreads) {
@@ -74,53 +81,65 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs a) {
         cs[t][j] = make_float2(c * a.scale, s * a.scale);
     }
     __syncthreads();
-    // items of a head: VEC pairs each, then VEC passing dims each
-    const int np = half / VEC, per = np + (a.D - a.r) / VEC, HT = a.H[0] + a.H[1];
+    auto turn = [](T x1, T x2, float2 k, T& y1, T& y2) {
+        const float u = E::up(x1), v = E::up(x2);
+        y1 = E::down(fmaf(u, k.x, -(v * k.y)));
+        y2 = E::down(fmaf(v, k.x, u * k.y));
+    };
+    // items of a head: N pairs each, then N passing dims each, then what is left of both one by one
+    const int pairs = half / N, wide = pairs + (a.D - a.r) / N, ends = wide + half % N, per = ends + (a.D - a.r) % N, HT = a.H[0] + a.H[1];
     for (int i = threadIdx.x; i < nt * HT * per; i += kRopeThreads) {
         const int c = i % per, th = i / per, t = th / HT;
         int h = th - t * HT;
         const int w = h >= a.H[0];
         if (w) h -= a.H[0];
-        const typename E::T* x = (const typename E::T*)a.x[w] + (t0 + t) * a.xt[w] + h * a.xh[w];
-        typename E::T* y = (typename E::T*)a.y[w] + (t0 + t) * a.yt[w] + h * a.yh[w];
-        if (c >= np) {
-            const int d = a.r + (c - np) * VEC;
-            *reinterpret_cast<V*>(y + d) = *reinterpret_cast<const V*>(x + d);
-            continue;
-        }
-        // the item's two vectors: dims [d0, +VEC) and [d1, +VEC)
-        const int d0 = INTER ? 2 * VEC * c : VEC * c, d1 = INTER ? d0 + VEC : d0 + half;
-        const V u = *reinterpret_cast<const V*>(x + d0), v = *reinterpret_cast<const V*>(x + d1);
-        V yu, yv;
+        const T* x = (const T*)a.x[w] + (t0 + t) * a.xt[w] + h * a.xh[w];
+        T* y = (T*)a.y[w] + (t0 + t) * a.yt[w] + h * a.yh[w];
+        if (c < pairs) {
+            // the item's two vectors: dims [d0, +N) and [d1, +N)
+            const int d0 = INTER ? 2 * N * c : N * c, d1 = INTER ? d0 + N : d0 + half;
+            V u, v, yu, yv;
+            u.load(x + d0);
+            v.load(x + d1);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float2 k = cs[t][VEC * c + e];
-            // element 2e of the 2 VEC in order (interleaved) or (u[e], v[e])
-            const float x1 = E::up(INTER ? (2 * e < VEC ? u.v[2 * e] : v.v[2 * e - VEC]) : u.v[e]);
-            const float x2 = E::up(INTER ? (2 * e + 1 < VEC ? u.v[2 * e + 1] : v.v[2 * e + 1 - VEC]) : v.v[e]);
-            const typename E::T y1 = E::down(fmaf(x1, k.x, -(x2 * k.y))), y2 = E::down(fmaf(x2, k.x, x1 * k.y));
-            if constexpr (INTER) {
-                (2 * e < VEC ? yu.v[2 * e] : yv.v[2 * e - VEC]) = y1;
-                (2 * e + 1 < VEC ? yu.v[2 * e + 1] : yv.v[2 * e + 1 - VEC]) = y2;
-            } else {
-                yu.v[e] = y1;
-                yv.v[e] = y2;
+            for (int e = 0; e < N; ++e) {
+                const float2 k = cs[t][N * c + e];
+                if constexpr (INTER) {  // element 2 e of the 2 N in order
+                    V &from = 2 * e < N ? u : v, &to = 2 * e < N ? yu : yv;
+                    turn(from.v[2 * e % N], from.v[2 * e % N + 1], k, to.v[2 * e % N], to.v[2 * e % N + 1]);
+                } else {
+                    turn(u.v[e], v.v[e], k, yu.v[e], yv.v[e]);
+                }
             }
+            yu.store(y + d0);
+            yv.store(y + d1);
+        } else if (c < wide) {
+            const int d = a.r + (c - pairs) * N;
+            V u;
+            u.load(x + d);
+            u.store(y + d);
+        } else if (c < ends) {
+            const int j = pairs * N + c - wide, d0 = INTER ? 2 * j : j, d1 = INTER ? d0 + 1 : d0 + half;
+            T y1, y2;
+            turn(x[d0], x[d1], cs[t][j], y1, y2);
+            y[d0] = y1;
+            y[d1] = y2;
+        } else {
+            const int d = a.D - (per - c);
+            y[d] = x[d];
         }
-        *reinterpret_cast<V*>(y + d0) = yu;
-        *reinterpret_cast<V*>(y + d1) = yv;
     }
 }
 
-template <int DT, int VEC>
+template <int DT>
 static void rope_launch(const RopeArgs& a, bool inter, hipStream_t st) {
     // four tokens a workgroup share the sincos phase's latency; short calls take one, for more workgroups
     const bool wide = a.T >= 2048;
     const dim3 grid(wide ? (a.T + 3) / 4 : a.T), block(kRopeThreads);
-    if (wide && inter) hipLaunchKernelGGL((k_rope<DT, VEC, true, 4>), grid, block, 0, st, a);
-    else if (wide) hipLaunchKernelGGL((k_rope<DT, VEC, false, 4>), grid, block, 0, st, a);
-    else if (inter) hipLaunchKernelGGL((k_rope<DT, VEC, true, 1>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((k_rope<DT, VEC, false, 1>), grid, block, 0, st, a);
+    if (wide && inter) hipLaunchKernelGGL((k_rope<DT, true, 4>), grid, block, 0, st, a);
+    else if (wide) hipLaunchKernelGGL((k_rope<DT, false, 4>), grid, block, 0, st, a);
+    else if (inter) hipLaunchKernelGGL((k_rope<DT, true, 1>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((k_rope<DT, false, 1>), grid, block, 0, st, a);
 }
 
 }  // namespace wf
@@ -142,16 +161,10 @@ int wf_rotary_embed(const void* q, int64_t q_st, int64_t q_sh, int Hq, const voi
     WF_REQUIRE(positions && freqs && (Hq == 0 || (q && q_out)) && (Hk == 0 || (k && k_out)), "rotary_embed: null pointer");
     RopeArgs a{{q, k}, {q_out, k_out}, {q_st, k_st}, {q_sh, k_sh}, {qo_st, ko_st}, {qo_sh, ko_sh}, {Hq, Hk}, positions, positions64,
                freqs, T, D, rotary_dim, scale};
-    const int vec = dtype == WF_F32 ? 4 : 8;
-    bool wide = rotary_dim % (2 * vec) == 0 && D % vec == 0;
-    for (int w = 0; w < 2; ++w)
-        if (a.H[w])
-            wide = wide && aligned16(a.x[w]) && aligned16(a.y[w]) && a.xt[w] % vec == 0 && a.xh[w] % vec == 0 && a.yt[w] % vec == 0 &&
-                   a.yh[w] % vec == 0;
     hipStream_t st = as_stream(stream);
-    if (dtype == WF_F32) wide ? rope_launch<DT_F32, 4>(a, interleaved, st) : rope_launch<DT_F32, 1>(a, interleaved, st);
-    else if (dtype == WF_BF16) wide ? rope_launch<DT_BF16, 8>(a, interleaved, st) : rope_launch<DT_BF16, 1>(a, interleaved, st);
-    else wide ? rope_launch<DT_F16, 8>(a, interleaved, st) : rope_launch<DT_F16, 1>(a, interleaved, st);
+    if (dtype == WF_F32) rope_launch<DT_F32>(a, interleaved, st);
+    else if (dtype == WF_BF16) rope_launch<DT_BF16>(a, interleaved, st);
+    else rope_launch<DT_F16>(a, interleaved, st);
     return check_launch("rotary_embed");
 }
 
