@@ -85,6 +85,9 @@ __device__ __forceinline__ PfSeq pf_seq(const PfArgs& a, int b) {
 __device__ __forceinline__ bool pf_shared(const PfArgs& a, int b, const PfSeq& s) {
     return s.same(pf_seq(a, b - 1)) || s.same(pf_seq(a, b + 1));
 }
+// Workgroups from one row tile to the next: a workgroup a (head, range), rounded up to 8 so that the row tiles of one meet
+// in one XCD's L2; fewer than 8 as they are, spread over the XCDs.
+__host__ __device__ __forceinline__ int64_t pf_width(int64_t Hkv, int NP) { return Hkv * NP < 8 ? Hkv * NP : (Hkv * NP + 7) / 8 * 8; }
 // tiles of one of `splits` ranges, and how many ranges hold something
 __device__ __forceinline__ int pf_per(int tiles, int splits, int least) { return max((tiles + splits - 1) / splits, least); }
 __device__ __forceinline__ int pf_tiles(int keys) { return (keys + kPfPage - 1) / kPfPage; }
@@ -452,13 +455,11 @@ __device__ void pf_suffix(const PfArgs& a, void* lds, int z, int hc, int b) {
 // The first np workgroups the prefixes, in row tiles of MT; the others the other keys: the one part waits for the
 // matrix cores and L1, the other for HBM.
 template <int KVQ, int QDT, int MT>
-constexpr int kPfWgs = MT == 32 && PfType<KVQ, QDT>::kTerms > 1 ? 1 : 2;  // a CU: a q of several terms takes the registers
-template <int KVQ, int QDT, int MT>
-__global__ __launch_bounds__(256, (kPfWgs<KVQ, QDT, MT>)) void k_shared_prefix(PfArgs a, int np, int turns) {
+__global__ __launch_bounds__(256, 2) void k_shared_prefix(PfArgs a, int np, int turns) {
     __shared__ PfShared<MT> sm;
     int x = blockIdx.x;
     if (x < np) {
-        const int w = (a.Hkv * a.NP + 7) / 8 * 8;
+        const int w = (int)pf_width(a.Hkv, a.NP);
         const int tile = x / w / turns;
         pf_prefix<KVQ, QDT, MT>(a, &sm, x % w, tile, x / w - tile * turns, turns);
         return;
@@ -530,21 +531,23 @@ struct PfPlan {
     int turns;       // workgroups of a row tile and range, which take its runs in turn
     int64_t np, ns;  // workgroups
 };
-// Launch shape from what the host knows: rows, kv heads and the table's width (an upper bound of every length).
-static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
+// Launch shape from what the host knows: whether q is one term (at most as many ranges where it is not), rows, kv heads and the table's width (an upper bound of every length).
+static PfPlan pf_plan(bool one, int B, int Hq, int Hkv, int cols) {
     const int64_t rows = (int64_t)B * (Hq / Hkv), groups = (Hq / Hkv + 15) / 16;
     PfPlan p;
-    p.MT = rows <= 16 ? 16 : 32;
+    // 32 rows of a q of several terms would leave one workgroup a CU its registers: 4096 shared keys 48 us (f32) and 42 (f16), 36 and
+    // 33 with 16 rows, short prefixes 33 -> 23
+    p.MT = rows <= 16 || !one ? 16 : 32;
     const int64_t tiles = (rows + p.MT - 1) / p.MT;
     auto clamp = [](int64_t v, int64_t hi) { return (int)max((int64_t)1, min(min(v, hi), (int64_t)kPfMaxRecords)); };
     // prefix ranges: one workgroup a CU. A second one reads no faster (L1, below), and its place goes to a suffix
     // workgroup, whose time is HBM's: 32768 shared keys 102 us, 118 with two.
     p.NP = clamp(256 / (tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
     p.NS = clamp(512 / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);
-    // runs of a tile on workgroups of their own while there are CUs for them (half of them where one workgroup fills a CU and the
-    // suffixes need the others): 30 sequences in 4 groups 27 -> 16 us, 19 in 8 20 -> 16
-    p.turns = (int)max((int64_t)1, min((dt == DT_BF16 ? 256 : 128) / (tiles * Hkv * p.NP), (int64_t)min(B / 2, 8)));
-    p.np = B > 1 ? ((int64_t)Hkv * p.NP + 7) / 8 * 8 * tiles * p.turns : 0;  // one sequence shares nothing
+    // runs of a tile on workgroups of their own while there are CUs for them: 30 sequences in 4 groups 27 -> 16 us, 19 in 8 20 -> 16
+    const int64_t w = pf_width(Hkv, p.NP) * tiles;
+    p.turns = (int)max((int64_t)1, min(256 / w, (int64_t)min(B / 2, 8)));
+    p.np = B > 1 ? w * p.turns : 0;  // one sequence shares nothing
     p.ns = p.NS * Hkv * groups * B;
     return p;
 }
@@ -552,8 +555,9 @@ static PfPlan pf_plan(int dt, int B, int Hq, int Hkv, int cols) {
 template <int KVQ, int QDT>
 static void pf_launch(const PfArgs& a, const PfPlan& p, int odt, hipStream_t st) {
     const dim3 grid((unsigned)(p.np + p.ns)), block(256);
+    constexpr int kWide = PfType<KVQ, QDT>::kTerms == 1 ? 32 : 16;
     if (p.MT == 16) hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 16>), grid, block, 0, st, a, (int)p.np, p.turns);
-    else hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, 32>), grid, block, 0, st, a, (int)p.np, p.turns);
+    else hipLaunchKernelGGL((k_shared_prefix<KVQ, QDT, kWide>), grid, block, 0, st, a, (int)p.np, p.turns);
     hipLaunchKernelGGL(k_prefix_join, dim3((unsigned)(((int64_t)a.B * a.Hq + 3) / 4)), block, 0, st, a, odt);
 }
 
@@ -572,7 +576,7 @@ extern "C" {
 
 int64_t wf_shared_prefix_attention_ws_bytes(int dtype, int B, int Hq, int Hkv, int max_blocks) {
     if (B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || max_blocks <= 0) return 0;
-    const PfPlan p = pf_plan(dtype, B, Hq, Hkv, max_blocks);
+    const PfPlan p = pf_plan(dtype != WF_F32, B, Hq, Hkv, max_blocks);  // f16: one term over some pools
     return (int64_t)B * Hq * (p.NP + p.NS) * (int64_t)(sizeof(float2) + 4 * kPfDim);
 }
 
@@ -599,7 +603,7 @@ int wf_shared_prefix_attention(const void* q, int dtype, int64_t q_sb, int64_t q
     WF_REQUIRE(q && k_pool && v_pool && page_table && seq_lens && prefix_rows && prefix_lens && out && ws,
                "shared_prefix_attention: null pointer");
     WF_REQUIRE(aligned16(k_pool) && aligned16(v_pool) && aligned16(ws), "shared_prefix_attention: pools and workspace must be 16-byte aligned");
-    const PfPlan p = pf_plan(dtype, B, Hq, Hkv, max_blocks);
+    const PfPlan p = pf_plan(dtype == WF_BF16 || (dtype == WF_F16 && kv_quant != WF_KV_BF16), B, Hq, Hkv, max_blocks);
     WF_REQUIRE(p.np + p.ns <= kMaxWgs256 && (int64_t)B * Hq <= 4 * kMaxWgs256, "shared_prefix_attention: batch %d with heads %d / %d too many", B, Hq,
                Hkv);
     const int64_t recs = (int64_t)B * Hq * (p.NP + p.NS);
