@@ -676,11 +676,13 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     }
 }
 
-// Chunks a row: enough waves to fill the device (4096; 6144 where that makes a row's chunks short enough for registers: 404
-// rows of 55653 37 -> 30 us with 20 alternatives; 8192 waves for it cost 1024 rows of 32000 27 -> 30), but no chunk
-// under a tile of a wave.
+// Chunks a row: enough waves to fill the device, 4096 at once, but no chunk under a tile of a wave. More of them where
+// that makes the chunks short enough for registers, up to 6144 (404 rows of 55653 with 20 alternatives 37 -> 30 us), or up
+// to 12288 where 4096 do not come out even and leave a second round anyway (203 rows of 143659 41 -> 31; where they do, 512
+// rows of 64000 would go 33 -> 36).
 static int lp_splits(int R, int V) {
-    const int64_t held = ((int64_t)V + 4095) / 4096, want = max((4096 + (int64_t)R - 1) / R, R * held <= 6144 ? held : 0);
+    const int64_t even = (4096 + (int64_t)R - 1) / R, held = ((int64_t)V + 4095) / 4096;
+    const int64_t want = R * held <= (R * even > 4096 ? 12288 : 6144) ? max(even, held) : even;
     return (int)max((int64_t)1, min(min(want, ((int64_t)V + 2047) / 2048), (int64_t)kLpMaxSplits));
 }
 
