@@ -10,14 +10,15 @@
 // A second launch, a wave per row, joins the chunks' sums and sorted lists.
 //
 // The top k without a data-dependent buffer, from maxima that the sums need anyway:
-//   short chunks (two tiles, few rows) stay in registers. The k-th greatest of the 64 lanes' maxima bounds the k-th
-//     logit from below; what reaches it (some 64 ln(64 / (64 - k)) logits) is packed by ballots and ordered once.
+//   short chunks (4096 logits, few rows) stay in registers. The k-th greatest of the 64 lanes' maxima bounds the k-th
+//     logit from below; what reaches it (some 64 ln(64 / (64 - k)) logits; from k = 33 on the vectors'
+//     maxima are taken instead) is packed by ballots and ordered once.
 //   long chunks are cut into groups of four neighbouring 16-byte vectors (the four lanes of a quad), each group's max two
 //     DPP steps more. The k first groups, by (max, lower group first), hold the chunk's k first elements: an
 //     element of a later group is preceded by the maxima of k groups, each greater, or equal and further left. The
 //     wave keeps the k best groups sorted across its lanes and reads just those again at the end. k <= 64 is the wave's width.
 // Measured, vocabulary 128256 in bf16: 2048 rows with 5 alternatives 119 us, 4.4 TB/s (97 us, 5.4 TB/s, without any); 128 rows
-// with 20: 17.5 us and 5 of the join (the reading and summing alone 11.7); one row 7 + 4 us, latencies.
+// with 20: 16 us and 5 of the join (the reading and summing alone 11.7); one row 6 + 5 us, latencies.
 #include "wf_common.h"
 #include "wf_device.h"
 
@@ -25,7 +26,7 @@ namespace wf {
 
 constexpr int kLpMaxTop = 64;
 constexpr int kLpUnroll = 4;        // 16-byte vectors a lane holds of a tile
-constexpr int kLpHeld = 2;          // tiles of a chunk that stay in registers
+constexpr int kLpHeld = 4096;       // logits of a chunk that stay in registers: 2 tiles of 16 bits, 4 of 32
 constexpr int kLpPlaces = 128;      // places for what may be among their alternatives
 constexpr int kLpMergeLists = 16;   // chunks of a row up to which the join merges whole lists
 constexpr int kLpMaxSplits = 64;    // chunks of a row: a lane each in the join
@@ -377,7 +378,7 @@ __device__ __forceinline__ float lp_kth(const float (&v)[M], int k) {
     return __uint_as_float(at & 0x80000000u ? at ^ 0x80000000u : ~at);
 }
 
-// HELD (TOP): the chunk has at most kLpHeld tiles, which stay in registers.
+// HELD (TOP): the chunk has at most kLpHeld logits, which stay in registers.
 template <int DT, bool TOP, bool TOK, bool HELD>
 __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     using E = LpElem<DT>;
@@ -402,7 +403,7 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
     };
     // Loads return in order: the first tile, the token's logit, what is left of the chunk, so that nothing waits for more than
     // it needs. The token itself comes through the scalar cache.
-    constexpr int H = HELD ? kLpHeld : 1;
+    constexpr int H = HELD ? kLpHeld / (64 * U * N) : 1;
     uint4 held[H][U];
     load(0, held[0]);
     int tok = -1;
@@ -681,7 +682,7 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
 // to 12288 where 4096 do not come out even and leave a second round anyway (203 rows of 143659 41 -> 31; where they do, 512
 // rows of 64000 would go 33 -> 36).
 static int lp_splits(int R, int V) {
-    const int64_t even = (4096 + (int64_t)R - 1) / R, held = ((int64_t)V + 4095) / 4096;
+    const int64_t even = (4096 + (int64_t)R - 1) / R, held = ((int64_t)V + kLpHeld - 1) / kLpHeld;
     const int64_t want = R * held <= (R * even > 4096 ? 12288 : 6144) ? max(even, held) : even;
     return (int)max((int64_t)1, min(min(want, ((int64_t)V + 2047) / 2048), (int64_t)kLpMaxSplits));
 }
@@ -721,7 +722,7 @@ int wf_token_logprobs(const void* logits, int dtype, int64_t ld, int R, int V, c
     WF_REQUIRE(!tokens || (logprobs && ranks), "token_logprobs: null logprobs / ranks");
     WF_REQUIRE(top_k == 0 || (top_ids && top_logprobs), "token_logprobs: null top_ids / top_logprobs");
     const int S = lp_splits(R, V), chunk = (int)((((int64_t)V + S - 1) / S + 31) / 32 * 32);
-    const bool held = chunk <= kLpHeld * 64 * kLpUnroll * (dtype == WF_F32 ? 4 : 8);
+    const bool held = chunk <= kLpHeld;
     WF_REQUIRE((int64_t)R * S <= 4 * kMaxWgs256, "token_logprobs: too many rows (%d)", R);
     LpPart* part = reinterpret_cast<LpPart*>(ws);
     LpArgs a{logits, ld, R, V, S, chunk, tokens, tokens64, top_k, part, reinterpret_cast<double*>(part + (int64_t)R * S), logprobs, entropy, top_logprobs, ranks, top_ids};
