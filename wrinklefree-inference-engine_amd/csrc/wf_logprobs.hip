@@ -17,7 +17,7 @@
 //     DPP steps more. The k first groups, by (max, lower group first), hold the chunk's k first elements: an
 //     element of a later group is preceded by the maxima of k groups, each greater, or equal and further left. The
 //     wave keeps the k best groups sorted across its lanes and reads just those again at the end. k <= 64 is the wave's width.
-// Measured, vocabulary 128256 in bf16: 2048 rows with 5 alternatives 119 us, 4.4 TB/s (97 us, 5.4 TB/s, without any); 128 rows
+// Measured, vocabulary 128256 in bf16: 2048 rows with 5 alternatives 118 us, 4.5 TB/s (109 us, 4.8 TB/s, without any); 128 rows
 // with 20: 16 us and 5 of the join (the reading and summing alone 11.7); one row 6 + 5 us, latencies.
 #include "wf_common.h"
 #include "wf_device.h"
