@@ -40,7 +40,7 @@ typedef float pf_f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPfDim = 128, kPfPage = 32;
 constexpr int kPfMaxRecords = 64;          // splits of each part: a lane each in the join, twice
-constexpr int kPfMinTiles = 12;            // tiles of a prefix range: a record costs its write and read in the join (8: +20% behind 1024 keys)
+constexpr int kPfMinTiles = 4;             // tiles of a prefix range: one a wave at least (12: 64 pairs behind 512 keys 37 us, 33 with 4)
 constexpr int kPfMinSuffix = 8;            // of a suffix range: two a wave
 constexpr float kPfLn2 = 0.69314718055994530942f;
 
