@@ -15,7 +15,7 @@ def _gpu():
     if not torch.cuda.is_available():
         pytest.skip("needs a GPU")
     from wfamd import _lib
-    assert _lib.kernel_available(), "gfx950 kernels must load on the GPU box (no fallback)"
+    assert _lib.kernel_available(), "gfx950 kernels must load (no fallback)"
     torch.cuda.set_device(0)
 
 
