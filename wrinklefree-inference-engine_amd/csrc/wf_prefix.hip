@@ -85,9 +85,6 @@ __device__ __forceinline__ PfSeq pf_seq(const PfArgs& a, int b) {
 __device__ __forceinline__ bool pf_shared(const PfArgs& a, int b, const PfSeq& s) {
     return s.same(pf_seq(a, b - 1)) || s.same(pf_seq(a, b + 1));
 }
-// Workgroups from one row tile to the next: a workgroup a (head, range), rounded up to 8 so that the row tiles of one meet
-// in one XCD's L2; fewer than 8 as they are, spread over the XCDs.
-__host__ __device__ __forceinline__ int64_t pf_width(int64_t Hkv, int NP) { return Hkv * NP < 8 ? Hkv * NP : (Hkv * NP + 7) / 8 * 8; }
 // tiles of one of `splits` ranges, and how many ranges hold something
 __device__ __forceinline__ int pf_per(int tiles, int splits, int least) { return max((tiles + splits - 1) / splits, least); }
 __device__ __forceinline__ int pf_tiles(int keys) { return (keys + kPfPage - 1) / kPfPage; }
@@ -366,9 +363,8 @@ __device__ __forceinline__ void pf_merge(const PfArgs& a, PfShared<W>& sm, const
 }
 
 // ---------------------------------------------------------------------------------------------
-// Shared prefixes. Block (kv head and key range, rounded up to 8, tile of MT rows): the row tiles of one (head, range)
-// are 8 k workgroups apart, so one XCD's L2 serves them all. A tile's rows are taken in runs of sequences with one
-// prefix, in 16 or 32 rows.
+// Shared prefixes. A workgroup per (kv head, key range, tile of MT rows) and turn. A tile's rows are taken in runs of
+// sequences with one prefix, in 16 or 32 rows.
 // ---------------------------------------------------------------------------------------------
 template <int KVQ, int QDT, int W>
 __device__ __forceinline__ void pf_run(const PfArgs& a, void* lds, int h, int z, int64_t ra, int64_t rb, int P, int owner, int k0, int k1) {
@@ -388,9 +384,8 @@ __device__ __forceinline__ void pf_run(const PfArgs& a, void* lds, int h, int z,
 }
 
 template <int KVQ, int QDT, int MT>
-__device__ void pf_prefix(const PfArgs& a, void* lds, int x, int tile, int turn, int turns) {
-    if (x >= a.Hkv * a.NP) return;  // turn of turns: which of the tile's runs are this workgroup's
-    const int h = x % a.Hkv, z = x / a.Hkv, lane = threadIdx.x & 63;
+__device__ void pf_prefix(const PfArgs& a, void* lds, int h, int z, int tile, int turn, int turns) {  // runs turn, turn + turns, .. of the tile
+    const int lane = threadIdx.x & 63;
     const int64_t r0 = (int64_t)tile * MT, r1 = min(r0 + MT, (int64_t)a.B * a.G);
     const int b0 = (int)(r0 / a.G), b1 = (int)((r1 - 1) / a.G);  // sequences of the tile: at most MT <= 32
     // lane i: sequence b0 + i
@@ -459,9 +454,12 @@ __global__ __launch_bounds__(256, 2) void k_shared_prefix(PfArgs a, int np, int 
     __shared__ PfShared<MT> sm;
     int x = blockIdx.x;
     if (x < np) {
-        const int w = (int)pf_width(a.Hkv, a.NP);
-        const int tile = x / w / turns;
-        pf_prefix<KVQ, QDT, MT>(a, &sm, x % w, tile, x / w - tile * turns, turns);
+        // consecutive workgroups go round the 8 XCDs: each takes an eighth of the list (head, range, row tile, turn), so that
+        // the row tiles of one (head, range) meet in one L2, or in two neighbours' (whole groups to an XCD: 160 sequences
+        // of 20 query and 5 kv heads behind 32768 keys 152 us, 115 so)
+        const int tiles = (int)(((int64_t)a.B * a.G + MT - 1) / MT), i = (x & 7) * (np >> 3) + (x >> 3);
+        const int u = i / turns, g = u / tiles, h = g / a.NP;
+        if (h < a.Hkv) pf_prefix<KVQ, QDT, MT>(a, &sm, h, g - h * a.NP, u - g * tiles, i - u * turns, turns);
         return;
     }
     x -= np;
@@ -545,9 +543,9 @@ static PfPlan pf_plan(bool one, int B, int Hq, int Hkv, int cols) {
     p.NP = clamp(256 / (tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
     p.NS = clamp(512 / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);
     // runs of a tile on workgroups of their own while there are CUs for them: 30 sequences in 4 groups 27 -> 16 us, 19 in 8 20 -> 16
-    const int64_t w = pf_width(Hkv, p.NP) * tiles;
+    const int64_t w = (int64_t)Hkv * p.NP * tiles;
     p.turns = (int)max((int64_t)1, min(256 / w, (int64_t)min(B / 2, 8)));
-    p.np = B > 1 ? w * p.turns : 0;  // one sequence shares nothing
+    p.np = B > 1 ? (w * p.turns + 7) / 8 * 8 : 0;  // one sequence shares nothing
     p.ns = p.NS * Hkv * groups * B;
     return p;
 }
