@@ -410,3 +410,18 @@ def test_decoder_reserves_a_batch_and_attends_over_its_pool(kv):
     c = dict(q=q, k_pool=a.k_cache[1], v_pool=a.v_cache[1], page_table=a.page_table, seq_lens=i32(pos), prefix_rows=i32([0] * 16),
              prefix_lens=i32([60] * 16), kv_dtype=kv, k_scale=0.05 if kv != "bf16" else 1.0, v_scale=0.03 if kv != "bf16" else 1.0)
     assert torch.equal(a.shared_prefix_attention(1, q, c["seq_lens"], c["prefix_rows"], c["prefix_lens"]), check(c)[0])
+
+
+@pytest.mark.parametrize("dtype,kv", [("bf16", "bf16"), ("f16", "bf16"), ("f16", "fp8"), ("f32", "int8")])
+@pytest.mark.parametrize("hkv,gq,sizes", [(1, 1, [7, 1, 9, 8, 5]), (4, 4, [3, 2, 2, 1, 2, 4, 2, 3]), (1, 3, [2] * 20), (5, 4, [40, 17, 100]), (2, 1, [33] * 6)])
+def test_runs_of_every_size(hkv, gq, sizes, dtype, kv):
+    """Groups of all sizes next to each other, more of them than a row tile's workgroups, prefixes of several ranges."""
+    b = sum(sizes)
+    rows, plens, lens = [], [], []
+    for i, n in enumerate(sizes):
+        first = len(rows)
+        p = 40 + 67 * (i % 5) + 300 * (i % 2)
+        rows += [first] * n
+        plens += [p] * n
+        lens += [p + (11 * j + 5 * i) % 70 for j in range(n)]
+    check(case(b, hkv, gq, lens, rows, plens, kv, dtype, seed=30 + b))
