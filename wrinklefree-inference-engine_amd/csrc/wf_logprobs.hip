@@ -677,13 +677,13 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     }
 }
 
-// Chunks a row: enough waves to fill the device, 4096 at once, but no chunk under a tile of a wave. More of them where
-// that makes the chunks short enough for registers, up to 6144 (404 rows of 55653 with 20 alternatives 37 -> 30 us), or up
-// to 12288 where 4096 do not come out even and leave a second round anyway (203 rows of 143659 41 -> 31; where they do, 512
-// rows of 64000 would go 33 -> 36).
+// Chunks a row: as many waves as the device holds at once, 4096, or a few less (535 rows of 155893 with 20 alternatives: 7
+// chunks 57 us, 8 leave a second round of 184 waves, 66); more where fewer would leave a seventh of it empty. More also where
+// that makes the chunks short enough for registers, up to 6144 waves (404 rows of 55653 37 -> 30 us), or 12288 where there is
+// a second round anyway. No chunk under a tile of a wave.
 static int lp_splits(int R, int V) {
-    const int64_t even = (4096 + (int64_t)R - 1) / R, held = ((int64_t)V + kLpHeld - 1) / kLpHeld;
-    const int64_t want = R * held <= (R * even > 4096 ? 12288 : 6144) ? max(even, held) : even;
+    const int64_t down = 4096 / (int64_t)R, fit = R * down >= 3500 ? down : (4096 + (int64_t)R - 1) / R;
+    const int64_t held = ((int64_t)V + kLpHeld - 1) / kLpHeld, want = R * held <= (R * fit > 4096 ? 12288 : 6144) ? max(fit, held) : fit;
     return (int)max((int64_t)1, min(min(want, ((int64_t)V + 2047) / 2048), (int64_t)kLpMaxSplits));
 }
 
