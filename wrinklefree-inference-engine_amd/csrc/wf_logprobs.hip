@@ -483,7 +483,8 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
         }
         // k lanes' maxima reach the k-th of them: nothing below it is among the k first. What reaches it is packed into the
         // queue's places: some 64 ln(64 / (64 - k)) logits; beyond k = 32, of the vectors' maxima, little more than k.
-        const float least = a.k <= 32 ? lp_kth(most, a.k) : lp_kth(vm, a.k);
+        float least = a.k <= 32 ? lp_kth(most, a.k) : lp_kth(vm, a.k);
+        if (least == 0.f) least = -0.f;  // the signs below: -0 - 0 has one, and both zeros reach 0; less -0 neither has
         if (least == -INFINITY) queue.n = kLpPlaces + 1;  // also logits of -inf, whose difference has no sign
         LpList elems;
         auto pack = [&](bool in, float v, int j) {
@@ -503,7 +504,7 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
             if (64 * U * t >= nv || queue.n > kLpPlaces) break;
             unpack(64 * U * t, held[t], x);
             // which of the lane's U N logits reach it, the first at the top: the differences' signs, two instructions a logit (a
-            // NaN's sign may be either: its key is that of no entry)
+            // NaN logit's sign may be either: its key is that of no entry)
             uint32_t mine = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u)
