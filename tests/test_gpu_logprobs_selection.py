@@ -1,4 +1,6 @@
-"""token_logprobs' alternatives where their selection can go wrong: zeros of both signs."""
+"""token_logprobs' alternatives where their selection can go wrong: zeros of both signs and +inf."""
+import math
+
 import pytest
 import torch
 
@@ -55,3 +57,22 @@ def test_zeros_of_both_signs_among_negatives(dtype, vocab):
         y = torch.full((1, vocab), -3.0, device="cuda")
         y[0, 1111], y[0, vocab - 40] = -0.0 * sign, 0.0 * sign
         assert check_order(y.to(DT[dtype]), [1111], 2).top_ids.tolist() == [[1111, vocab - 40]]
+
+
+@pytest.mark.parametrize("vocab", [2048, 40011, 300001])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_several_infinities(dtype, vocab):
+    assert (chunk_of(6, vocab) > HELD) == (vocab == 300001)
+    g = torch.Generator("cuda").manual_seed(vocab)
+    x = torch.randn(6, vocab, generator=g, device="cuda").to(DT[dtype])
+    inf, high = math.inf, torch.finfo(DT[dtype]).max
+    x[0, 777] = inf                          # k = 1: the least that can be among them is +inf itself
+    x[1, 9:1900:8] = inf                     # in every lane, more than there are places
+    x[2, 11:2000:80] = inf                   # 25 of them
+    x[3, 1500], x[3, 20], x[3, 1200] = inf, high, high
+    x[4] = inf
+    x[5, 64:96], x[5, 1000:1100] = inf, high  # few lanes; the type's highest value behind them
+    for k in (1, 2, 3, 20, 33, 64):
+        for tokens in ((777, 9, 11, 1500, 0, 64), (0, 17, 2, 20, vocab - 1, 1000), (778, 1897, 1931, 1200, 900, 1099)):
+            p = check_order(x, tokens, k)
+            assert p.logprobs.isnan().all() and p.entropy.isnan().all() and p.top_logprobs.isnan().all()

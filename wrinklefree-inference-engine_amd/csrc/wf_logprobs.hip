@@ -484,7 +484,10 @@ __global__ __launch_bounds__(256) void k_logprobs_part(LpArgs a) {
         // k lanes' maxima reach the k-th of them: nothing below it is among the k first. What reaches it is packed into the
         // queue's places: some 64 ln(64 / (64 - k)) logits; beyond k = 32, of the vectors' maxima, little more than k.
         float least = a.k <= 32 ? lp_kth(most, a.k) : lp_kth(vm, a.k);
-        if (least == 0.f) least = -0.f;  // the signs below: -0 - 0 has one, and both zeros reach 0; less -0 neither has
+        // for the signs below: -0 - 0 has one, and both zeros reach 0; less -0 neither has. inf - inf is a NaN with a sign of its own;
+        // inf less the greatest number is not, and what else that lets in the keys leave behind
+        if (least == 0.f) least = -0.f;
+        least = fminf(least, 0x1.fffffep127f);
         if (least == -INFINITY) queue.n = kLpPlaces + 1;  // also logits of -inf, whose difference has no sign
         LpList elems;
         auto pack = [&](bool in, float v, int j) {
