@@ -1,10 +1,10 @@
-"""token_logprobs' alternatives where their selection can go wrong: zeros of both signs and +inf."""
+"""token_logprobs' alternatives where their selection can go wrong: zeros of both signs, +inf, and chunks too long for registers."""
 import math
 
 import pytest
 import torch
 
-from test_gpu_serving_ops import DT
+from test_gpu_serving_ops import DT, close, logprobs_ref
 
 pytestmark = pytest.mark.gpu
 HELD = 4096  # logits of a chunk that stay in registers
@@ -76,3 +76,101 @@ def test_several_infinities(dtype, vocab):
         for tokens in ((777, 9, 11, 1500, 0, 64), (0, 17, 2, 20, vocab - 1, 1000), (778, 1897, 1931, 1200, 900, 1099)):
             p = check_order(x, tokens, k)
             assert p.logprobs.isnan().all() and p.entropy.isnan().all() and p.top_logprobs.isnan().all()
+
+
+def check_long(x, tokens, k):
+    """Against the definition in 64 bits, in units of u = 2^-24. A chunk of c logits: a lane adds n = c / 64 + 16 terms one after the
+    other, whose exponent is a difference and a product (2 |y|, weighted by 2^y: under 2 (1 + 1.45 H)) and whose exp2 is good
+    to 2; at each of its c / 1024 tiles its max may rise, which scales the sums by a power (its exponent's 2 |d| 2^d, under
+    1.1; exp2's 2; the product: 5 together); lanes and chunks are joined in 12 sums and 5 more such factors; log2, the
+    products and differences behind it 4 and 3 |log p|."""
+    from wfamd import ops
+    R, V = x.shape
+    c = chunk_of(R, V)
+    assert c > HELD, "this shape's chunks stay in registers"
+    p = ops.token_logprobs(x, torch.as_tensor(tokens, device="cuda"), top_k=k)
+    lp, rank, ent, ids, top = logprobs_ref(x, tokens, k)
+    u = 2.0 ** -24
+    base = c / 64 + 16 + 2 + 2 * (1 + 1.45 * ent.clamp(min=0)) + 5 * (c / 1024 + 1) + 12 + 10 + 4
+    assert torch.equal(p.ranks.cpu().long(), rank)
+    assert torch.equal(p.top_ids.cpu().long(), ids)
+    close(p.logprobs, lp, u * (base + 3 * lp.abs().nan_to_num(posinf=0.0)))
+    close(p.top_logprobs, top, u * (base[:, None] + 3 * top.abs().nan_to_num(posinf=0.0)))
+    close(p.entropy, ent, u * (2 * base * (1 + ent) + 4))  # log z's error, and that of the mean of y, which carries its factors'
+    q = ops.token_logprobs(x, None, top_k=k)
+    assert q.logprobs is None and torch.equal(q.top_ids, p.top_ids) and torch.equal(q.entropy, p.entropy)
+    z = ops.token_logprobs(x, torch.as_tensor(tokens, device="cuda"))
+    assert torch.equal(z.ranks, p.ranks) and torch.equal(z.logprobs, p.logprobs)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,vocab,ks", [(3, 300001, (1, 5, 20, 33, 64)), (2, 524321, (20,)), (700, 40003, (5,))])
+def test_long_chunks(rows, vocab, ks, dtype):
+    g = torch.Generator("cuda").manual_seed(rows)
+    x = torch.randn(rows, vocab, generator=g, device="cuda") * 3
+    x[1::2] += 8.0 * (torch.arange(vocab, device="cuda") // 8 % 64 < 19)  # the greatest in a few lanes
+    x = x.to(DT[dtype])
+    tokens = torch.randint(0, vocab, (rows,), generator=g, device="cuda").tolist()
+    for k in ks:
+        check_long(x, tokens, k)
+
+
+@pytest.mark.parametrize("kind", ["equal", "rising", "falling", "two values", "masked", "few left", "none left", "lowest", "one group", "edges"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_long_chunks_of_awkward_rows(kind, dtype):
+    g = torch.Generator("cuda").manual_seed(1)
+    R, V = 3, 300001
+    whole = torch.randn(R, V + 1, generator=g, device="cuda") * 2
+    x = whole[:, 1:]  # rows that begin off any 16-byte line
+    ramp = torch.arange(V, device="cuda") / 50000
+    if kind == "equal":
+        x.fill_(1.25)
+    elif kind == "rising":
+        x.copy_(ramp.expand(R, V))
+    elif kind == "falling":
+        x.copy_(ramp.flip(0).expand(R, V))
+    elif kind == "two values":
+        x.copy_((x > 3).float())
+    elif kind == "masked":
+        x[torch.rand(R, V, generator=g, device="cuda") < 0.999] = -math.inf
+    elif kind in ("few left", "none left"):
+        keep = x[:, 70777:70777 + (11 if kind == "few left" else 0)].clone()
+        x.fill_(-math.inf)
+        x[:, 70777:70777 + keep.shape[1]] = keep
+    elif kind == "lowest":
+        x[torch.rand(R, V, generator=g, device="cuda") < 0.9] = torch.finfo(DT[dtype]).min
+        x[2] = torch.finfo(DT[dtype]).min
+    elif kind == "one group":  # the greatest 40 next to each other
+        x[:, 100003:100043] += 30.0
+    else:  # the greatest where chunks begin and end
+        c = chunk_of(R, V)
+        for e in range(-4, 5):
+            x[:, c + e::c] += 20.0
+        x[:, :3] += 20.0
+        x[:, -3:] += 20.0
+    x = whole.to(DT[dtype])[:, 1:]
+    for k in (1, 20, 64):
+        check_long(x, [0, V - 1, 70780], k)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_long_chunks_among_nan_of_both_signs(dtype):
+    from wfamd import ops
+    g = torch.Generator("cuda").manual_seed(4)
+    R, V, k = 3, 300001, 33
+    assert chunk_of(R, V) > HELD
+    x = torch.randn(R, V, generator=g, device="cuda").to(DT[dtype])
+    bits = x.view(torch.int32 if dtype == "f32" else torch.int16)
+    bad = torch.rand(R, V, generator=g, device="cuda") < 0.5
+    bad[1] = True
+    bad[1, [5, 4700, 123456, V - 1]] = False
+    bad[2] = True
+    neg = torch.rand(R, V, generator=g, device="cuda") < 0.5
+    nan = torch.full((), math.nan, dtype=DT[dtype], device="cuda").view(bits.dtype)
+    bits[bad] = nan & (2 ** (31 if dtype == "f32" else 15) - 1)
+    bits[bad & neg] |= -2 ** (31 if dtype == "f32" else 15)
+    assert (x.isnan() == bad).all()
+    p = ops.token_logprobs(x, top_k=k)
+    want = torch.sort(x.float().nan_to_num(-math.inf), dim=1, descending=True, stable=True).indices[:, :k]
+    want[torch.arange(k, device="cuda") >= (~bad).sum(1, keepdim=True)] = -1
+    assert torch.equal(p.top_ids.long(), want) and p.top_logprobs.isnan().all() and p.entropy.isnan().all()
