@@ -427,6 +427,11 @@ def _int32_rows(name: str, n, **tensors) -> None:
             raise ValueError(f"{name}: {what} must be a contiguous int32 [{n}], got {t.dtype} {tuple(t.shape)}")
 
 
+def _too_large(name: str, **sizes) -> None:
+    """ValueError that names the size which is no 32-bit int: the C-ABI would see the bits below alone."""
+    raise ValueError(f"{name}: {', '.join(f'{what} {n}' for what, n in sizes.items() if n >> 31)} not in [0, 2^31)")
+
+
 def _table_stride(name: str, t: torch.Tensor, b: int) -> int:
     """The row stride of an int32 [b, blocks] page table whose rows are contiguous."""
     if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != b or (b and t.shape[1] > 1 and t.stride(1) != 1):
@@ -489,8 +494,11 @@ def kv_page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
         _int32_rows("kv_page_plan", free, free_pages=free_pages)
     ts = _table_stride("kv_page_plan", page_table, b)
     n = int(num_tokens)
+    page = int(page_size)
     if n < 0:
         raise ValueError(f"kv_page_plan: num_tokens {n} is negative")
+    if (b | free | n | page | page_table.shape[1]) >> 31:
+        _too_large("kv_page_plan", batch=b, free_pages=free, num_tokens=n, page_size=page, blocks=page_table.shape[1])
     pad = -n % 4 if n > 4096 else 0  # large arrays begin on 16-byte lines
     out = cached_lens.new_empty(4 * (n + pad) + b + 5)
     if pad:
@@ -501,7 +509,7 @@ def kv_page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
     ws = torch.empty(nws, dtype=torch.uint8, device=out.device) if nws else None
     base, step = out.data_ptr(), 4 * (n + pad)
     _call_on(index, "wf_kv_page_plan", (cached_lens.data_ptr(), new_lens.data_ptr(), b, free_pages.data_ptr(), free, page_table.data_ptr(),
-             ts, page_table.shape[1], int(page_size), n, base, base + step, base + 2 * step, base + 3 * step, base + 4 * step + 16,
+             ts, page_table.shape[1], page, n, base, base + step, base + 2 * step, base + 3 * step, base + 4 * step + 16,
              base + 4 * step, _ptr(ws)))
     return KVPagePlan(pages, slots, rows, pos, cu, counts)
 
@@ -585,6 +593,9 @@ def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         raise ValueError(f"rotary_embed: k must be [{T}, heads, {D}] {q.dtype} as q is, got {k.dtype} {tuple(k.shape)}")
     if positions.shape != (T,) or positions.dtype not in (torch.int64, torch.int32) or not positions.is_contiguous():
         raise ValueError(f"rotary_embed: positions must be a contiguous int32 or int64 [{T}], got {positions.dtype} {tuple(positions.shape)}")
+    Hk = 0 if k is None else k.shape[1]
+    if (T | Hq | Hk | D) >> 31:
+        _too_large("rotary_embed", tokens=T, heads=Hq, k_heads=Hk, head_dim=D)
     r = 2 * freqs.numel()
     if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or not 0 < r <= D:
         raise ValueError(f"rotary_embed: freqs must be a contiguous float64 [n], 0 < 2 n <= {D}, got {freqs.dtype} {tuple(freqs.shape)}")
@@ -597,7 +608,7 @@ def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         qo, ko = q, k
     else:
         qo = q.new_empty((T, Hq, D))
-        ko = None if k is None else q.new_empty((T, k.shape[1], D))
+        ko = None if k is None else q.new_empty((T, Hk, D))
         if q.stride(2) != 1:
             q = q.contiguous()
         if k is not None and k.stride(2) != 1:
@@ -607,7 +618,7 @@ def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         kargs, koargs = (None, 0, 0, 0), (None, 0, 0)
     else:
         ks, kos = k.stride(), ko.stride()
-        kargs, koargs = (k.data_ptr(), ks[0], ks[1], k.shape[1]), (ko.data_ptr(), kos[0], kos[1])
+        kargs, koargs = (k.data_ptr(), ks[0], ks[1], Hk), (ko.data_ptr(), kos[0], kos[1])
     _call_on(index, "wf_rotary_embed", (q.data_ptr(), qs[0], qs[1], Hq, *kargs, code, positions.data_ptr(),
              positions.dtype is torch.int64, freqs.data_ptr(), T, D, r, bool(interleaved), scale, qo.data_ptr(), qos[0], qos[1], *koargs))
     return qo, ko
@@ -649,6 +660,9 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError(f"{name}: {Hq} query heads for {Hkv} kv heads")
     ts = _table_stride(name, page_table, B)
+    cols = page_table.shape[1]
+    if (pages | Hkv | B | Hq | cols) >> 31:
+        _too_large(name, pages=pages, kv_heads=Hkv, batch=B, heads=Hq, blocks=cols)
     if not (seq_lens.dtype is prefix_rows.dtype is prefix_lens.dtype is torch.int32 and
             seq_lens.shape == (B,) == prefix_rows.shape == prefix_lens.shape and seq_lens.is_contiguous() and
             prefix_rows.is_contiguous() and prefix_lens.is_contiguous()):
@@ -657,7 +671,6 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     if qs[2] != 1:
         q = q.contiguous()
         qs = q.stride()
-    cols = page_table.shape[1]
     out = q.new_empty((B, Hq, D))
     lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     ws = q.new_empty(_ws_bytes("wf_shared_prefix_attention_ws_bytes", code, B, Hq, Hkv, cols), dtype=torch.uint8)
@@ -687,6 +700,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"token_logprobs: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
     R, V = logits.shape
+    if (R | V) >> 31:
+        _too_large("token_logprobs", rows=R, vocabulary=V)
     k = int(top_k)
     if not 0 <= k <= min(64, V):
         raise ValueError(f"token_logprobs: top_k {k} not in [0, {min(64, V)}]")
