@@ -349,7 +349,8 @@ class BitNetDecoder:
             pass
 
     def reserve(self, b: int, n_tokens: int) -> None:
-        """Give sequence b pages for positions [0, n_tokens) (allocating only the missing blocks)."""
+        """Give sequence b pages for positions [0, n_tokens) (allocating only the missing blocks). The row of page_table is
+        written whole from the host's record (seq_pages): pages that a caller put there otherwise are lost, see map_pages."""
         need = (int(n_tokens) + 31) // 32 - len(self.seq_pages[b])
         if need <= 0:
             return

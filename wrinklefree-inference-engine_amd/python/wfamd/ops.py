@@ -482,7 +482,8 @@ def kv_page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
     free_pages (int32 ids, in order) and written into its row of page_table [B, blocks] (in place). num_tokens
     sizes the token arrays (the sum of new_lens, or a bound). `pages` / `slots` are what KVCacheManager.scatter_kv
     takes. The first counts[2] of free_pages are in use afterwards; a sequence that does not fit its table row or
-    the free list is refused whole (counts[3]) and its tokens have page -1."""
+    the free list is refused whole (counts[3]) and its tokens have page -1. A BitNetDecoder does not see what is planned
+    into its own page_table (it keeps a host record of its pages): plan into another, and hand over with map_pages."""
     index = cached_lens.get_device()
     if not index == new_lens.get_device() == free_pages.get_device() == page_table.get_device() or index < 0:
         _one_device("kv_page_plan", cached_lens=cached_lens, new_lens=new_lens, free_pages=free_pages, page_table=page_table)
