@@ -439,8 +439,10 @@ def _table_stride(name: str, t: torch.Tensor, b: int) -> int:
     return t.stride(0) if b > 1 else t.shape[1]
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a torch.cuda.Stream around it (2 us)
-_current_device = torch._C._cuda_getDevice  # what torch.cuda.current_device() returns once there is a device tensor
+# The current stream's handle without a torch.cuda.Stream around it (2 us), and what torch.cuda.current_device() returns once there is a
+# device tensor. A torch without a GPU backend has neither, and no device tensor that could get as far.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 @functools.lru_cache(maxsize=None)
