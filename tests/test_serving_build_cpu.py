@@ -1,4 +1,5 @@
-"""How the package is imported: host-only functions need no GPU."""
+"""How the library is built and the package imported: objects follow the flags, and host-only functions need no GPU."""
+import re
 import subprocess
 import sys
 from pathlib import Path
@@ -20,3 +21,29 @@ def test_ops_import_without_a_gpu_backend():
             "except ValueError as e: assert 'device tensors only' in str(e)\n"
             "else: raise AssertionError\n")
     subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+
+
+def make_rules(*args):
+    """make's data base for the package: target -> prerequisites."""
+    out = subprocess.run(["make", "-C", str(PKG), "-pn", *args], capture_output=True, text=True, timeout=60).stdout
+    return {m[1]: m[2].split() for m in re.finditer(r"^([^\s#:=%]+):(?!=)[ ]*(.*)$", out, re.M)}
+
+
+def test_objects_follow_the_flags():
+    """The Makefile holds the flags: every object, the study objects too, is older than it after a change there."""
+    rules = make_rules("all", "stamps")
+    for f in (PKG / "csrc").glob("*.hip"):
+        for at in ("build", "build/stamps"):
+            assert "Makefile" in rules[f"{at}/{f.stem}.o"] and f"csrc/{f.name}" in rules[f"{at}/{f.stem}.o"]
+        assert f"build/{f.stem}.o" in rules["lib/libwfbitnet.so"]
+
+
+def test_build_compiles_whatever_is_there(monkeypatch):
+    import __graft_entry__ as entry
+    calls = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda cmd, **kw: calls.append(cmd))
+    try:
+        entry.build()
+    except (ImportError, OSError):  # nothing built yet: the library cannot load
+        pass
+    assert any(cmd[0] == "make" and str(PKG) in cmd and "-B" in cmd for cmd in calls)
