@@ -1744,7 +1744,7 @@ int wf_decode_attention(const void* q, int q_dtype, int64_t q_sb, int64_t q_sh, 
     WF_REQUIRE(out_dtype == WF_F32 || out_dtype == WF_BF16 || out_dtype == WF_F16, "decode_attention: bad out dtype");
     WF_REQUIRE(kv_st % 8 == 0 && kv_sh % 8 == 0 && kv_sb % 8 == 0, "decode_attention: KV strides must be multiples of 8");
     WF_REQUIRE(aligned16(k) && aligned16(v), "decode_attention: K/V must be 16-byte aligned");
-    WF_HIP(hipMemsetAsync(ws, 0, attn_cnt_bytes(B, Hkv), as_stream(stream)));  // tickets (graph-capturable)
+    clear32(ws, attn_cnt_bytes(B, Hkv) / 4, as_stream(stream));  // tickets
     return decode_attention_impl(q, q_dtype, q_sb, q_sh, k, v, kv_dtype, kv_sb, kv_sh, kv_st, k_scale, v_scale, B, Hq,
                                  Hkv, D, S, seq_lens, sm_scale, out, out_dtype, o_sb, o_sh, ws, as_stream(stream));
 }

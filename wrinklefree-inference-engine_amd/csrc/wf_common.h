@@ -29,6 +29,16 @@ inline int check_launch(const char* what) {
     return WF_OK;
 }
 
+// n words to zero on the stream, by a kernel: a captured hipMemsetAsync node has given wrong results on replays after the first.
+template <int = 0>
+__global__ void k_clear32(uint32_t* p, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = 0;
+}
+inline void clear32(void* p, int64_t n, hipStream_t st) {
+    hipLaunchKernelGGL((k_clear32<>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, static_cast<uint32_t*>(p), n);
+}
+
 // Decode attention's in-launch exchanges (k_attn_sdpa, k_attn_sdpa_mfma's split-2 sequences): codes of
 // the model's host-visible error word (wf_model_check) and the model-owned hook the launches take.
 enum { WF_ATTN_ERR_SDPA = 1, WF_ATTN_ERR_SPLIT2 = 2 };

@@ -487,7 +487,7 @@ static int quant_common(const void* x, int dtype, int64_t n, int8_t* q, float* a
     WF_REQUIRE(x && q && absmax && n > 0, "quantize: bad arguments");
     WF_REQUIRE(dtype == WF_F32 || dtype == WF_BF16 || dtype == WF_F16, "quantize: unsupported dtype %d", dtype);
     hipStream_t st = as_stream(stream);
-    WF_HIP(hipMemsetAsync(absmax, 0, sizeof(float), st));
+    clear32(absmax, 1, st);
     const int g = grid_for(n, 256, 2048);
     hipLaunchKernelGGL(k_absmax, dim3(g), dim3(256), 0, st, x, dtype, n, reinterpret_cast<unsigned*>(absmax));
     hipLaunchKernelGGL(k_quant_apply, dim3(g), dim3(256), 0, st, x, dtype, n, absmax, q, mode);

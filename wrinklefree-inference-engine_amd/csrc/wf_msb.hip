@@ -222,8 +222,8 @@ extern "C" int wf_absmax(const void* x, int dtype, int64_t n, float* out, void* 
     WF_REQUIRE(dtype == WF_F32 || dtype == WF_BF16 || dtype == WF_F16, "wf_absmax: dtype must be f32/bf16/f16");
     WF_REQUIRE(n >= 0, "wf_absmax: n < 0");
     hipStream_t st = as_stream(stream);
-    WF_HIP(hipMemsetAsync(out, 0, sizeof(float), st));
-    if (n == 0) return WF_OK;
+    clear32(out, 1, st);
+    if (n == 0) return check_launch("absmax");
     return launch_absmax(x, dtype, n, out, st);
 }
 
