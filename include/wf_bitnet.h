@@ -205,6 +205,8 @@ int wf_rotary_embed(const void* q, int64_t q_st, int64_t q_sh, int Hq, const voi
  *            stand for code * k_scale / code * v_scale; 16-byte aligned, strides multiples of 16 bytes;
  *   page_table [B][max_blocks] int32 (row stride table_stride). Lengths are cut at 32 * max_blocks. Keys on page ids
  *            outside [0, num_pages) count as absent.
+ * Scores, sums and outputs in progress have 32 bits; probabilities are rounded to bf16 for a BF16 q, and to f16 for an F16 q over one-byte
+ * codes, before they meet V (16 and 24 bits of them for an F16 q over a bf16 pool and for an F32 q).
  * A sequence without keys, or without a score above -inf, gives zeros and lse -inf. max_blocks also sizes the launch: a
  * table much wider than the sequences are long costs some idle workgroups.
  * ws: wf_shared_prefix_attention_ws_bytes(dtype, B, Hq, Hkv, max_blocks) bytes, 16-byte aligned. */

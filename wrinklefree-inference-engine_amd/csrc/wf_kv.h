@@ -21,7 +21,7 @@ __device__ __forceinline__ uint4 fp8x8_to_bf16(uint2 r) {
 // static per-layer scale): a fragment is 8 signed codes (8 bytes per lane), widened exactly -- each
 // byte biased to unsigned (xor 0x80), v_cvt_f32_ubyteN, -128, then bf16 (|code| <= 127 is
 // exact in bf16). Scales folded like FP8's.
-#ifndef WF_I8_PK  // 0: the round-5 form (hipcc folds the -128 into an integer subtract: SDWA + v_cvt_f32_i32)
+#ifndef WF_I8_PK  // 0: the earlier form (hipcc folds the -128 into an integer subtract: SDWA + v_cvt_f32_i32)
 #define WF_I8_PK 1
 #endif
 __device__ __forceinline__ uint32_t i8x2_to_bf16(uint32_t u, int sh) {

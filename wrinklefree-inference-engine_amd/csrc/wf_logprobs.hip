@@ -17,8 +17,10 @@
 //     DPP steps more. The k first groups, by (max, lower group first), hold the chunk's k first elements: an
 //     element of a later group is preceded by the maxima of k groups, each greater, or equal and further left. The
 //     wave keeps the k best groups sorted across its lanes and reads just those again at the end. k <= 64 is the wave's width.
-// Measured, vocabulary 128256 in bf16: 2048 rows with 5 alternatives 118 us, 4.5 TB/s (109 us, 4.8 TB/s, without any); 128 rows
-// with 20: 16 us and 5 of the join (the reading and summing alone 11.7); one row 6 + 5 us, latencies.
+// Rounding: 32 bits throughout, a lane's sums one logit after the other (up to a thousand for a prompt's rows) with the hardware's
+// exp2: log probabilities of 2048 rows are off by 1.3e-7 of their size (root mean square), where whole rows summed as a tree are off by 5e-8.
+// Measured, vocabulary 128256 in bf16: 2048 rows with 5 alternatives 117 us, 4.5 TB/s (109 us, 4.8 TB/s, without any); 128 rows
+// with 20: 17 us and 5 of the join (the reading and summing alone 11.7); one row 6.6 + 3.8 us, latencies.
 #include "wf_common.h"
 #include "wf_device.h"
 
@@ -121,8 +123,6 @@ struct LpList {
     }
 };
 
-// Candidates on their way to a list: packed into the wave's 64 places in LDS by a ballot and a lane count each, taken in
-// together when the places are full or at the end.
 // LDS of one wave: its accesses are in order, the compiler's too
 __device__ __forceinline__ void lp_meet() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -163,6 +163,8 @@ __device__ __forceinline__ double lp_order(double* q, int n) {
     return v;
 }
 
+// Candidates on their way to a list: packed into the wave's 64 places in LDS by a ballot and a lane count each, taken in
+// together when the places are full or at the end.
 struct LpQueue {
     double* q;
     int n;  // of the wave, in a scalar
@@ -684,7 +686,7 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
 // Chunks a row: as many waves as the device holds at once, 4096, or a few less (535 rows of 155893 with 20 alternatives: 7
 // chunks 57 us, 8 leave a second round of 184 waves, 66); more where fewer would leave a seventh of it empty. More also where
 // that makes the chunks short enough for registers, up to 6144 waves (404 rows of 55653 37 -> 30 us), or 12288 where there is
-// a second round anyway. No chunk under a tile of a wave.
+// a second round anyway. At most a chunk for every 2048 logits (V = 2049: two of them, half a tile of 16 bits each).
 static int lp_splits(int R, int V) {
     const int64_t down = 4096 / (int64_t)R, fit = R * down >= 3500 ? down : (4096 + (int64_t)R - 1) / R;
     const int64_t held = ((int64_t)V + kLpHeld - 1) / kLpHeld, want = R * held <= (R * fit > 4096 ? 12288 : 6144) ? max(fit, held) : fit;

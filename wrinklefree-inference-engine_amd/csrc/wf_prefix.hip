@@ -20,16 +20,20 @@
 // The running max is raised only when a tile passes it by 2^8 (its exchange between the four lanes of a row and
 // the rescaling of o are rare then): p <= 2^8 is as exact in bf16 and 32 bits as p <= 1.
 //
-// What bounds it: a wave loads 16 KiB (bf16) a tile for 32 rows, through the 64 bytes a cycle of its CU's L1: some 2000 cycles
-// a tile for four waves, twice the matrix and softmax work. Suffixes run at HBM's rate beside them. Measured a call, 20 query and 5 kv
-// heads, bf16, batch 128: 1024 shared keys and suffixes to 512 (88 MB) 31 us; 32768 and suffixes to 1024 (253 MB) 101 us; no
-// sharing, 1024 keys each (335 MB) 59 us, 5.6 TB/s.
+// What bounds it: the loads and the arithmetic of a prefix wave follow each other, and it is alone on its SIMD. Issuing the 16 KiB
+// (bf16) of a tile for 32 rows takes it some 1250 cycles beside the CU's three others (52 of the L1's 64 bytes a cycle), scores,
+// softmax and products 425 + 370 + 454: 2500 cycles a tile, 86 tiles a wave behind 32768 keys. (A second prefix workgroup a CU
+// loads no faster and was slower, see the launch rule.) Suffixes run at HBM's rate beside them. Measured a call, 20 query and 5 kv heads, bf16, batch 128:
+// 1024 shared keys and suffixes to 512 (88 MB) 30 us, 35 where the inputs come round too late for the 256 MB cache in front of
+// memory; 32768 and suffixes to 1024 (253 MB) 101 us; no sharing, 1024 keys each (335 MB) 59 us, 5.6 TB/s.
 //
 // Operands and rounding: scores, max, sums and o in 32 bits. The matrices are bf16, and f16 where q is f16 and the pool holds
 // one-byte codes (all of them f16 values). Where the pool is bf16, an f16 q enters as the exact sum of two bf16 terms;
 // an f32 q as three. P is rounded once to the output's type where that is the matrices' (bf16 2^-8, f16 2^-11 a
 // term at most, as much as the output's own rounding; f16 with the exponents 7 higher, so that only p < 2^-21 lose bits,
-// 2^-32 at most); else it has as many terms as q.
+// 2^-32 at most); else it has as many terms as q. What the one rounding costs: outputs off by 0.0018 (500 shared keys) to 0.0023
+// (32768) of their size (root mean square), 0.0017 of it the output's own rounding; f16 over int8 0.00028, 0.00021 of it the output's. Who wants
+// P in 32 bits passes q in f32: three terms each, at the cost given in pf_plan.
 #include "wf_common.h"
 #include "wf_device.h"
 #include "wf_kv.h"
@@ -534,11 +538,12 @@ static PfPlan pf_plan(bool one, int B, int Hq, int Hkv, int cols) {
     const int64_t rows = (int64_t)B * (Hq / Hkv), groups = (Hq / Hkv + 15) / 16;
     PfPlan p;
     // 32 rows of a q of several terms would leave one workgroup a CU its registers: 4096 shared keys 48 us (f32) and 42 (f16), 36 and
-    // 33 with 16 rows, short prefixes 33 -> 23
+    // 33 with 16 rows (a smaller batch), short prefixes 33 -> 23. 128 sequences of 20 and 5 heads over a bf16 pool, behind 4096 keys / 32768: 41 us /
+    // 101 in bf16, 46 / 231 in f16, 47 / 234 in f32 (half the rows a load serves, two and three times the products)
     p.MT = rows <= 16 || !one ? 16 : 32;
     const int64_t tiles = (rows + p.MT - 1) / p.MT;
     auto clamp = [](int64_t v, int64_t hi) { return (int)max((int64_t)1, min(min(v, hi), (int64_t)kPfMaxRecords)); };
-    // prefix ranges: one workgroup a CU. A second one reads no faster (L1, below), and its place goes to a suffix
+    // prefix ranges: one workgroup a CU. A second one reads no faster (L1: 52 bytes a cycle with one), and its place goes to a suffix
     // workgroup, whose time is HBM's: 32768 shared keys 102 us, 118 with two.
     p.NP = clamp(256 / (tiles * Hkv), (cols + kPfMinTiles - 1) / kPfMinTiles);
     p.NS = clamp(512 / ((int64_t)B * Hkv * groups), (cols + 1 + kPfMinSuffix - 1) / kPfMinSuffix);

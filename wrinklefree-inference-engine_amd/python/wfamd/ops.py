@@ -640,7 +640,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     those below prefix_lens[b] stand on the pages of row prefix_rows[b] (a negative row: no prefix), the rest on its
     own. Neighbours in the batch with the same prefix_rows and prefix_lens share its reading. Returns out [B, Hq, 128] in
     q's dtype, with return_lse=True also the log of the sum of exponentials [B, Hq] float32. A sequence of no keys
-    gives zeros and -inf."""
+    gives zeros and -inf. Probabilities are rounded to q's 16 bits before they meet V (f16 over a bf16 pool: to 16 bits of
+    mantissa); an f32 q keeps them in 32."""
     name = "shared_prefix_attention"
     index = q.get_device()
     if index < 0 or not index == k_pool.get_device() == v_pool.get_device() == page_table.get_device() == seq_lens.get_device() == \
