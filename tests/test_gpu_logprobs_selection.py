@@ -174,3 +174,24 @@ def test_long_chunks_among_nan_of_both_signs(dtype):
     want = torch.sort(x.float().nan_to_num(-math.inf), dim=1, descending=True, stable=True).indices[:, :k]
     want[torch.arange(k, device="cuda") >= (~bad).sum(1, keepdim=True)] = -1
     assert torch.equal(p.top_ids.long(), want) and p.top_logprobs.isnan().all() and p.entropy.isnan().all()
+
+
+@pytest.mark.parametrize("vocab", [1, 700, 40011, 300001])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_probabilities_stay_below_one(dtype, vocab):
+    """One logit far above the others, at any level: its log probability is at most 0, the entropy at least 0."""
+    from wfamd import ops
+    g = torch.Generator("cuda").manual_seed(vocab)
+    R = 5 if vocab > 100000 else 60
+    for below in (math.inf, 40.0, 15.0):
+        level = (torch.rand(R, 1, generator=g, device="cuda") * 200 - 100).to(DT[dtype])
+        x = (level.float() - below).to(DT[dtype]).expand(R, vocab).clone()
+        at = torch.randint(0, vocab, (R, 1), generator=g, device="cuda")
+        x.scatter_(1, at, level)
+        p = ops.token_logprobs(x, at[:, 0], top_k=1)
+        assert (p.logprobs <= 0).all() and (p.top_logprobs <= 0).all() and (p.entropy >= 0).all()
+        lp, rank, ent, ids, top = logprobs_ref(x, at[:, 0].tolist(), 1)
+        # in units of 2^-24: a lane adds 1 and c / 64 + 16 terms (90 for the longest chunk here), 40 for exponents' errors, joins and
+        # the logarithm as in check_long; 2^-16 of the small terms' sum, |log p|, for their own errors
+        close(p.logprobs, lp, 2.0 ** -24 * (90 + 40 + 3 * lp.abs()) + 2.0 ** -16 * lp.abs())
+        assert torch.equal(p.ranks.cpu().long(), rank)

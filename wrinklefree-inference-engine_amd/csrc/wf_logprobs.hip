@@ -636,10 +636,12 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LpArgs a) {
     sum.m = p.m, sum.z = p.z, sum.t = p.t;
     sum.join();
     const int rank = wave_sum_i(p.rank);
-    const float lz = log2f(sum.z), ln_z = lz * kLn2;
     const bool empty = sum.z == 0.f;  // every logit is -inf
+    // the greatest logit's own term is 1: a sum that the frames' roundings left below would make a sure token's log probability positive
+    if (sum.z < 1.f && !empty) sum.z = 1.f;
+    const float lz = log2f(sum.z), ln_z = lz * kLn2, ent = (lz - sum.t / sum.z) * kLn2;
     if (lane == 0) {
-        if (a.ent) a.ent[r] = empty ? 0.f : (lz - sum.t / sum.z) * kLn2;
+        if (a.ent) a.ent[r] = empty || ent < 0.f ? 0.f : ent;
         if (a.tok) {
             const int64_t tok = lp_token(a, r);
             const bool in = tok >= 0 && tok < a.V;
